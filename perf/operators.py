@@ -1,0 +1,448 @@
+"""Group norm with an activation, rotary positions over several axes, and masked attention: the cases that are measured.
+
+Each case is one call between two convolutions of a network that mixes convolutions with attention over the positions of
+its feature maps (image decoders, image and video encoders, text with an image prefix):
+
+group_norm  x [n, h, w, c] channels last, normalised over each group of channels and all positions, then activated.
+rotary      x [tokens, heads, head_dim] as a projection wrote it: the first rot_heads heads (queries, keys) are rotated by
+            the token's position on each axis, the others (values) are only converted.
+attention   q [batch, q_len, q_heads, d] over k, v [batch, kv_len, kv_heads, d], with a tanh cap on the scores, a bias that
+            falls with the distance, ragged cache lengths, causal, prefix and document masks.
+"""
+import math
+
+import torch
+
+own = False
+
+F32, BF16, F16 = "float32", "bfloat16", "float16"
+
+
+# ------------------------------------------------------------------------------------------------- cases
+
+
+def _group_norm(name, n, h, w, c, groups, act, x, y):
+    return {"name": name, "op": "group_norm", "n": n, "h": h, "w": w, "c": c, "groups": groups, "act": act, "x": x, "y": y}
+
+
+def _rotary(name, grid, batch, heads, rot_heads, d, section, layout, freq, x, y, far=0):
+    t, h, w = grid
+    a = [int(v) for v in section] + [0] * (3 - len(section))
+    return {"name": name, "op": "rotary", "t": t, "h": h, "w": w, "batch": batch, "heads": heads, "rot_heads": rot_heads, "d": d, "axes": len(section), "s0": a[0], "s1": a[1], "s2": a[2], "layout": layout, "freq": freq, "x": x, "y": y, "far": far}
+
+
+def _attention(name, batch, q_len, kv_len, q_heads, kv_heads, d, dtype, causal=False, cap=0.0, bias=False, ragged=False, prefix=False, documents=0, lse=False):
+    return {"name": name, "op": "attention", "batch": batch, "q_len": q_len, "kv_len": kv_len, "q_heads": q_heads, "kv_heads": kv_heads, "d": d, "dtype": dtype, "causal": causal, "cap": cap, "bias": bias, "ragged": ragged, "prefix": prefix, "documents": documents, "lse": lse}
+
+
+def listed():
+    return [
+        # the lowest level of a U-shaped network for one image: a few hundred kilobytes, latency is all
+        _group_norm("gn_8x8x256", 1, 8, 8, 256, 32, "silu", BF16, BF16),
+        # the highest level of such a network, ten channels a group, a batch of two (with and without guidance)
+        _group_norm("gn_64x64x320_b2", 2, 64, 64, 320, 32, "silu", F16, F16),
+        # the first stage of the residual network that this repository benchmarks, in the type its fp32 convolutions write
+        _group_norm("gn_56x56x256_b32_f32", 32, 56, 56, 256, 32, "relu", F32, F32),
+        # the last stage of an image decoder: one image whose activation is larger than the caches
+        _group_norm("gn_512x512x128", 1, 512, 512, 128, 32, "silu", BF16, BF16),
+        # one new token for each of eight requests, far into their contexts: time, height and width positions
+        _rotary("rotary_step_b8", (1, 1, 1), 8, 40, 40, 128, (16, 24, 24), "halves", "shared", BF16, BF16, far=1000000),
+        # four images of 32 x 32 patches: the fp32 qkv of a 1x1 convolution becomes bf16, height and width each in its own half
+        _rotary("rotary_image_qkv_f32", (1, 32, 32), 4, 48, 32, 72, (18, 18), "axis_halves", "per_axis", F32, BF16),
+        # the queries and keys of a video clip
+        _rotary("rotary_video", (21, 30, 52), 1, 48, 48, 128, (22, 21, 21), "pairs", "per_axis", BF16, BF16),
+        # one new token for each of 32 requests over ragged caches (some requests have just begun, one slot is empty)
+        _attention("attn_step_b32_4096", 32, 1, 4096, 32, 8, 128, BF16, cap=50.0, ragged=True, lse=True),
+        # a short prompt
+        _attention("attn_77_causal", 1, 77, 77, 12, 12, 64, F16, causal=True),
+        # twelve images of different sizes packed into one sequence, each seen by its own tokens only
+        _attention("attn_documents_8192", 1, 8192, 8192, 16, 16, 72, BF16, documents=12, lse=True),
+        # image prefixes that all tokens see, then text; a bias that falls with the distance
+        _attention("attn_prefix_bias_3001_b2", 2, 3001, 3001, 16, 4, 128, BF16, causal=True, bias=True, prefix=True),
+        # a long prompt with capped scores
+        _attention("attn_causal_cap_8192", 1, 8192, 8192, 32, 8, 128, BF16, causal=True, cap=30.0),
+    ]
+
+
+def _spread(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["group_norm", "rotary", "attention", "attention"])
+    if op == "group_norm":
+        groups = rng.choice([1, 4, 8, 16, 32, 32])
+        c = groups * _spread(rng, 1, 1024 // groups)
+        x = rng.choice([F32, BF16, BF16, F16])
+        y = rng.choice([x, x, F32, BF16])
+        h, w = _spread(rng, 4, 256), _spread(rng, 4, 256)
+        n = min(_spread(rng, 1, 32), max(1, (1 << 25) // (h * w * c)))
+        case = _group_norm("", n, h, w, c, groups, rng.choice(["none", "relu", "relu6", "silu", "silu", "gelu"]), x, y)
+    elif op == "rotary":
+        d = rng.choice([32, 64, 72, 80, 96, 128])
+        axes = rng.choice([1, 2, 3])
+        pairs = d // 2 if rng.random() < 0.7 else d // 4
+        first = rng.randint(1, pairs // 2) if axes > 1 else pairs
+        second = (pairs - first if axes == 2 else rng.randint(1, pairs - first - 1)) if axes > 1 else 0
+        section = [first, second, pairs - first - second][:axes]
+        q, k = rng.choice([4, 12, 16, 24]), rng.choice([1, 2, 4, 8])
+        heads = q + 2 * k
+        x = rng.choice([F32, BF16, F16])
+        y = x if x != F32 else rng.choice([F32, BF16, F16])
+        h, w = _spread(rng, 1, 64), _spread(rng, 1, 64)
+        t = _spread(rng, 1, max(1, min(64, (1 << 26) // (h * w * heads * d))))
+        case = _rotary("", (t, h, w), rng.choice([1, 1, 2, 3]), heads, rng.choice([q + k, heads]), d, section, rng.choice(["halves", "pairs", "axis_halves"]), rng.choice(["shared", "per_axis"]), x, y, far=rng.choice([0, 0, 100000, 2000000]))
+    else:
+        d = rng.choice([64, 64, 72, 80, 96, 128, 128])
+        kv_heads = rng.choice([1, 2, 4, 8, 12])
+        q_heads = kv_heads * rng.choice([1, 1, 2, 4, 8])
+        dtype = rng.choice([BF16, BF16, F16])
+        cap = rng.choice([0.0, 0.0, 20.0, 50.0])
+        bias = rng.random() < 0.3
+        lse = rng.random() < 0.4
+        kind = rng.choice(["step", "few", "prompt", "documents"])
+        if kind == "documents":
+            total = min(_spread(rng, 64, 8192), int(math.sqrt((1 << 31) / q_heads)))
+            case = _attention("", 1, total, total, q_heads, kv_heads, d, dtype, causal=rng.random() < 0.5, cap=cap, bias=bias, documents=_spread(rng, 1, 48), lse=lse)
+        else:
+            batch = _spread(rng, 1, 64) if kind == "step" else rng.choice([1, 1, 2, 4])
+            q_len = 1 if kind == "step" else _spread(rng, 2, 24) if kind == "few" else _spread(rng, 32, 4096)
+            q_len = min(q_len, int(math.sqrt((1 << 31) / (batch * q_heads))))
+            room = (1 << 28) // (batch * kv_heads * d) if kind != "prompt" else (1 << 31) // (batch * q_heads * q_len)
+            kv_len = max(q_len, min(room, _spread(rng, 16, 65536) if kind != "prompt" else q_len + rng.choice([0, 0, 1, 500])))
+            causal = rng.random() < 0.7
+            case = _attention("", batch, q_len, kv_len, q_heads, kv_heads, d, dtype, causal=causal, cap=cap, bias=bias, ragged=rng.random() < 0.6, prefix=causal and rng.random() < 0.3, lse=lse)
+    del case["name"]
+    return case
+
+
+# ------------------------------------------------------------------------------------------------ inputs
+
+
+def _type(name):
+    return getattr(torch, name)
+
+
+def _normal(g, shape, dtype, gain=1.0):
+    return (torch.randn(shape, generator=g, device="cuda") * gain).to(dtype)
+
+
+def _splits(g, total, parts):
+    """parts + 1 ascending offsets from 0: documents of different lengths, at times an empty one; the last tokens may belong to none."""
+    cuts = torch.randint(0, total + 1, (parts,), generator=g, device="cuda").sort().values
+    if parts > 3:
+        cuts[1] = cuts[0]
+    cuts[-1] = total - total // 50
+    return torch.cat([cuts.new_zeros(1), cuts.clamp(max=total - total // 50)]).to(torch.int32)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    s = {"case": case}
+    if case["op"] == "group_norm":
+        n, h, w, c = (case[k] for k in "nhwc")
+        # activations behind a convolution: each channel with a mean and a spread of its own
+        mean, spread = _normal(g, (c,), torch.float32, 0.5), torch.rand(c, generator=g, device="cuda") + 0.5
+        s["x"] = (torch.randn((n, h, w, c), generator=g, device="cuda") * spread + mean).to(_type(case["x"]))
+        s["gamma"] = 1 + _normal(g, (c,), torch.float32, 0.2)
+        s["beta"] = _normal(g, (c,), torch.float32, 0.2)
+        s["y"] = torch.empty((n, h, w, c), dtype=_type(case["y"]), device="cuda")
+        s["eps"] = 1e-5
+    elif case["op"] == "rotary":
+        t, h, w, batch = case["t"], case["h"], case["w"], case["batch"]
+        tokens = batch * t * h * w
+        s["x"] = _normal(g, (tokens, case["heads"], case["d"]), _type(case["x"]))
+        s["y"] = torch.empty(s["x"].shape, dtype=_type(case["y"]), device="cuda")
+        at = torch.arange(tokens, device="cuda") % (t * h * w)
+        axes = [at // (h * w), at // w % h, at % w]
+        axes = axes if case["axes"] == 3 else axes[1:] if case["axes"] == 2 else [at]
+        # each sequence of the batch is somewhere else in its context
+        begin = torch.randint(0, case["far"] + 1, (batch,), generator=g, device="cuda").repeat_interleave(t * h * w)
+        s["positions"] = (torch.stack(axes) + begin).to(torch.int32).contiguous()
+        s["theta"] = 10000.0
+    else:
+        b, sq, sk, hq, hk, d = (case[k] for k in ("batch", "q_len", "kv_len", "q_heads", "kv_heads", "d"))
+        dtype = _type(case["dtype"])
+        s["q"] = _normal(g, (b, sq, hq, d), dtype, 2.0)
+        s["k"] = _normal(g, (b, sk, hk, d), dtype)
+        s["v"] = _normal(g, (b, sk, hk, d), dtype)
+        s["o"] = torch.zeros((b, sq, hq, d), dtype=dtype, device="cuda")
+        s["lse"] = torch.full((b, hq, sq), -math.inf, device="cuda") if case["lse"] else None
+        s["scale"] = d**-0.5
+        s["slopes"] = 2.0 ** -(8.0 * torch.arange(1, hq + 1, device="cuda") / hq) if case["bias"] else None
+        s["kv_lens"] = s["prefix"] = s["offsets"] = None
+        if case["ragged"]:
+            s["kv_lens"] = torch.randint(1, sk + 1, (b,), generator=g, device="cuda").to(torch.int32)
+            s["kv_lens"][0] = sk
+            if b > 4:
+                s["kv_lens"][3] = 0
+        if case["prefix"]:
+            s["prefix"] = torch.randint(0, sk // 2 + 1, (b,), generator=g, device="cuda").to(torch.int32)
+        if case["documents"]:
+            s["offsets"] = _splits(g, sq, case["documents"])
+    return s
+
+
+def work(case):
+    size = {F32: 4, BF16: 2, F16: 2}
+    if case["op"] == "group_norm":
+        e = case["n"] * case["h"] * case["w"] * case["c"]
+        return {"bytes": e * (size[case["x"]] + size[case["y"]]) + 8 * case["c"], "flops": 8 * e}
+    if case["op"] == "rotary":
+        tokens = case["batch"] * case["t"] * case["h"] * case["w"]
+        e = tokens * case["heads"] * case["d"]
+        return {"bytes": e * (size[case["x"]] + size[case["y"]]) + 4 * tokens * case["axes"], "flops": 3 * e * case["rot_heads"] // case["heads"]}
+    b, sq, sk, hq, hk, d = (case[k] for k in ("batch", "q_len", "kv_len", "q_heads", "kv_heads", "d"))
+    # lengths are drawn evenly: half the cache on average; documents cut at k even places leave 2 / (k + 1) of the square
+    share = 1.0
+    if case["ragged"] and b > 1:
+        share = (1 + (b - 1) * 0.5) / b
+    pairs = b * sq * sk * share
+    if case["documents"]:
+        pairs *= 2 / (case["documents"] + 1)
+    if case["causal"]:
+        pairs *= 1 - 0.5 * sq / sk
+    flops = 4 * d * hq * pairs
+    kv = b * sk * hk * d * 2 * share
+    return {"bytes": int(2 * (2 * b * sq * hq * d + kv) + (4 * b * hq * sq if case["lse"] else 0)), "flops": int(flops)}
+
+
+# --------------------------------------------------------------------------------------------- plain form
+
+
+def _plain_group_norm(s):
+    case, x = s["case"], s["x"].float()
+    n, h, w, c = x.shape
+    v = x.reshape(n, h * w, case["groups"], c // case["groups"])
+    mean = v.double().mean(dim=(1, 3), keepdim=True).float()
+    v = v - mean
+    var = v.square().double().mean(dim=(1, 3), keepdim=True).float()
+    v = (v * torch.rsqrt(var + s["eps"])).reshape(n, h, w, c) * s["gamma"] + s["beta"]
+    act = case["act"]
+    if act == "relu":
+        v = v.clamp(min=0)
+    elif act == "relu6":
+        v = v.clamp(min=0, max=6)
+    elif act == "silu":
+        v = v / (1 + torch.exp(-v))
+    elif act == "gelu":
+        v = 0.5 * v * (1 + torch.erf(v * 0.7071067811865476))
+    return v.to(s["y"].dtype)
+
+
+def _pairs(case):
+    """For each rotated pair: its axis, its exponent of theta, and its two places in the head."""
+    section = torch.tensor([case["s0"], case["s1"], case["s2"]][: case["axes"]])
+    pairs = int(section.sum())
+    i = torch.arange(pairs)
+    ends = section.cumsum(0)
+    axis = (i[:, None] >= ends[None, :]).sum(1)
+    begin = (ends - section)[axis]
+    j = i - begin
+    power = -j.double() / section[axis] if case["freq"] == "per_axis" else -i.double() / pairs
+    if case["layout"] == "pairs":
+        u, v = 2 * i, 2 * i + 1
+    elif case["layout"] == "halves":
+        u, v = i, i + pairs
+    else:
+        u, v = 2 * begin + j, 2 * begin + section[axis] + j
+    return axis.cuda(), power.cuda(), u.cuda(), v.cuda()
+
+
+def _plain_rotary(s):
+    case = s["case"]
+    axis, power, u, v = _pairs(case)
+    angle = s["positions"][axis].double().t() * s["theta"] ** power
+    cos, sin = angle.cos().float()[:, None, :], angle.sin().float()[:, None, :]
+    y = s["x"].float()
+    r = y[:, : case["rot_heads"]]
+    a, b = r[..., u], r[..., v]
+    y = y.clone() if y is s["x"] else y
+    y[:, : case["rot_heads"], u] = a * cos - b * sin
+    y[:, : case["rot_heads"], v] = a * sin + b * cos
+    return y.to(s["y"].dtype)
+
+
+def _visible(s, device):
+    """[batch, q_len, kv_len] truth values of who sees whom, the distances, and which rows belong to a sequence."""
+    case = s["case"]
+    b, sq, sk = case["batch"], case["q_len"], case["kv_len"]
+    i, j = torch.arange(sq, device=device)[None, :, None], torch.arange(sk, device=device)[None, None, :]
+    length = s["kv_lens"][:, None, None].long() if s["kv_lens"] is not None else torch.full((b, 1, 1), sk, device=device)
+    at = i + length - sq
+    sees = (j < length).expand(b, sq, sk)
+    if s["offsets"] is not None:
+        at = i.expand(b, sq, 1)
+        inner = s["offsets"][1:].long()
+        doc = (torch.arange(sq, device=device)[:, None] >= inner[None, :]).sum(1)
+        sees = ((doc[:, None] == doc[None, :]) & (doc < inner.numel())[:, None])[None]
+    if case["causal"]:
+        early = j <= at
+        if s["prefix"] is not None:
+            early = early | (j < s["prefix"][:, None, None])
+        sees = sees & early
+    return sees, (at - j).abs()
+
+
+def _plain_attention(s):
+    case = s["case"]
+    b, sq, sk, hq, hk, d = (case[k] for k in ("batch", "q_len", "kv_len", "q_heads", "kv_heads", "d"))
+    q = s["q"].float().permute(0, 2, 1, 3).reshape(b, hk, hq // hk * sq, d)
+    k, v = (s[n].float().permute(0, 2, 1, 3) for n in "kv")
+    x = (q @ k.transpose(2, 3)).reshape(b, hk, hq // hk, sq, sk).mul_(s["scale"])
+    if case["cap"]:
+        x.div_(case["cap"]).tanh_().mul_(case["cap"])
+    sees, distance = _visible(s, x.device)
+    if s["slopes"] is not None:
+        x.sub_(s["slopes"].reshape(1, hk, hq // hk, 1, 1) * distance[:, None, None].float())
+    x.masked_fill_(~sees[:, None, None], -math.inf)
+    top = x.amax(dim=-1, keepdim=True)
+    top = torch.where(torch.isinf(top), torch.zeros_like(top), top)
+    x.sub_(top).exp_()
+    total = x.sum(dim=-1, keepdim=True)
+    o = (x.reshape(b, hk, -1, sk) @ v).reshape(b, hk, hq // hk, sq, d)
+    o = o / torch.where(total > 0, total, torch.ones_like(total))
+    o = o.reshape(b, hq, sq, d).permute(0, 2, 1, 3).to(s["o"].dtype).contiguous()
+    if s["lse"] is None:
+        return {"o": o}
+    return {"o": o, "lse": (top + total.log()).reshape(b, hq, sq)}
+
+
+# ---------------------------------------------------------------------------------------- own operators
+
+ACTS = {"none": 0, "relu": 1, "relu6": 2, "silu": 3, "gelu": 4}
+TYPES = {F32: 0, BF16: 1, F16: 2}
+LAYOUTS = {"pairs": 0, "halves": 1, "axis_halves": 2}
+FREQS = {"shared": 0, "per_axis": 1}
+
+
+def _kept(s):
+    """The descriptors, plans and workspaces that a program makes once for its shapes."""
+    from computeengine_b200 import _lib as L
+
+    case, kept = s["case"], {"lib": L}
+    kept["stream"] = torch.cuda.current_stream().cuda_stream
+    if case["op"] == "group_norm":
+        c = case["c"]
+        kept["desc"] = d = L.GroupNormDesc(n=case["n"], c=c, h=case["h"], w=case["w"], c_store=c, groups=case["groups"], eps=s["eps"], act=ACTS[case["act"]], x_type=TYPES[case["x"]], y_type=TYPES[case["y"]])
+        size = L.lib.ie_cuda_group_norm_workspace_bytes(d)
+    elif case["op"] == "rotary":
+        heads, dim = case["heads"], case["d"]
+        section = (L.C.c_int32 * 4)(case["s0"], case["s1"], case["s2"], 0)
+        kept["desc"] = d = L.RotaryDesc(tokens=s["x"].shape[0], x_token_stride=heads * dim, x_head_stride=dim, y_token_stride=heads * dim, y_head_stride=dim, pos_axis_stride=s["x"].shape[0], theta=s["theta"], heads=heads, rot_heads=case["rot_heads"], head_dim=dim, axes=case["axes"], section=section, layout=LAYOUTS[case["layout"]], freq=FREQS[case["freq"]], inverse=0, x_type=TYPES[case["x"]], y_type=TYPES[case["y"]], pos_bits=32)
+        kept["plan"] = L.RotaryPlan()
+        L.check(L.lib.ie_rotary_plan_init(d, kept["plan"]))
+        size = 0
+    else:
+        b, sq, sk, hq, hk, dim = (case[k] for k in ("batch", "q_len", "kv_len", "q_heads", "kv_heads", "d"))
+        qs, ks = (L.C.c_int64 * 3)(sq * hq * dim, hq * dim, dim), (L.C.c_int64 * 3)(sk * hk * dim, hk * dim, dim)
+        kept["desc"] = d = L.AttentionDesc(batch=b, q_len=sq, kv_len=sk, q_stride=qs, k_stride=ks, v_stride=ks, o_stride=qs, q_heads=hq, kv_heads=hk, head_dim=dim, type=TYPES[case["dtype"]], o_type=TYPES[case["dtype"]], scale=s["scale"], softcap=case["cap"])
+        at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+        kept["mask"] = m = L.AttentionMask(causal=int(case["causal"]), documents=case["documents"], kv_lens=at(s["kv_lens"]), prefix_lens=at(s["prefix"]), q_offsets=at(s["offsets"]), kv_offsets=at(s["offsets"]), slopes=at(s["slopes"]))
+        size = L.lib.ie_cuda_attention_workspace_bytes(d, m)
+    kept["workspace"] = torch.empty(max(size, 16), dtype=torch.uint8, device="cuda")
+    return kept
+
+
+def _own(s):
+    if "kept" not in s:
+        s["kept"] = _kept(s)
+    case, kept = s["case"], s["kept"]
+    L, d, ws, stream = kept["lib"], kept["desc"], kept["workspace"], kept["stream"]
+    if case["op"] == "group_norm":
+        L.check(L.lib.ie_cuda_group_norm_nhwc(d, s["x"].data_ptr(), s["gamma"].data_ptr(), s["beta"].data_ptr(), s["y"].data_ptr(), ws.data_ptr(), ws.numel(), stream))
+        return s["y"]
+    if case["op"] == "rotary":
+        L.check(L.lib.ie_cuda_rotary(d, kept["plan"], s["x"].data_ptr(), s["positions"].data_ptr(), s["y"].data_ptr(), stream))
+        return s["y"]
+    lse = s["lse"]
+    L.check(L.lib.ie_cuda_attention(d, kept["mask"], s["q"].data_ptr(), s["k"].data_ptr(), s["v"].data_ptr(), s["o"].data_ptr(), None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+    return {"o": s["o"]} if lse is None else {"o": s["o"], "lse": lse}
+
+
+def run(state):
+    if own:
+        return _own(state)
+    op = state["case"]["op"]
+    return _plain_group_norm(state) if op == "group_norm" else _plain_rotary(state) if op == "rotary" else _plain_attention(state)
+
+
+# ------------------------------------------------------------------------------------------ in 64 bits
+
+
+def _exact_group_norm(s):
+    case = s["case"]
+    n, h, w, c = s["x"].shape
+    x = s["x"].double().reshape(n, h * w, case["groups"], c // case["groups"]).transpose(1, 2)
+    flat = x.reshape(n, case["groups"], -1)
+    mean = flat.sum(-1) / flat.shape[-1]
+    var = ((flat - mean[..., None]) ** 2).sum(-1) / flat.shape[-1]
+    z = (x - mean[..., None, None]) / torch.sqrt(var + s["eps"])[..., None, None]
+    z = z.transpose(1, 2).reshape(n, h, w, c) * s["gamma"].double() + s["beta"].double()
+    zero = torch.zeros((), dtype=torch.float64, device=z.device)
+    return {
+        "none": lambda: z,
+        "relu": lambda: torch.maximum(z, zero),
+        "relu6": lambda: torch.minimum(torch.maximum(z, zero), zero + 6),
+        "silu": lambda: z * torch.sigmoid(z),
+        "gelu": lambda: z * 0.5 * torch.erfc(-z / math.sqrt(2.0)),
+    }[case["act"]]()
+
+
+def _exact_rotary(s):
+    case = s["case"]
+    section = [case["s0"], case["s1"], case["s2"]][: case["axes"]]
+    pairs, y = sum(section), s["x"].double().clone()
+    i, begin = 0, 0
+    for a, size in enumerate(section):
+        p = s["positions"][a].double()
+        for j in range(size):
+            f = s["theta"] ** (-j / size if case["freq"] == "per_axis" else -i / pairs)
+            u, v = {"pairs": (2 * i, 2 * i + 1), "halves": (i, i + pairs), "axis_halves": (2 * begin + j, 2 * begin + size + j)}[case["layout"]]
+            z = torch.complex(y[:, : case["rot_heads"], u], y[:, : case["rot_heads"], v])
+            z = z * torch.polar(torch.ones_like(p), p * f)[:, None]
+            y[:, : case["rot_heads"], u], y[:, : case["rot_heads"], v] = z.real, z.imag
+            i += 1
+        begin += size
+    return y
+
+
+def _exact_attention(s):
+    """Sequence by sequence and head by head, over the keys of that sequence only."""
+    case = s["case"]
+    b, sq, sk, hq, hk = (case[k] for k in ("batch", "q_len", "kv_len", "q_heads", "kv_heads"))
+    o = torch.zeros(s["o"].shape, dtype=torch.float64, device="cuda")
+    lse = torch.full((b, hq, sq), -math.inf, dtype=torch.float64, device="cuda")
+    if s["offsets"] is not None:
+        cut = s["offsets"].tolist()
+        parts = [(0, x, y, x, y, 0) for x, y in zip(cut, cut[1:])]
+    else:
+        lens = s["kv_lens"].tolist() if s["kv_lens"] is not None else [sk] * b
+        pre = s["prefix"].tolist() if s["prefix"] is not None else [0] * b
+        parts = [(n, 0, sq, 0, lens[n], pre[n]) for n in range(b)]
+    for n, q0, q1, k0, k1, prefix in parts:
+        if q1 == q0 or k1 == k0:
+            continue
+        far = torch.arange(q1 - q0, device="cuda")[:, None] + (k1 - k0) - (q1 - q0) - torch.arange(k1 - k0, device="cuda")[None]
+        hidden = torch.zeros_like(far, dtype=torch.bool)
+        if case["causal"]:
+            hidden = far < 0
+            hidden[:, :prefix] = False
+        for h in range(hq):
+            c = h * hk // hq
+            x = s["q"][n, q0:q1, h].double() @ s["k"][n, k0:k1, c].double().t() * s["scale"]
+            if case["cap"]:
+                x = case["cap"] * torch.tanh(x / case["cap"])
+            if s["slopes"] is not None:
+                x = x - s["slopes"][h].double() * far.abs()
+            x = x.masked_fill(hidden, -math.inf)
+            l = torch.logsumexp(x, dim=1)
+            lse[n, h, q0:q1] = l
+            p = torch.exp(x - torch.where(torch.isinf(l), 0.0, l)[:, None])
+            o[n, q0:q1, h] = p @ s["v"][n, k0:k1, c].double()
+    return {"o": o} if s["lse"] is None else {"o": o, "lse": lse}
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"group_norm": _exact_group_norm, "rotary": _exact_rotary, "attention": _exact_attention}[case["op"]](s)
