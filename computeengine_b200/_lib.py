@@ -25,6 +25,10 @@ IE_PAD = {"NOTSET": 0, "": 0, "VALID": 1, "SAME_UPPER": 2, "SAME_LOWER": 3}
 IE_ACT_NONE, IE_ACT_RELU, IE_ACT_RELU6 = 0, 1, 2
 IE_Y_F32_NHWC, IE_Y_F32_NCHW, IE_Y_BF16X2_NHWC = 0, 1, 2
 IE_TILE_FILL, IE_TILE_DEFAULT = 0, 1
+IE_DT_F32, IE_DT_BF16, IE_DT_F16, IE_DT_BF16X2 = 0, 1, 2, 3
+IE_ACT_SILU, IE_ACT_GELU = 3, 4  # group normalization only
+IE_ROTARY_PAIRS, IE_ROTARY_HALVES, IE_ROTARY_AXIS_HALVES = 0, 1, 2
+IE_ROTARY_FREQ_SHARED, IE_ROTARY_FREQ_PER_AXIS = 0, 1
 
 _i64 = C.c_int64
 _i32 = C.c_int32
@@ -62,6 +66,38 @@ class QAddParams(C.Structure):
 class ConvPlan(C.Structure):
     _fields_ = [(n, _i32) for n in ("bn", "bk_bytes", "m_sub", "stages", "resident_weights",
                                     "out_bufs", "row_band", "grid", "a_tiled")]
+
+
+class GroupNormDesc(C.Structure):
+    _fields_ = [(n, _i64) for n in ("n", "c", "h", "w", "c_store", "groups")] + \
+               [("eps", C.c_float), ("act", _i32), ("x_type", _i32), ("y_type", _i32)]
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [(n, _i64) for n in ("tokens", "x_token_stride", "x_head_stride",
+                                    "y_token_stride", "y_head_stride", "pos_axis_stride")] + \
+               [("theta", C.c_double)] + \
+               [(n, _i32) for n in ("heads", "rot_heads", "head_dim", "axes")] + \
+               [("section", _i32 * 4)] + \
+               [(n, _i32) for n in ("layout", "freq", "inverse", "x_type", "y_type", "pos_bits")]
+
+
+class RotaryPlan(C.Structure):
+    _fields_ = [("turns", C.c_uint64 * 128), ("axis", C.c_uint8 * 128), ("head_dim", _i32),
+                ("axes", _i32), ("section", _i32 * 4), ("layout", _i32), ("freq", _i32),
+                ("pairs", _i32), ("theta", C.c_double)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [(n, _i64) for n in ("batch", "q_len", "kv_len")] + \
+               [(n, _i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "o_stride")] + \
+               [(n, _i32) for n in ("q_heads", "kv_heads", "head_dim", "type", "o_type")] + \
+               [("scale", C.c_float), ("softcap", C.c_float)]
+
+
+class AttentionMask(C.Structure):
+    _fields_ = [("causal", _i32), ("documents", _i32)] + \
+               [(n, _p) for n in ("kv_lens", "prefix_lens", "q_offsets", "kv_offsets", "slopes")]
 
 
 class CudaConvError(RuntimeError):
@@ -125,6 +161,14 @@ def _load() -> C.CDLL:
         "ie_cuda_gemm_f32_workspace_bytes": (C.c_size_t, [_i64, _i64, _i64, _i32, _i32]),
         "ie_cuda_gemm_f32": (C.c_int, [_i64, _i64, _i64, _i32, _i32, C.c_float, C.c_float, _p,
                                        _p, _p, _i32, _p, _p, C.c_size_t, _p]),
+        "ie_cuda_group_norm_workspace_bytes": (C.c_size_t, [P(GroupNormDesc)]),
+        "ie_cuda_group_norm_nhwc": (C.c_int, [P(GroupNormDesc), _p, _p, _p, _p, _p, C.c_size_t,
+                                              _p]),
+        "ie_rotary_plan_init": (C.c_int, [P(RotaryDesc), P(RotaryPlan)]),
+        "ie_cuda_rotary": (C.c_int, [P(RotaryDesc), P(RotaryPlan), _p, _p, _p, _p]),
+        "ie_cuda_attention_workspace_bytes": (C.c_size_t, [P(AttentionDesc), P(AttentionMask)]),
+        "ie_cuda_attention": (C.c_int, [P(AttentionDesc), P(AttentionMask), _p, _p, _p, _p, _p,
+                                        _p, C.c_size_t, _p]),
         "ie_cuda_f32x2_maxpool2d": (C.c_int, [_p, _p] + [_i64] * 7 + [_p]),
     }
     for name, (res, args) in sig.items():

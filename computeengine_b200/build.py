@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -48,13 +49,28 @@ def _run(cmd):
 
 
 def build_cuda(force: bool = False) -> Path:
-    sources = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) \
+    """Each .cu is compiled to its own object (in parallel), then linked."""
+    units = sorted(CSRC.glob("*.cu"))
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) \
         + [ROOT / "include" / "ie_cuda_conv.h"]
-    if not force and _newer(LIB, sources):
+    if not force and _newer(LIB, units + headers):
         return LIB
+    BUILD_DIR.mkdir(exist_ok=True)
+
+    def compile_unit(unit: Path) -> Path:
+        obj, deps = BUILD_DIR / (unit.stem + ".o"), BUILD_DIR / (unit.stem + ".d")
+        read = [unit, *headers]
+        if deps.exists():  # what the last compilation of this unit read
+            read = [Path(f) for f in deps.read_text().replace("\\\n", " ").split()[1:]]
+            read = [f for f in read if ROOT in f.parents or not f.exists()]
+        if force or not all(f.exists() for f in read) or not _newer(obj, read):
+            _run([nvcc(), *NVCC_FLAGS, "-MMD", "-MF", deps, "-c", "-o", obj, unit])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=len(units)) as pool:
+        objects = list(pool.map(compile_unit, units))
     cuda_lib = Path(nvcc()).resolve().parent.parent / "lib64"
-    _run([nvcc(), *NVCC_FLAGS, "-shared", "-o", LIB, CSRC / "ie_cuda_conv.cu",
-          "-Xlinker", f"-rpath={cuda_lib}"])
+    _run([nvcc(), *ARCH, "-shared", "-o", LIB, *objects, "-Xlinker", f"-rpath={cuda_lib}"])
     return LIB
 
 

@@ -11,23 +11,29 @@ names, argument meanings and error codes for the CUDA backend:
 * ``QLinearConv2DOp`` -- the int8-quantized form the reference only plans
   (quant_plugins.h:7-22 is a stub): uint8/int8 activations, per-channel int8
   weights, int32 bias, fused requantize + ReLU/ReLU6.
+* ``GroupNormOp``, ``RotaryOp``, ``AttentionOp`` -- what runs between two
+  convolutions of a network that mixes them with attention over the positions
+  of a feature map (no counterpart in the reference); channels last.
 * ``OpRegistry`` + ``register_cuda_ops`` -- registration with the reference's
   AlreadyExists behaviour (op_registry.cpp:23-32).
 
-Tensors are torch tensors on a CUDA device (NCHW).  There is no CPU fallback:
+Tensors are torch tensors on a CUDA device (NCHW unless an op says channels
+last).  There is no CPU fallback:
 a CPU tensor is an InvalidArgument, and the module fails to import when the
 CUDA library is not built.
 """
 from __future__ import annotations
 
 import enum
+import math
 from dataclasses import dataclass, field
 from typing import Callable, Dict, List, Optional
 
 import torch
 
 from . import _lib
-from ._lib import ConvDesc, ConvShape, Q8Params, lib
+from ._lib import (AttentionDesc, AttentionMask, ConvDesc, ConvShape, GroupNormDesc, Q8Params,
+                   RotaryDesc, RotaryPlan, lib)
 
 
 class Code(enum.IntEnum):
@@ -388,6 +394,298 @@ class QLinearConv2DOp(Op):
         return st
 
 
+# ----------------------------------------- blocks between convolutions
+
+_DTYPES = {torch.float32: _lib.IE_DT_F32, torch.bfloat16: _lib.IE_DT_BF16,
+           torch.float16: _lib.IE_DT_F16}
+
+
+def _number(attrs, key, default):
+    v = attrs.get(key, default)
+    if isinstance(v, bool) or not isinstance(v, (int, float)) or not math.isfinite(v):
+        return default, Status.error(Code.InvalidArgument, f"attribute '{key}' must be a finite number")
+    return float(v), OK
+
+
+def _choice(attrs, key, table, default):
+    v = attrs.get(key, default)
+    if v not in table:
+        return None, Status.error(Code.InvalidArgument, f"unsupported {key}: {v}")
+    return table[v], OK
+
+
+def _one_device(tensors, op_name) -> Status:
+    """Every given tensor on the same CUDA device."""
+    device = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            return Status.error(Code.InvalidArgument, f"{op_name}: tensors must be on a CUDA device")
+        if device is not None and t.device != device:
+            return Status.error(Code.InvalidArgument, f"{op_name}: tensors are on several devices")
+        device = t.device
+    return OK
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class GroupNormOp(Op):
+    """Group normalization with an activation, channels last.
+
+    Inputs [x], [x, gamma] or [x, gamma, beta]: x [n, h, w, c] fp32, bf16 or
+    fp16, gamma and beta fp32 [c].  Attributes: ``groups`` (required),
+    ``epsilon`` (1e-5), ``activation`` ("NONE", "RELU", "RELU6", "SILU",
+    "GELU"), ``dtype`` (torch dtype of the output, x's by default).
+    """
+
+    ACTIVATIONS = {"NONE": _lib.IE_ACT_NONE, "RELU": _lib.IE_ACT_RELU, "RELU6": _lib.IE_ACT_RELU6,
+                   "SILU": _lib.IE_ACT_SILU, "GELU": _lib.IE_ACT_GELU}
+
+    def __init__(self):
+        self.groups, self.eps, self.act, self.dtype = 1, 1e-5, _lib.IE_ACT_NONE, None
+
+    def configure(self, attrs: dict) -> Status:
+        g = attrs.get("groups")
+        if isinstance(g, bool) or not isinstance(g, int) or g <= 0:
+            return Status.error(Code.InvalidArgument, "attribute 'groups' must be a positive int")
+        self.groups = g
+        self.eps, st = _number(attrs, "epsilon", 1e-5)
+        if st and self.eps < 0:
+            st = Status.error(Code.InvalidArgument, "epsilon must not be negative")
+        if not st:
+            return st
+        self.act, st = _choice(attrs, "activation", self.ACTIVATIONS, "NONE")
+        if not st:
+            return st
+        self.dtype, st = _choice(attrs, "dtype", {None: None, **{d: d for d in _DTYPES}}, None)
+        return st
+
+    def forward(self, inputs, outputs, context=None) -> Status:
+        if not 1 <= len(inputs) <= 3 or len(outputs) != 1:
+            return Status.error(Code.InvalidArgument, "GroupNorm expects one to three inputs and one output")
+        x, gamma, beta = (list(inputs) + [None, None])[:3]
+        if x is None:
+            return Status.error(Code.InvalidArgument, "null tensor or buffer")
+        st = _one_device((x, gamma, beta), "GroupNorm")
+        if not st:
+            return st
+        if x.dtype not in _DTYPES:
+            return Status.error(Code.Unsupported, f"GroupNorm: unsupported dtype {x.dtype}")
+        if x.dim() != 4:
+            return Status.error(Code.InvalidArgument, "GroupNorm expects a 4D channels-last tensor")
+        n, h, w, c = (int(v) for v in x.shape)
+        for t in (gamma, beta):
+            if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != (c,)):
+                return Status.error(Code.InvalidArgument, "GroupNorm gamma and beta must be fp32 [C]")
+        x = x.contiguous()
+        gamma, beta = (t if t is None else t.contiguous() for t in (gamma, beta))
+        y = torch.empty(x.shape, dtype=self.dtype or x.dtype, device=x.device)
+        d = GroupNormDesc(n=n, c=c, h=h, w=w, c_store=c, groups=self.groups, eps=self.eps,
+                          act=self.act, x_type=_DTYPES[x.dtype], y_type=_DTYPES[y.dtype])
+        with torch.cuda.device(x.device):
+            need = int(lib.ie_cuda_group_norm_workspace_bytes(d))
+            ws = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+            st = _from_abi(lib.ie_cuda_group_norm_nhwc(d, x.data_ptr(), _ptr(gamma), _ptr(beta),
+                                                       y.data_ptr(), _ptr(ws), need,
+                                                       _stream_handle()))
+        if st:
+            outputs[0] = y
+        return st
+
+
+class RotaryOp(Op):
+    """Rotary positions over up to four axes.
+
+    Inputs [x, positions]: x [tokens, heads, head_dim] fp32, bf16 or fp16
+    (heads contiguous, any other strides), positions int32 or int64
+    [axes, tokens].  Attributes: ``section`` (pairs per axis, required),
+    ``layout`` ("PAIRS", "HALVES", "AXIS_HALVES"), ``frequencies`` ("SHARED",
+    "PER_AXIS"), ``theta`` (10000), ``rot_heads`` (the first heads, all by
+    default; the others are copied), ``inverse``, ``dtype`` of the output.
+    """
+
+    LAYOUTS = {"PAIRS": _lib.IE_ROTARY_PAIRS, "HALVES": _lib.IE_ROTARY_HALVES,
+               "AXIS_HALVES": _lib.IE_ROTARY_AXIS_HALVES}
+    FREQUENCIES = {"SHARED": _lib.IE_ROTARY_FREQ_SHARED, "PER_AXIS": _lib.IE_ROTARY_FREQ_PER_AXIS}
+
+    def __init__(self):
+        self.section, self.rot_heads, self.dtype = [], None, None
+        self.layout, self.freq, self.theta, self.inverse = _lib.IE_ROTARY_HALVES, 0, 10000.0, False
+        self._plans: Dict[int, RotaryPlan] = {}  # by head_dim: the frequencies
+
+    def configure(self, attrs: dict) -> Status:
+        section, st = _int_list(attrs, "section")
+        if not st:
+            return st
+        if not section or len(section) > 4:
+            return Status.error(Code.InvalidArgument, "attribute 'section' must hold 1 to 4 ints")
+        self.section = section
+        self.layout, st = _choice(attrs, "layout", self.LAYOUTS, "HALVES")
+        if not st:
+            return st
+        self.freq, st = _choice(attrs, "frequencies", self.FREQUENCIES, "SHARED")
+        if not st:
+            return st
+        self.theta, st = _number(attrs, "theta", 10000.0)
+        if not st:
+            return st
+        r = attrs.get("rot_heads")
+        if r is not None and (isinstance(r, bool) or not isinstance(r, int)):
+            return Status.error(Code.InvalidArgument, "attribute 'rot_heads' must be an int")
+        self.rot_heads, self.inverse = r, bool(attrs.get("inverse", False))
+        self.dtype, st = _choice(attrs, "dtype", {None: None, **{d: d for d in _DTYPES}}, None)
+        self._plans = {}
+        return st
+
+    def forward(self, inputs, outputs, context=None) -> Status:
+        if len(inputs) != 2 or len(outputs) != 1:
+            return Status.error(Code.InvalidArgument, "Rotary expects two inputs and one output")
+        x, pos = inputs
+        if x is None or pos is None:
+            return Status.error(Code.InvalidArgument, "null tensor or buffer")
+        st = _one_device((x, pos), "Rotary")
+        if not st:
+            return st
+        if x.dtype not in _DTYPES or pos.dtype not in (torch.int32, torch.int64):
+            return Status.error(Code.Unsupported, f"Rotary: unsupported dtypes {x.dtype}, {pos.dtype}")
+        if x.dim() != 3 or tuple(pos.shape) != (len(self.section), x.shape[0]):
+            return Status.error(Code.InvalidArgument,
+                                "Rotary expects x [tokens, heads, head_dim] and positions [axes, tokens]")
+        if x.stride(2) != 1:
+            x = x.contiguous()
+        if pos.stride(1) != 1:
+            pos = pos.contiguous()
+        y = torch.empty(x.shape, dtype=self.dtype or x.dtype, device=x.device)
+        heads, dim = int(x.shape[1]), int(x.shape[2])
+        d = RotaryDesc(tokens=x.shape[0], x_token_stride=x.stride(0), x_head_stride=x.stride(1),
+                       y_token_stride=y.stride(0), y_head_stride=y.stride(1),
+                       pos_axis_stride=pos.stride(0), theta=self.theta, heads=heads,
+                       rot_heads=heads if self.rot_heads is None else self.rot_heads, head_dim=dim,
+                       axes=len(self.section), layout=self.layout, freq=self.freq,
+                       inverse=int(self.inverse), x_type=_DTYPES[x.dtype], y_type=_DTYPES[y.dtype],
+                       pos_bits=64 if pos.dtype == torch.int64 else 32)
+        for i, s in enumerate(self.section):
+            d.section[i] = s
+        plan = self._plans.get(dim)
+        if plan is None:
+            plan = RotaryPlan()
+            st = _from_abi(lib.ie_rotary_plan_init(d, plan))
+            if not st:
+                return st
+            self._plans[dim] = plan
+        with torch.cuda.device(x.device):
+            st = _from_abi(lib.ie_cuda_rotary(d, plan, x.data_ptr(), pos.data_ptr(), y.data_ptr(),
+                                              _stream_handle()))
+        if st:
+            outputs[0] = y
+        return st
+
+
+class AttentionOp(Op):
+    """Attention with a tanh cap, a distance bias and causal, prefix, length
+    and document masks.
+
+    Inputs [q, k, v], then optionally kv_lens, prefix_lens, q_offsets,
+    kv_offsets and slopes in this order (None for one that is not given): q
+    [batch, q_len, q_heads, head_dim], k and v [batch, kv_len, kv_heads,
+    head_dim], bf16 or fp16 (head_dim contiguous, any other strides); slopes
+    fp32 [q_heads], the others int32.  q_offsets and kv_offsets [documents + 1]
+    pack documents into one batch row.  Attributes: ``scale`` (head_dim^-0.5),
+    ``softcap`` (0: none), ``causal``.  outputs[0] receives o, a second output
+    the log-sum-exp [batch, q_heads, q_len].  Rows that see no key, and rows
+    that belong to no document, are zero (log-sum-exp -inf).
+    """
+
+    def __init__(self):
+        self.scale, self.softcap, self.causal = None, 0.0, False
+
+    def configure(self, attrs: dict) -> Status:
+        self.scale = None
+        if attrs.get("scale") is not None:
+            self.scale, st = _number(attrs, "scale", 1.0)
+            if not st:
+                return st
+        self.softcap, st = _number(attrs, "softcap", 0.0)
+        if st and self.softcap < 0:
+            st = Status.error(Code.InvalidArgument, "softcap must not be negative")
+        if not st:
+            return st
+        c = attrs.get("causal", False)
+        if not isinstance(c, (bool, int)):
+            return Status.error(Code.InvalidArgument, "attribute 'causal' must be a bool")
+        self.causal = bool(c)
+        return OK
+
+    def forward(self, inputs, outputs, context=None) -> Status:
+        if not 3 <= len(inputs) <= 8 or len(outputs) not in (1, 2):
+            return Status.error(Code.InvalidArgument,
+                                "Attention expects three to eight inputs and one or two outputs")
+        q, k, v, lens, prefix, q_off, kv_off, slopes = (list(inputs) + [None] * 5)[:8]
+        if q is None or k is None or v is None:
+            return Status.error(Code.InvalidArgument, "null tensor or buffer")
+        st = _one_device((q, k, v, lens, prefix, q_off, kv_off, slopes), "Attention")
+        if not st:
+            return st
+        if q.dtype not in (torch.bfloat16, torch.float16):
+            return Status.error(Code.Unsupported, f"Attention: unsupported dtype {q.dtype}")
+        if any(t.dim() != 4 for t in (q, k, v)) or k.shape != v.shape \
+                or k.dtype != q.dtype or v.dtype != q.dtype \
+                or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
+            return Status.error(Code.InvalidArgument,
+                                "Attention expects q [batch, q_len, q_heads, head_dim] and k, v "
+                                "[batch, kv_len, kv_heads, head_dim] of one dtype")
+        batch, q_len, q_heads, dim = (int(s) for s in q.shape)
+        documents = 0
+        if q_off is not None or kv_off is not None:
+            if q_off is None or kv_off is None or q_off.dim() != 1 or q_off.shape != kv_off.shape \
+                    or q_off.numel() < 2:
+                return Status.error(Code.InvalidArgument,
+                                    "Attention q_offsets and kv_offsets must be [documents + 1]")
+            documents = q_off.numel() - 1
+        for t, shape in ((lens, (batch,)), (prefix, (documents or batch,)), (q_off, None),
+                         (kv_off, None)):
+            if t is not None and (t.dtype != torch.int32 or (shape and tuple(t.shape) != shape)):
+                return Status.error(Code.InvalidArgument,
+                                    "Attention lengths and offsets must be int32, one per sequence")
+        if slopes is not None and (slopes.dtype != torch.float32
+                                   or tuple(slopes.shape) != (q_heads,)):
+            return Status.error(Code.InvalidArgument, "Attention slopes must be fp32 [q_heads]")
+        q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
+        lens, prefix, q_off, kv_off, slopes = (t if t is None else t.contiguous()
+                                               for t in (lens, prefix, q_off, kv_off, slopes))
+        # rows of no document are left as they were by the kernels
+        o = (torch.zeros if documents else torch.empty)(q.shape, dtype=q.dtype, device=q.device)
+        lse = None
+        if len(outputs) == 2:
+            lse = torch.full((batch, q_heads, q_len), -math.inf, dtype=torch.float32,
+                             device=q.device)
+        d = AttentionDesc(batch=batch, q_len=q_len, kv_len=k.shape[1], q_heads=q_heads,
+                          kv_heads=k.shape[2], head_dim=dim, type=_DTYPES[q.dtype],
+                          o_type=_DTYPES[q.dtype],
+                          scale=dim ** -0.5 if self.scale is None else self.scale,
+                          softcap=self.softcap)
+        for i in range(3):
+            d.q_stride[i], d.k_stride[i] = q.stride(i), k.stride(i)
+            d.v_stride[i], d.o_stride[i] = v.stride(i), o.stride(i)
+        m = AttentionMask(causal=int(self.causal), documents=documents, kv_lens=_ptr(lens),
+                          prefix_lens=_ptr(prefix), q_offsets=_ptr(q_off), kv_offsets=_ptr(kv_off),
+                          slopes=_ptr(slopes))
+        with torch.cuda.device(q.device):
+            need = int(lib.ie_cuda_attention_workspace_bytes(d, m))
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            st = _from_abi(lib.ie_cuda_attention(d, m, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                                 o.data_ptr(), _ptr(lse), _ptr(ws), need,
+                                                 _stream_handle()))
+        if st:
+            outputs[0] = o
+            if lse is not None:
+                outputs[1] = lse
+        return st
+
+
 class OpRegistry:
     """OpRegistry (reference src/core/ops/op_registry.h:15-30)."""
 
@@ -416,11 +714,12 @@ class OpRegistry:
 
 
 def register_cuda_ops(registry: OpRegistry) -> Status:
-    """Registers the CUDA convolution ops (the reference registers Conv2D and
-    DepthwiseConv2D at op_registry.cpp:76-80).  Fails with AlreadyExists if an
+    """Registers the CUDA ops (the reference registers Conv2D and
+    DepthwiseConv2D at op_registry.cpp:76-80; the others are this backend's).  Fails with AlreadyExists if an
     op type is taken, so call it before any builtin registration."""
     for name, cls in (("Conv2D", Conv2DOp), ("DepthwiseConv2D", DepthwiseConv2DOp),
-                      ("QLinearConv2D", QLinearConv2DOp)):
+                      ("QLinearConv2D", QLinearConv2DOp), ("GroupNorm", GroupNormOp),
+                      ("Rotary", RotaryOp), ("Attention", AttentionOp)):
         st = registry.register_op(name, cls)
         if not st:
             return st

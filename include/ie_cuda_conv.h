@@ -432,6 +432,159 @@ int ie_cuda_gemm_f32(int64_t m, int64_t n, int64_t k, int32_t trans_a, int32_t t
                      int32_t c_mode, float* y, void* workspace, size_t workspace_bytes,
                      void* stream);
 
+/* ------------------------------------------- blocks between convolutions
+ * What a network that mixes convolutions with attention over the positions of
+ * a feature map runs between two convolutions: group normalization with an
+ * activation, rotary positions, attention.  No counterpart in the reference
+ * (its Transformer ops are stubs).  A feature map [n, h, w, c] is h * w tokens
+ * of c channels, so the fp32 NHWC output of a 1x1 convolution is the q, k, v
+ * these read, and their BF16X2 outputs are the split input
+ * ie_cuda_conv2d_bf16x3 reads.  Calls are asynchronous on the stream, keep
+ * nothing between calls and can be captured; tensors live on the current
+ * device.  Inputs may not overlap outputs unless an entry says so. */
+
+/* Element types.  IE_DT_BF16X2 is the split form of IE_Y_BF16X2_NHWC: bf16
+ * [hi plane | lo plane] per pixel, standing for hi + lo. */
+enum { IE_DT_F32 = 0, IE_DT_BF16 = 1, IE_DT_F16 = 2, IE_DT_BF16X2 = 3 };
+
+/* Activations of ie_cuda_group_norm_nhwc beyond IE_ACT_*: x / (1 + exp(-x))
+ * and x / 2 * (1 + erf(x / sqrt(2))).  The convolutions reject them. */
+enum { IE_ACT_SILU = 3, IE_ACT_GELU = 4 };
+
+/* Group normalization of a channels-last tensor: for image n and group g of
+ * c / groups consecutive channels,
+ *   y = act((x - mean[n, g]) / sqrt(var[n, g] + eps) * gamma[c] + beta[c])
+ * with mean and var (divided by the count) over the group's channels and all
+ * h * w positions.  Tensors are [n, h, w, c_store] (BF16X2: 2 * c_store bf16
+ * per pixel); channels c .. c_store - 1 of x are ignored and of y are written
+ * as zeros.  Statistics and arithmetic are fp32, each output is rounded once. */
+typedef struct ie_group_norm_desc {
+  int64_t n, c, h, w;
+  int64_t c_store; /* channels per stored pixel, >= c; a multiple of 16 for BF16X2 */
+  int64_t groups;  /* divides c */
+  float eps;       /* >= 0 */
+  int32_t act;     /* IE_ACT_NONE .. IE_ACT_GELU */
+  int32_t x_type, y_type; /* IE_DT_* */
+} ie_group_norm_desc;
+
+/* gamma, beta: fp32 [c] or NULL (1 and 0).  y may be x when the types are
+ * equal.  workspace must hold ie_cuda_group_norm_workspace_bytes(desc) bytes
+ * (16-byte aligned; 0 for most sizes, then it may be NULL); its contents need
+ * not be kept, calls that overlap on the GPU need one each.  Any alignment of
+ * x and y to their element is accepted; 16-byte aligned pointers with c_store
+ * a multiple of 8 run at full speed. */
+size_t ie_cuda_group_norm_workspace_bytes(const ie_group_norm_desc* desc);
+int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const float* gamma,
+                            const float* beta, void* y, void* workspace, size_t workspace_bytes,
+                            void* stream);
+
+/* Rotary positions over up to 4 axes (for instance time, height, width).
+ * Pair i of a head belongs to axis a, the first section[0] pairs to axis 0 and
+ * so on; P = sum of section, 2 * P <= head_dim.  With j the index of the pair
+ * within its axis, its frequency is
+ *   IE_ROTARY_FREQ_SHARED    theta^(-i / P)
+ *   IE_ROTARY_FREQ_PER_AXIS  theta^(-j / section[a])
+ * and the pair (u, v) of a token at position pos[a] becomes
+ *   (u cos t - v sin t, u sin t + v cos t),   t = pos[a] * frequency
+ * (inverse: -t, which is also the gradient's rotation).  The pair's elements:
+ *   IE_ROTARY_PAIRS          2i, 2i + 1
+ *   IE_ROTARY_HALVES         i, i + P
+ *   IE_ROTARY_AXIS_HALVES    b + j, b + section[a] + j with b twice the number
+ *                            of pairs of the axes before a
+ * Angles are taken modulo one turn in fixed point (frequencies rounded to
+ * 2^-64 turns), so far positions lose nothing: at position 2^32 an angle is
+ * still within 2^-32 turns before its sine and cosine are taken in fp32. */
+enum { IE_ROTARY_PAIRS = 0, IE_ROTARY_HALVES = 1, IE_ROTARY_AXIS_HALVES = 2 };
+enum { IE_ROTARY_FREQ_SHARED = 0, IE_ROTARY_FREQ_PER_AXIS = 1 };
+
+typedef struct ie_rotary_desc {
+  int64_t tokens;
+  int64_t x_token_stride, x_head_stride; /* elements; a head is contiguous */
+  int64_t y_token_stride, y_head_stride;
+  int64_t pos_axis_stride; /* elements between the axes of positions */
+  double theta;            /* > 0 */
+  int32_t heads;           /* heads of x and y */
+  int32_t rot_heads;       /* the first of them are rotated, the others (v) converted */
+  int32_t head_dim;        /* <= 256 */
+  int32_t axes;            /* 1 .. 4 */
+  int32_t section[4];      /* pairs per axis, >= 0 */
+  int32_t layout;          /* IE_ROTARY_PAIRS .. */
+  int32_t freq;            /* IE_ROTARY_FREQ_* */
+  int32_t inverse;
+  int32_t x_type, y_type;  /* IE_DT_F32, IE_DT_BF16, IE_DT_F16 */
+  int32_t pos_bits;        /* 32 or 64: signed positions [axes][tokens] */
+} ie_rotary_desc;
+
+/* The frequencies of a desc as turns per position (host memory, made once per
+ * head layout; reads head_dim, axes, section, layout, freq and theta). */
+typedef struct ie_rotary_plan {
+  uint64_t turns[128]; /* frequency / (2 pi), in 2^-64 turns */
+  uint8_t axis[128];
+  int32_t head_dim, axes, section[4], layout, freq, pairs;
+  double theta;
+} ie_rotary_plan;
+int ie_rotary_plan_init(const ie_rotary_desc* desc, ie_rotary_plan* plan);
+
+/* x [tokens, heads, head_dim] -> y, elements that are not rotated converted.
+ * y may be x when types and strides are equal (then only rotated elements are
+ * written).  plan must come from a desc with the same head layout. */
+int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const void* x,
+                   const void* positions, void* y, void* stream);
+
+/* Attention of q [batch, q_len, q_heads, head_dim] over k, v
+ * [batch, kv_len, kv_heads, head_dim]; query head h reads kv head
+ * h * kv_heads / q_heads.
+ *   s = scale * q.k;  softcap > 0: s = softcap * tanh(s / softcap)
+ *   slopes:  s -= slopes[h] * |p - j|
+ *   o = softmax over the visible keys j of s, times v;  lse = log sum exp s
+ * p is the query's place among its keys: the queries are the last q_len of the
+ * sequence's keys, p = i + (length - q_len).  A key is visible when it belongs
+ * to the query's sequence and, if causal, j <= p or j < prefix_lens. */
+typedef struct ie_attention_desc {
+  int64_t batch, q_len, kv_len;
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* batch, token, head; elements */
+  int32_t q_heads, kv_heads; /* kv_heads divides q_heads */
+  int32_t head_dim;          /* 1 .. 128, contiguous */
+  int32_t type;              /* q, k, v: IE_DT_BF16 or IE_DT_F16 */
+  int32_t o_type;            /* type, or IE_DT_BF16X2 for IE_DT_BF16: the lo plane of a token
+                                lies o_stride[1] / 2 elements behind its hi plane */
+  float scale;
+  float softcap; /* 0: none */
+} ie_attention_desc;
+
+/* Which keys a query sees; all pointers are device memory and may be NULL.
+ *   kv_lens      [batch] keys of each sequence (0 .. kv_len), kv_len without it
+ *   prefix_lens  [batch] (or [documents]) keys from the sequence's start that
+ *                every query of it sees; needs causal
+ *   documents    packed sequences in one batch row (batch must be 1): document
+ *                r has the queries q_offsets[r] .. q_offsets[r + 1] - 1 and the
+ *                keys kv_offsets[r] .. kv_offsets[r + 1] - 1, offsets ascending
+ *                [documents + 1]; kv_lens must be NULL
+ *   slopes       [q_heads] fp32
+ * A query that sees no key gets o = 0 and lse = -inf.  Rows of o and lse that
+ * belong to no document are left as they were.  Keys and values behind a
+ * sequence's length may hold anything.  Values outside the ranges above are
+ * clamped to them. */
+typedef struct ie_attention_mask {
+  int32_t causal;
+  int32_t documents;
+  const int32_t* kv_lens;
+  const int32_t* prefix_lens;
+  const int32_t* q_offsets;
+  const int32_t* kv_offsets;
+  const float* slopes;
+} ie_attention_mask;
+
+/* mask may be NULL (every key visible).  lse: fp32 [batch, q_heads, q_len] or
+ * NULL.  workspace must hold ie_cuda_attention_workspace_bytes(desc, mask)
+ * bytes (256-byte aligned, 0 for prompts, then it may be NULL); its contents need not be
+ * kept, calls that overlap on the GPU need one each. */
+size_t ie_cuda_attention_workspace_bytes(const ie_attention_desc* desc,
+                                         const ie_attention_mask* mask);
+int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* mask, const void* q,
+                      const void* k, const void* v, void* o, float* lse, void* workspace,
+                      size_t workspace_bytes, void* stream);
+
 /* Tile plan of the last implicit-GEMM launch issued on the calling host thread
  * (performance introspection; no counterpart in the reference).  row_band is 1
  * when the stride-1 row-band mode ran: tiles of whole output rows, one input
