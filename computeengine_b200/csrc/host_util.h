@@ -190,6 +190,9 @@ inline int encode_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dty
   return IE_OK;
 }
 
+// Reads and clears the device error word of ie_cuda_attention.cu's kernels.
+int take_attention_error(unsigned int* code);
+
 inline int num_sms() {
   static int sms = [] {
     int dev = 0, v = 148;

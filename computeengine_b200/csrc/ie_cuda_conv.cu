@@ -1,6 +1,7 @@
 // C ABI of the sm_100a Conv2D forward backend (declared in
 // include/ie_cuda_conv.h).  One translation unit: the kernels are included
-// here so the device-side error word is a single object.
+// here so their device-side error word is a single object (the attention
+// kernels of ie_cuda_attention.cu have one of their own).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -769,7 +770,10 @@ int ie_cuda_take_device_error(uint32_t* code) {
   const unsigned int zero = 0;
   e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
   if (e != cudaSuccess) return fail(IE_RUNTIME, "clear error word: %s", cudaGetErrorString(e));
-  if (code != nullptr) *code = v;
+  unsigned int other = 0;  // the attention kernels' word
+  const int rc = take_attention_error(&other);
+  if (rc != IE_OK) return rc;
+  if (code != nullptr) *code = v != 0 ? v : other;
   return IE_OK;
 }
 
