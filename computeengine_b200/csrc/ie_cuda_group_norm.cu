@@ -2,6 +2,7 @@
 // include/ie_cuda_conv.h): argument checks, choice of the kernel, launch.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -44,29 +45,219 @@ int check_group_norm(const ie_group_norm_desc* d) {
   return IE_OK;
 }
 
-using Launch = void (*)(const GroupNormArgs&, dim3, cudaStream_t);
+constexpr int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
+
+constexpr int64_t kSms = 148;
+constexpr int64_t kSmemPerSm = 227 * 1024;
+// Bytes of x that the two-kernel path normalizes per pair of launches: with
+// the y they become they stay in the 126 MB L2 between the two reads.
+constexpr int64_t kWaveBytes = 48 << 20;
+
+int64_t item_bytes(int x_type, int v) {
+  return int64_t{v} * element_bytes(x_type) * (x_type == IE_DT_BF16X2 ? 2 : 1);
+}
+
+struct Plan {
+  int v = 1;
+  bool cluster = false;
+  int range_groups = 1, ranges = 1;  // channel ranges of whole groups
+  int blocks = 1;                    // per image and range: cluster size, or statistics blocks
+  int64_t smem = 0;
+  // two-kernel path: (image, range) units of one pair of launches
+  int64_t wave_images = 1;
+  int wave_ranges = 1;
+  int apply_blocks = 1;
+  int64_t workspace = 0;
+};
+
+// Whether ranges of g groups begin and end on vectors of v channels.
+bool range_fits(const ie_group_norm_desc* d, int64_t g, int v) {
+  return d->groups % g == 0 && (g == d->groups || g * (d->c / d->groups) % v == 0);
+}
+
+// The choice between one kernel that holds x in shared memory and two that
+// read it twice, and the split of the work, by an estimate of the time:
+// blocks run in waves over the SMs, each wave costs about 3 us of latencies
+// and moves its bytes at the SM's share of the memory bandwidth (44 bytes/ns);
+// pieces of a pixel narrower than 128 bytes waste part of each DRAM access.
+Plan plan_for(const ie_group_norm_desc* d, int v) {
+  Plan best;
+  const int64_t cg = d->c / d->groups, pixels = d->h * d->w;
+  const int64_t xb = item_bytes(d->x_type, 1), yb = item_bytes(d->y_type, 1);
+  best.v = v;
+  double best_ns = 1e30;
+  for (int64_t g = 1; v > 1 && g <= d->groups; ++g) {
+    if (!range_fits(d, g, v)) continue;
+    const int64_t ranges = d->groups / g;
+    const int64_t stored = d->c_store - (ranges - 1) * g * cg;  // of the last range
+    const int64_t cols = ceil_div(std::max(stored, g * cg), v);
+    if (cols > kGnThreads) break;
+    const int64_t rows = kGnThreads / cols;
+    const double segment = static_cast<double>(g * cg * xb);
+    const double waste = segment < 32 ? 2.0 : segment < 64 ? 1.5 : segment < 128 ? 1.15 : 1.0;
+    for (int blocks = 1; blocks <= 16; blocks *= 2) {
+      const int64_t share = ceil_div(pixels, blocks);
+      const int64_t held = ceil_div(share, rows) * kGnThreads * item_bytes(d->x_type, v);
+      const int64_t smem = held + (2 * v + 1) * kGnThreads * 4 + 16 * g + 32;
+      if (smem > kSmemPerSm || (blocks > 1 && share * (blocks - 1) >= pixels)) continue;
+      const int64_t per_sm = smem + 1024 <= kSmemPerSm / 2 ? 2 : 1;
+      const int64_t total = d->n * ranges * blocks;
+      const int64_t waves = ceil_div(total, kSms * per_sm);
+      const double resident = static_cast<double>(std::min(per_sm, ceil_div(total, kSms)));
+      const double bytes = static_cast<double>(share * g * cg * (xb + yb));
+      double ns = static_cast<double>(waves) *
+                  (3000.0 + (blocks > 8 ? 1500.0 : blocks > 1 ? 500.0 : 0.0) +
+                   waste * bytes * resident / 44.0);
+      if (ns < best_ns) {
+        best_ns = ns;
+        best.cluster = true;
+        best.range_groups = static_cast<int>(g);
+        best.ranges = static_cast<int>(ranges);
+        best.blocks = blocks;
+        best.smem = smem;
+      }
+    }
+  }
+  // two kernels: a second launch, x read again from L2 (about twice as fast)
+  const double two_ns = 8000.0 + static_cast<double>(d->n * pixels * d->c_store) *
+                                     (1.5 * static_cast<double>(xb) + static_cast<double>(yb)) /
+                                     (44.0 * kSms);
+  if (best.cluster && best_ns <= two_ns) return best;
+  best.cluster = false;
+  // ranges: whole pixels if the threads cover them and the image fits a wave,
+  // else the narrowest range of at least 256 bytes
+  const int64_t image = pixels * d->c_store * xb;
+  best.range_groups = static_cast<int>(d->groups);
+  const bool whole = ceil_div(d->c, v) <= kGnThreads && image <= kWaveBytes;
+  if (!whole) {
+    best.range_groups = 0;
+    for (int64_t g = 1; g <= d->groups; ++g) {
+      if (!range_fits(d, g, v)) continue;
+      // several groups only within the threads' columns
+      if (best.range_groups > 0 && ceil_div(g * cg, v) > kGnThreads) break;
+      best.range_groups = static_cast<int>(g);
+      if (g * cg * xb >= 256) break;
+    }
+  }
+  const int64_t channels = best.range_groups * cg;
+  best.ranges = static_cast<int>(d->groups / best.range_groups);
+  const int64_t rows = std::max<int64_t>(1, kGnThreads / ceil_div(channels, v));
+  if (image <= kWaveBytes) {
+    best.wave_images = std::min(d->n, std::max<int64_t>(1, kWaveBytes / image));
+    best.wave_ranges = best.ranges;
+  } else {
+    best.wave_images = 1;
+    best.wave_ranges = static_cast<int>(
+        std::min<int64_t>(best.ranges, std::max<int64_t>(1, kWaveBytes * best.ranges / image)));
+  }
+  const int64_t units = best.wave_images * best.wave_ranges;
+  best.blocks = static_cast<int>(
+      std::max<int64_t>(1, std::min(ceil_div(2 * kSms, units), ceil_div(pixels, kGnBatch * rows))));
+  best.apply_blocks = static_cast<int>(
+      std::max<int64_t>(1, std::min(ceil_div(4 * kSms, units), ceil_div(pixels, 4 * rows))));
+  best.smem = (2 * v + 1) * kGnThreads * 4 + 8 * best.range_groups;
+  best.workspace = units * best.blocks * best.range_groups * static_cast<int64_t>(sizeof(float2));
+  return best;
+}
+
+// Vectors of 16 bytes of x where pixels, pointers and ranges allow it.
+int vector_width(const ie_group_norm_desc* d) {
+  const int v = d->x_type == IE_DT_F32 ? 4 : 8;
+  if (d->c_store % v != 0) return 1;
+  // a group wider than the threads' columns must be a range of its own
+  const int64_t cg = d->c / d->groups;
+  for (int64_t g = 1; g <= d->groups; ++g) {
+    if (!range_fits(d, g, v)) continue;
+    if (ceil_div(g * cg, v) <= kGnThreads || (g == 1 && cg % v == 0)) return v;
+    break;
+  }
+  return 1;
+}
+
+template <class Kernel>
+int allow_smem(Kernel kernel, int64_t smem, bool wide_cluster) {
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       static_cast<int>(smem));
+  if (e == cudaSuccess && wide_cluster) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  }
+  return e == cudaSuccess ? IE_OK : fail(IE_RUNTIME, "group_norm: %s", cudaGetErrorString(e));
+}
+
+template <int XT, int YT, int V>
+int launch_cluster(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
+  auto kernel = group_norm_cluster_kernel<XT, YT, V>;
+  const int rc = allow_smem(kernel, p.smem, p.blocks > 8);
+  if (rc != IE_OK) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(images * p.ranges * p.blocks));
+  cfg.blockDim = dim3(kGnThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(p.smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = static_cast<unsigned>(p.blocks);
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(IE_RUNTIME, "group_norm: %s", cudaGetErrorString(e));
+  }
+  return check_launch("group_norm");
+}
+
+template <int XT, int YT, int V>
+int launch_two(GroupNormArgs a, const Plan& p, int64_t images, cudaStream_t s) {
+  auto stats = group_norm_stats_kernel<XT, V>;
+  auto apply = group_norm_apply_kernel<XT, YT, V>;
+  const int64_t apply_smem = 8 * p.range_groups;
+  int rc = allow_smem(stats, p.smem, false);
+  if (rc == IE_OK) rc = allow_smem(apply, apply_smem, false);
+  for (int64_t i = 0; rc == IE_OK && i < images; i += p.wave_images) {
+    a.first_image = i;
+    const int64_t wave = std::min(p.wave_images, images - i);
+    for (int r = 0; rc == IE_OK && r < p.ranges; r += p.wave_ranges) {
+      a.first_range = r;
+      a.launch_ranges = std::min(p.wave_ranges, p.ranges - r);
+      const int64_t units = wave * a.launch_ranges;
+      stats<<<static_cast<unsigned>(units * p.blocks), kGnThreads, p.smem, s>>>(a);
+      rc = check_launch("group_norm statistics");
+      if (rc != IE_OK) break;
+      apply<<<static_cast<unsigned>(units * p.apply_blocks), kGnThreads, apply_smem, s>>>(
+          a, p.apply_blocks);
+      rc = check_launch("group_norm");
+    }
+  }
+  return rc;
+}
 
 template <int XT, int YT>
-void launch_simple(const GroupNormArgs& a, dim3 grid, cudaStream_t s) {
-  group_norm_simple_kernel<XT, YT><<<grid, 256, 0, s>>>(a);
+int launch(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
+  constexpr int V = XT == IE_DT_F32 ? 4 : 8;
+  if (p.v == 1) return launch_two<XT, YT, 1>(a, p, images, s);
+  return p.cluster ? launch_cluster<XT, YT, V>(a, p, images, s)
+                   : launch_two<XT, YT, V>(a, p, images, s);
 }
 
 template <int XT>
-Launch simple_for(int y_type) {
+int launch(int y_type, const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
   switch (y_type) {
-    case IE_DT_F32: return launch_simple<XT, IE_DT_F32>;
-    case IE_DT_BF16: return launch_simple<XT, IE_DT_BF16>;
-    case IE_DT_F16: return launch_simple<XT, IE_DT_F16>;
-    default: return launch_simple<XT, IE_DT_BF16X2>;
+    case IE_DT_F32: return launch<XT, IE_DT_F32>(a, p, images, s);
+    case IE_DT_BF16: return launch<XT, IE_DT_BF16>(a, p, images, s);
+    case IE_DT_F16: return launch<XT, IE_DT_F16>(a, p, images, s);
+    default: return launch<XT, IE_DT_BF16X2>(a, p, images, s);
   }
 }
 
-Launch simple_for(int x_type, int y_type) {
+int launch(int x_type, int y_type, const GroupNormArgs& a, const Plan& p, int64_t images,
+           cudaStream_t s) {
   switch (x_type) {
-    case IE_DT_F32: return simple_for<IE_DT_F32>(y_type);
-    case IE_DT_BF16: return simple_for<IE_DT_BF16>(y_type);
-    case IE_DT_F16: return simple_for<IE_DT_F16>(y_type);
-    default: return simple_for<IE_DT_BF16X2>(y_type);
+    case IE_DT_F32: return launch<IE_DT_F32>(y_type, a, p, images, s);
+    case IE_DT_BF16: return launch<IE_DT_BF16>(y_type, a, p, images, s);
+    case IE_DT_F16: return launch<IE_DT_F16>(y_type, a, p, images, s);
+    default: return launch<IE_DT_BF16X2>(y_type, a, p, images, s);
   }
 }
 
@@ -74,7 +265,12 @@ Launch simple_for(int x_type, int y_type) {
 
 extern "C" {
 
-size_t ie_cuda_group_norm_workspace_bytes(const ie_group_norm_desc*) { return 0; }
+size_t ie_cuda_group_norm_workspace_bytes(const ie_group_norm_desc* desc) {
+  if (check_group_norm(desc) != IE_OK) return 0;
+  // what unaligned tensors need, too
+  return static_cast<size_t>(
+      std::max(plan_for(desc, vector_width(desc)).workspace, plan_for(desc, 1).workspace));
+}
 
 int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const float* gamma,
                             const float* beta, void* y, void* workspace, size_t workspace_bytes,
@@ -85,15 +281,35 @@ int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const
   if (x == y && desc->x_type != desc->y_type) {
     return fail(IE_INVALID_ARGUMENT, "GroupNorm in place needs equal element types");
   }
-  (void)workspace;
-  (void)workspace_bytes;
-  GroupNormArgs a{x, gamma, beta, y, desc->h * desc->w, static_cast<int>(desc->c),
-                  static_cast<int>(desc->c_store), static_cast<int>(desc->groups), desc->act,
-                  desc->eps};
-  simple_for(desc->x_type, desc->y_type)(
-      a, dim3(static_cast<unsigned>(desc->groups), static_cast<unsigned>(desc->n)),
-      as_stream(stream));
-  return check_launch("group_norm");
+  int v = vector_width(desc);
+  const uintptr_t y_bytes =
+      std::min<uintptr_t>(16, static_cast<uintptr_t>(v) * element_bytes(desc->y_type));
+  if (reinterpret_cast<uintptr_t>(x) % 16 != 0 || reinterpret_cast<uintptr_t>(y) % y_bytes != 0) {
+    v = 1;
+  }
+  const Plan p = plan_for(desc, v);
+  if (p.workspace > 0 &&
+      (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 != 0 ||
+       workspace_bytes < static_cast<size_t>(p.workspace))) {
+    return fail(IE_INVALID_ARGUMENT, "GroupNorm needs %lld bytes of 16-byte aligned workspace",
+                static_cast<long long>(p.workspace));
+  }
+  GroupNormArgs a{};
+  a.x = x;
+  a.gamma = gamma;
+  a.beta = beta;
+  a.y = y;
+  a.pixels = desc->h * desc->w;
+  a.c = static_cast<int>(desc->c);
+  a.c_store = static_cast<int>(desc->c_store);
+  a.groups = static_cast<int>(desc->groups);
+  a.act = desc->act;
+  a.eps = desc->eps;
+  a.range_groups = p.range_groups;
+  a.ranges = p.ranges;
+  a.blocks = p.blocks;
+  a.partial = static_cast<float2*>(workspace);
+  return launch(desc->x_type, desc->y_type, a, p, desc->n, as_stream(stream));
 }
 
 }  // extern "C"

@@ -1,6 +1,7 @@
 // C ABI of the rotary positions (declared in include/ie_cuda_conv.h).
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <cstdint>
@@ -40,28 +41,61 @@ int check_head_layout(const ie_rotary_desc* d, int* pairs) {
   return IE_OK;
 }
 
-using Launch = void (*)(const RotaryArgs&, cudaStream_t);
+using Launch = void (*)(const RotaryArgs&, dim3, cudaStream_t);
+
+template <int XT, int YT, int W, int CW>
+void launch(const RotaryArgs& a, dim3 grid, cudaStream_t s) {
+  const size_t smem = sizeof(float2) * a.block_tokens * a.pairs;
+  rotary_kernel<XT, YT, W, CW><<<grid, 256, smem, s>>>(a);
+}
 
 template <int XT, int YT>
-void launch_simple(const RotaryArgs& a, cudaStream_t s) {
-  rotary_simple_kernel<XT, YT><<<static_cast<unsigned>(a.tokens), 128, 0, s>>>(a);
+Launch launch_for(int w, bool copy8) {
+  switch (w) {
+    case 8: return copy8 ? launch<XT, YT, 8, 8> : launch<XT, YT, 8, 1>;
+    case 4: return copy8 ? launch<XT, YT, 4, 8> : launch<XT, YT, 4, 1>;
+    case 2: return copy8 ? launch<XT, YT, 2, 8> : launch<XT, YT, 2, 1>;
+    default: return copy8 ? launch<XT, YT, 1, 8> : launch<XT, YT, 1, 1>;
+  }
 }
 
 template <int XT>
-Launch simple_for(int y_type) {
+Launch launch_for(int y_type, int w, bool copy8) {
   switch (y_type) {
-    case IE_DT_F32: return launch_simple<XT, IE_DT_F32>;
-    case IE_DT_BF16: return launch_simple<XT, IE_DT_BF16>;
-    default: return launch_simple<XT, IE_DT_F16>;
+    case IE_DT_F32: return launch_for<XT, IE_DT_F32>(w, copy8);
+    case IE_DT_BF16: return launch_for<XT, IE_DT_BF16>(w, copy8);
+    default: return launch_for<XT, IE_DT_F16>(w, copy8);
   }
 }
 
-Launch simple_for(int x_type, int y_type) {
+Launch launch_for(int x_type, int y_type, int w, bool copy8) {
   switch (x_type) {
-    case IE_DT_F32: return simple_for<IE_DT_F32>(y_type);
-    case IE_DT_BF16: return simple_for<IE_DT_BF16>(y_type);
-    default: return simple_for<IE_DT_F16>(y_type);
+    case IE_DT_F32: return launch_for<IE_DT_F32>(y_type, w, copy8);
+    case IE_DT_BF16: return launch_for<IE_DT_BF16>(y_type, w, copy8);
+    default: return launch_for<IE_DT_F16>(y_type, w, copy8);
   }
+}
+
+// Whether both tensors can be read and written in vectors of w elements.
+bool vectors_of(const ie_rotary_desc* d, const void* x, const void* y, int w) {
+  const uintptr_t bytes_x = std::min(16, w * element_bytes(d->x_type));
+  const uintptr_t bytes_y = std::min(16, w * element_bytes(d->y_type));
+  return reinterpret_cast<uintptr_t>(x) % bytes_x == 0 &&
+         reinterpret_cast<uintptr_t>(y) % bytes_y == 0 && d->x_token_stride % w == 0 &&
+         d->x_head_stride % w == 0 && d->y_token_stride % w == 0 && d->y_head_stride % w == 0;
+}
+
+// The widest unit that every run of pairs, the elements behind them and the
+// strides are a multiple of.
+int unit_width(const ie_rotary_desc* d, const void* x, const void* y, int pairs) {
+  for (int w : {8, 4, 2}) {
+    bool fits = vectors_of(d, x, y, w) && pairs % w == 0 && (d->head_dim - 2 * pairs) % w == 0;
+    if (d->layout == IE_ROTARY_AXIS_HALVES) {
+      for (int s = 0; s < d->axes; ++s) fits = fits && d->section[s] % w == 0;
+    }
+    if (fits) return w;
+  }
+  return 1;
 }
 
 }  // namespace
@@ -115,7 +149,9 @@ int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const
   if (desc->tokens <= 0 || desc->heads <= 0) {
     return fail(IE_INVALID_ARGUMENT, "Rotary expects positive dimensions");
   }
-  if (desc->tokens > INT_MAX) return fail(IE_UNSUPPORTED, "Rotary takes at most 2^31 - 1 tokens");
+  if (desc->tokens > INT_MAX || desc->heads > 65535) {
+    return fail(IE_UNSUPPORTED, "Rotary takes at most 2^31 - 1 tokens of 2^16 - 1 heads");
+  }
   if (desc->rot_heads < 0 || desc->rot_heads > desc->heads) {
     return fail(IE_INVALID_ARGUMENT, "rot_heads must be between 0 and heads");
   }
@@ -164,7 +200,30 @@ int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const
   }
   std::memcpy(a.turns, plan->turns, sizeof(a.turns));
   std::memcpy(a.axis, plan->axis, sizeof(a.axis));
-  simple_for(desc->x_type, desc->y_type)(a, as_stream(stream));
+  const int w = unit_width(desc, x, y, pairs);
+  const bool copy8 = desc->head_dim % 8 == 0 && vectors_of(desc, x, y, 8);
+  a.units = SmallDivisor::of(static_cast<uint32_t>(pairs / w));
+  a.copies = SmallDivisor::of(static_cast<uint32_t>(copy8 ? desc->head_dim / 8 : desc->head_dim));
+  // Tokens per block: about eight units a thread, as long as that leaves four
+  // blocks per SM; heads are shared out among blocks when there are fewer
+  // tokens than SMs (one token per block then).
+  constexpr int64_t kSms = 148, kMaxItems = 1 << 15;
+  const int64_t units = std::max<int64_t>(1, int64_t{desc->rot_heads} * (pairs / w));
+  int64_t block_tokens = std::min<int64_t>(8, std::max<int64_t>(1, 2048 / units));
+  block_tokens = std::max<int64_t>(1, std::min(block_tokens, desc->tokens / (4 * kSms)));
+  // a block's units stay below 2^16 (SmallDivisor)
+  int64_t shares = 1;
+  if (block_tokens == 1) {
+    shares = std::max((units + kMaxItems - 1) / kMaxItems,
+                      std::min((units + 255) / 256, (kSms + desc->tokens - 1) / desc->tokens));
+  }
+  a.block_tokens = static_cast<int>(block_tokens);
+  a.block_heads = static_cast<int>((desc->rot_heads + shares - 1) / shares);
+  if (a.block_heads == 0) a.block_heads = 1;
+  a.head_count = SmallDivisor::of(static_cast<uint32_t>(a.block_heads));
+  const dim3 grid(static_cast<unsigned>((desc->tokens + block_tokens - 1) / block_tokens),
+                  static_cast<unsigned>(shares));
+  launch_for(desc->x_type, desc->y_type, w, copy8)(a, grid, as_stream(stream));
   return check_launch("rotary");
 }
 

@@ -469,10 +469,11 @@ typedef struct ie_group_norm_desc {
 
 /* gamma, beta: fp32 [c] or NULL (1 and 0).  y may be x when the types are
  * equal.  workspace must hold ie_cuda_group_norm_workspace_bytes(desc) bytes
- * (16-byte aligned; 0 for most sizes, then it may be NULL); its contents need
- * not be kept, calls that overlap on the GPU need one each.  Any alignment of
- * x and y to their element is accepted; 16-byte aligned pointers with c_store
- * a multiple of 8 run at full speed. */
+ * (16-byte aligned); images that fit the shared memory of a cluster use none
+ * of it (then it may be NULL).  Its contents need not be kept; calls that
+ * overlap on the GPU need one each.  Any alignment of x and y to their element
+ * is accepted; 16-byte aligned pointers with c_store a multiple of 8 run at
+ * full speed. */
 size_t ie_cuda_group_norm_workspace_bytes(const ie_group_norm_desc* desc);
 int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const float* gamma,
                             const float* beta, void* y, void* workspace, size_t workspace_bytes,
