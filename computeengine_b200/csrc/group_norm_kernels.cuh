@@ -16,6 +16,8 @@
 
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "element_types.cuh"
 
 namespace ie_cuda {
@@ -38,7 +40,7 @@ struct GroupNormArgs {
   int launch_ranges;    // ranges of this launch
 };
 
-constexpr int kGnThreads = 512;
+constexpr int kGnThreads = 256;
 constexpr int kGnBatch = 8;  // pixels per exact mean
 
 __device__ __forceinline__ float activate(float v, int act) {
@@ -178,16 +180,19 @@ __device__ __forceinline__ float warp_sum(float v) {
 // Joins the threads' channels into the groups of the block's channel range:
 // out[g] = (mean, sum of squared differences).  Thread t holds the channels
 // (t % cols) * V .. of the range, rows = threads per column; scratch holds
-// (2 * V + 1) * threads floats.  (A single group wider than the threads' columns: every
-// thread's channels are that group's.)
+// (2 * V + 2) * threads floats.  First every channel's rows are joined in
+// slices, so that all threads take part; then a warp joins a group's channels.
+// (A single group wider than the threads' columns: every thread's channels are
+// that group's.)
 template <int V>
 __device__ __forceinline__ void join_threads(const Running<V>& r, int cols, int rows,
                                              int group_channels, int groups, float* scratch,
                                              float2* out) {
   const int width = cols * V;
-  float* mean = scratch;
-  float* m2 = scratch + rows * width;
-  float* count = m2 + rows * width;
+  float* mean = scratch;                   // [rows][width]
+  float* m2 = mean + V * kGnThreads;       // [rows][width]
+  float* count = m2 + V * kGnThreads;      // [rows][cols]
+  float* joined = count + kGnThreads;      // [slices][cols]
   const int t = threadIdx.x;
   if (t < cols * rows) {
     const int at = t / cols * width + t % cols * V;
@@ -199,24 +204,48 @@ __device__ __forceinline__ void join_threads(const Running<V>& r, int cols, int 
     count[t] = static_cast<float>(r.n);
   }
   __syncthreads();
+  // slices of whole rows; a slice's result replaces its first row
+  const int slices = max(1, min(rows, kGnThreads / width));
+  const int deep = (rows + slices - 1) / slices;
+  for (int i = t; i < slices * width; i += kGnThreads) {
+    const int slice = i / width, ch = i - slice * width, col = ch / V;
+    const int from = slice * deep, to = min(rows, from + deep);
+    float n = 0.0f, s = 0.0f, q = 0.0f;
+    for (int k = from; k < to; ++k) {
+      n += count[k * cols + col];
+      s += count[k * cols + col] * mean[k * width + ch];
+    }
+    const float mu = n > 0.0f ? s / n : 0.0f;
+    for (int k = from; k < to; ++k) {
+      const float w = count[k * cols + col], d = mean[k * width + ch] - mu;
+      if (w > 0.0f) q += m2[k * width + ch] + w * d * d;
+    }
+    if (from < rows) {
+      mean[from * width + ch] = mu;
+      m2[from * width + ch] = q;
+    }
+    joined[slice * cols + col] = n;  // the same from each of the column's channels
+  }
+  __syncthreads();
   const int lane = t & 31;
   for (int g = t >> 5; g < groups; g += kGnThreads / 32) {
-    const int entries = rows * group_channels;
-    float n = 0.0f, s = 0.0f;
+    const int entries = slices * group_channels;
+    float n = 0.0f, s = 0.0f, q = 0.0f;
     for (int i = lane; i < entries; i += 32) {
-      const int row = i / group_channels;
-      const int at = row * width + g * group_channels + (i - row * group_channels);
-      n += count[at / V];
-      s += count[at / V] * mean[at];
+      const int slice = i / group_channels, ch = g * group_channels + i - slice * group_channels;
+      const float w = joined[slice * cols + ch / V];
+      if (w > 0.0f) {
+        n += w;
+        s += w * mean[slice * deep * width + ch];
+      }
     }
     n = warp_sum(n);
     const float mu = warp_sum(s) / n;
-    float q = 0.0f;
     for (int i = lane; i < entries; i += 32) {
-      const int row = i / group_channels;
-      const int at = row * width + g * group_channels + (i - row * group_channels);
-      const float d = mean[at] - mu;
-      if (count[at / V] > 0.0f) q += m2[at] + count[at / V] * d * d;
+      const int slice = i / group_channels, ch = g * group_channels + i - slice * group_channels;
+      const float w = joined[slice * cols + ch / V];
+      const float d = w > 0.0f ? mean[slice * deep * width + ch] - mu : 0.0f;
+      if (w > 0.0f) q += m2[slice * deep * width + ch] + w * d * d;
     }
     q = warp_sum(q);
     if (lane == 0) out[g] = make_float2(mu, q);
@@ -238,23 +267,39 @@ struct Range {
   }
 };
 
-// Normalizes, activates and stores one item; channels past c become zero.
-template <int YT, int V>
+// Normalizes, activates and stores one item; channels past c become zero
+// (mul and add are zero there, but x may hold anything).
+template <int YT, int V, int ACT>
 __device__ __forceinline__ void finish_item(const GroupNormArgs& a, float (&f)[V],
-                                            const float (&mul)[V], const float (&sub)[V],
-                                            const float (&add)[V], int64_t pixel, int c) {
+                                            const float (&mul)[V], const float (&add)[V],
+                                            int64_t pixel, int c) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    f[e] = c + e < a.c ? activate(fmaf(f[e] - sub[e], mul[e], add[e]), a.act) : 0.0f;
+  for (int e = 0; e < V; ++e) f[e] = activate(fmaf(f[e], mul[e], add[e]), ACT);
+  if (c + V > a.c) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = c + e < a.c ? f[e] : 0.0f;
   }
   store_item<YT, V>(a.y, channel_at<YT>(pixel, a.c_store, c), a.c_store, f);
+}
+
+// Runs body(std::integral_constant<int, act>) for the activation, so that the
+// choice is made once and not per element.
+template <class Body>
+__device__ __forceinline__ void with_activation(int act, const Body& body) {
+  switch (act) {
+    case IE_ACT_RELU: body(std::integral_constant<int, IE_ACT_RELU>()); break;
+    case IE_ACT_RELU6: body(std::integral_constant<int, IE_ACT_RELU6>()); break;
+    case IE_ACT_SILU: body(std::integral_constant<int, IE_ACT_SILU>()); break;
+    case IE_ACT_GELU: body(std::integral_constant<int, IE_ACT_GELU>()); break;
+    default: body(std::integral_constant<int, IE_ACT_NONE>()); break;
+  }
 }
 
 // One cluster per (image, channel range); each block holds its pixels' items
 // in shared memory.  The copies are issued at once, so the whole range is in
 // flight; a thread reads back only what it copied itself.
 template <int XT, int YT, int V>
-__global__ void __launch_bounds__(kGnThreads, 2) group_norm_cluster_kernel(const GroupNormArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const GroupNormArgs a) {
   namespace cg = cooperative_groups;
   constexpr int kItem = Item<XT, V>::kBytes * (XT == IE_DT_BF16X2 ? 2 : 1);
   static_assert(Item<XT, V>::kBytes == 16, "16-byte copies");
@@ -262,7 +307,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_cluster_kernel(const
   float2* own = reinterpret_cast<float2*>(smem);  // [range_groups] of this block
   float2* stat = own + a.range_groups;            // [range_groups] mean, 1 / sigma
   float* scratch = reinterpret_cast<float*>(stat + a.range_groups);
-  uint8_t* items = reinterpret_cast<uint8_t*>(scratch + (2 * V + 1) * kGnThreads);
+  uint8_t* items = reinterpret_cast<uint8_t*>(scratch + (2 * V + 2) * kGnThreads);
   items += (16 - reinterpret_cast<uintptr_t>(items) % 16) % 16;
 
   cg::cluster_group cluster = cg::this_cluster();
@@ -295,7 +340,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_cluster_kernel(const
       }
     }
   }
-  float g[V], b[V], sub[V];
+  float g[V], b[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     g[e] = works && a.gamma != nullptr && c + e < a.c ? a.gamma[c + e] : 1.0f;
@@ -349,21 +394,25 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_cluster_kernel(const
     const int gi = (c + e - r.c0) / r.group_channels;
     const float2 st = works && c + e < a.c ? stat[gi] : make_float2(0.0f, 0.0f);
     g[e] *= st.y;
-    sub[e] = st.x;
+    b[e] = fmaf(-st.x, g[e], b[e]);  // the mean goes into the addend
   }
-  for (int i = 0; i < n; ++i) {
-    float f[V];
-    item(i, f);
-    finish_item<YT, V>(a, f, g, sub, b, p0 + row + static_cast<int64_t>(i) * r.rows, c);
-  }
+  with_activation(a.act, [&](auto act) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+      float f[V];
+      item(i, f);
+      finish_item<YT, V, decltype(act)::value>(a, f, g, b,
+                                               p0 + row + static_cast<int64_t>(i) * r.rows, c);
+    }
+  });
 }
 
 // Statistics of one block of pixels of an image and channel range.
 template <int XT, int V>
-__global__ void __launch_bounds__(kGnThreads) group_norm_stats_kernel(const GroupNormArgs a) {
+__global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const GroupNormArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
   float* scratch = reinterpret_cast<float*>(smem);
-  float2* own = reinterpret_cast<float2*>(scratch + (2 * V + 1) * kGnThreads);
+  float2* own = reinterpret_cast<float2*>(scratch + (2 * V + 2) * kGnThreads);
   const int block = blockIdx.x % a.blocks;
   const int64_t unit = blockIdx.x / a.blocks;
   const int range = a.first_range + static_cast<int>(unit % a.launch_ranges);
@@ -404,7 +453,7 @@ __global__ void __launch_bounds__(kGnThreads) group_norm_stats_kernel(const Grou
 // Joins the blocks' statistics (every block of the launch for itself) and
 // normalizes.  Blocks run over the pixels from the end, which L2 still holds.
 template <int XT, int YT, int V>
-__global__ void __launch_bounds__(kGnThreads) group_norm_apply_kernel(const GroupNormArgs a,
+__global__ void __launch_bounds__(kGnThreads, 2) group_norm_apply_kernel(const GroupNormArgs a,
                                                                       int apply_blocks) {
   extern __shared__ __align__(16) uint8_t smem[];
   float2* stat = reinterpret_cast<float2*>(smem);
@@ -447,35 +496,37 @@ __global__ void __launch_bounds__(kGnThreads) group_norm_apply_kernel(const Grou
     const int col = col0 + threadIdx.x % cols, row = threadIdx.x / cols;
     if (row >= rows) continue;
     const int c = r.c0 + col * V;
-    float mul[V], sub[V], add[V];
+    float mul[V], add[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      mul[e] = sub[e] = add[e] = 0.0f;
+      mul[e] = add[e] = 0.0f;
       if (c + e < a.c) {
         const float2 st = stat[(c + e - r.c0) / r.group_channels];
         mul[e] = a.gamma == nullptr ? st.y : st.y * a.gamma[c + e];
-        sub[e] = st.x;
-        add[e] = a.beta == nullptr ? 0.0f : a.beta[c + e];
+        // the mean goes into the addend
+        add[e] = fmaf(-st.x, mul[e], a.beta == nullptr ? 0.0f : a.beta[c + e]);
       }
     }
-    constexpr int K = 4;
-    for (int64_t p = row; p < count; p += K * rows) {
-      Item<XT, V> it[K];
+    constexpr int K = XT == IE_DT_BF16X2 ? 2 : 4;
+    with_activation(a.act, [&](auto act) {
+      for (int64_t p = row; p < count; p += K * rows) {
+        Item<XT, V> it[K];
 #pragma unroll
-      for (int e = 0; e < K; ++e) {
-        if (p + int64_t{e} * rows < count) {
-          it[e] = load_item<XT, V>(a.x, channel_at<XT>(p0 + p + int64_t{e} * rows, a.c_store, c),
-                                   a.c_store);
+        for (int e = 0; e < K; ++e) {
+          if (p + int64_t{e} * rows < count) {
+            it[e] = load_item<XT, V>(a.x, channel_at<XT>(p0 + p + int64_t{e} * rows, a.c_store, c),
+                                     a.c_store);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < K; ++e) {
+          if (p + int64_t{e} * rows >= count) break;
+          float f[V];
+          item_floats<XT, V>(it[e], f);
+          finish_item<YT, V, decltype(act)::value>(a, f, mul, add, p0 + p + int64_t{e} * rows, c);
         }
       }
-#pragma unroll
-      for (int e = 0; e < K; ++e) {
-        if (p + int64_t{e} * rows >= count) break;
-        float f[V];
-        item_floats<XT, V>(it[e], f);
-        finish_item<YT, V>(a, f, mul, sub, add, p0 + p + int64_t{e} * rows, c);
-      }
-    }
+    });
   }
 }
 

@@ -76,10 +76,11 @@ bool range_fits(const ie_group_norm_desc* d, int64_t g, int v) {
 }
 
 // The choice between one kernel that holds x in shared memory and two that
-// read it twice, and the split of the work, by an estimate of the time:
-// blocks run in waves over the SMs, each wave costs about 3 us of latencies
-// and moves its bytes at the SM's share of the memory bandwidth (44 bytes/ns);
-// pieces of a pixel narrower than 128 bytes waste part of each DRAM access.
+// read it twice, and the split of the work, by an estimate of the time: blocks
+// run in waves over the SMs; a wave costs about 4 us of latencies (load, join,
+// store), more with the cluster's barriers, and all of them together no less
+// than the bytes at the measured 6.5 TB/s.  Pieces of a pixel narrower than
+// 128 bytes waste part of each DRAM access.
 Plan plan_for(const ie_group_norm_desc* d, int v) {
   Plan best;
   const int64_t cg = d->c / d->groups, pixels = d->h * d->w;
@@ -98,16 +99,17 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
     for (int blocks = 1; blocks <= 16; blocks *= 2) {
       const int64_t share = ceil_div(pixels, blocks);
       const int64_t held = ceil_div(share, rows) * kGnThreads * item_bytes(d->x_type, v);
-      const int64_t smem = held + (2 * v + 1) * kGnThreads * 4 + 16 * g + 32;
+      const int64_t smem = held + (2 * v + 2) * kGnThreads * 4 + 16 * g + 32;
       if (smem > kSmemPerSm || (blocks > 1 && share * (blocks - 1) >= pixels)) continue;
-      const int64_t per_sm = smem + 1024 <= kSmemPerSm / 2 ? 2 : 1;
+      const int64_t per_sm = std::min<int64_t>(4, (kSmemPerSm + 1024) / (smem + 1024));
       const int64_t total = d->n * ranges * blocks;
       const int64_t waves = ceil_div(total, kSms * per_sm);
-      const double resident = static_cast<double>(std::min(per_sm, ceil_div(total, kSms)));
-      const double bytes = static_cast<double>(share * g * cg * (xb + yb));
-      double ns = static_cast<double>(waves) *
-                  (3000.0 + (blocks > 8 ? 1500.0 : blocks > 1 ? 500.0 : 0.0) +
-                   waste * bytes * resident / 44.0);
+      const double latency = blocks > 8 ? 5500.0 : blocks > 1 ? 4500.0 : 4000.0;
+      // one wave: no SM can do better than its own share of the bandwidth
+      const double busy = static_cast<double>(std::min<int64_t>(total, kSms)) / kSms;
+      const double bytes = static_cast<double>(d->n * pixels * d->c) * static_cast<double>(xb + yb);
+      const double ns = latency + std::max(latency * static_cast<double>(waves - 1),
+                                           waste * bytes / (6500.0 * busy));
       if (ns < best_ns) {
         best_ns = ns;
         best.cluster = true;
@@ -119,9 +121,9 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
     }
   }
   // two kernels: a second launch, x read again from L2 (about twice as fast)
-  const double two_ns = 8000.0 + static_cast<double>(d->n * pixels * d->c_store) *
+  const double two_ns = 9000.0 + static_cast<double>(d->n * pixels * d->c_store) *
                                      (1.5 * static_cast<double>(xb) + static_cast<double>(yb)) /
-                                     (44.0 * kSms);
+                                     6500.0;
   if (best.cluster && best_ns <= two_ns) return best;
   best.cluster = false;
   // ranges: whole pixels if the threads cover them and the image fits a wave,
@@ -152,10 +154,10 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
   }
   const int64_t units = best.wave_images * best.wave_ranges;
   best.blocks = static_cast<int>(
-      std::max<int64_t>(1, std::min(ceil_div(2 * kSms, units), ceil_div(pixels, kGnBatch * rows))));
+      std::max<int64_t>(1, std::min(2 * kSms / units, ceil_div(pixels, kGnBatch * rows))));
   best.apply_blocks = static_cast<int>(
-      std::max<int64_t>(1, std::min(ceil_div(4 * kSms, units), ceil_div(pixels, 4 * rows))));
-  best.smem = (2 * v + 1) * kGnThreads * 4 + 8 * best.range_groups;
+      std::max<int64_t>(1, std::min(2 * kSms / units, ceil_div(pixels, 4 * rows))));
+  best.smem = (2 * v + 2) * kGnThreads * 4 + 8 * best.range_groups;
   best.workspace = units * best.blocks * best.range_groups * static_cast<int64_t>(sizeof(float2));
   return best;
 }

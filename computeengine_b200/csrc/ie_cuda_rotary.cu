@@ -45,7 +45,7 @@ using Launch = void (*)(const RotaryArgs&, dim3, cudaStream_t);
 
 template <int XT, int YT, int W, int CW>
 void launch(const RotaryArgs& a, dim3 grid, cudaStream_t s) {
-  const size_t smem = sizeof(float2) * a.block_tokens * a.pairs;
+  const size_t smem = sizeof(float2) * a.block_tokens * a.pairs + sizeof(uint32_t) * a.units.d;
   rotary_kernel<XT, YT, W, CW><<<grid, 256, smem, s>>>(a);
 }
 
