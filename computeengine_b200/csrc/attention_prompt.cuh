@@ -39,65 +39,6 @@ struct PromptPlan {
   static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024 + 256;
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float y;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-  return y;
-}
-
-template <int T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  uint32_t y;
-  if constexpr (T == IE_DT_BF16) {
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-  } else {
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
-  }
-  return y;
-}
-
-// The block's sequence and first query row; false when it has none.
-// Documents: the blocks of 256 rows are counted through all documents.
-__device__ __forceinline__ bool prompt_rows(const PromptArgs& a, int tile, int batch_row,
-                                            Sequence* s, int* row0) {
-  if (a.documents == 0) {
-    *s = sequence(a, batch_row);
-    *row0 = tile * 256;
-    return *row0 < s->q1;
-  }
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  for (int r0 = 0; r0 < a.documents; r0 += 32) {
-    const int r = r0 + lane;
-    int count = 0;
-    if (r < a.documents) {
-      const Sequence d = sequence(a, r);
-      count = (d.q1 - d.q0 + 255) / 256;
-    }
-    int sum = count;
-    for (int w = 1; w < 32; w <<= 1) {
-      const int up = __shfl_up_sync(0xFFFFFFFFu, sum, w);
-      if (lane >= w) sum += up;
-    }
-    const unsigned hit = __ballot_sync(0xFFFFFFFFu, before + sum > tile);
-    if (hit != 0) {
-      const int at = __ffs(hit) - 1;
-      const int skipped = before + __shfl_sync(0xFFFFFFFFu, sum - count, at);
-      *s = sequence(a, r0 + at);
-      *row0 = s->q0 + (tile - skipped) * 256;
-      return true;
-    }
-    before += __shfl_sync(0xFFFFFFFFu, sum, 31);
-  }
-  return false;
-}
-
 template <int DP, int T, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kPromptThreads, 1)
     attention_prompt_kernel(const PromptArgs a, const __grid_constant__ CUtensorMap map_q,
@@ -114,7 +55,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x / a.q_heads / a.batch);  // causal: longest first
   Sequence seq;
   int row0 = 0;
-  if (!prompt_rows(a, tile, batch_row, &seq, &row0)) return;
+  if (!tile_sequence(a, tile, batch_row, 256, &seq, &row0)) return;
   const int length = seq.k1 - seq.k0;
   // key tiles of each row tile: up to what its last row sees
   int tiles_t[2];
@@ -398,7 +339,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           const float p1 = ex2(fmaf(x[64 * c + 2 * e + 1], to_log2, -base));
           sum[e & 1] += p0;
           sum[2 + (e & 1)] += p1;
-          p[e] = pack2<T>(p0, p1);
+          p[e] = pack_pair<T>(p0, p1);
         }
         tmem_st_32x32b_x32(s_at + 32 * c, p);
       }
@@ -448,11 +389,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
             }
             uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int f = 0; f < 4; ++f) hi[f] = pack2<T>(y[e + 2 * f], y[e + 2 * f + 1]);
+            for (int f = 0; f < 4; ++f) hi[f] = pack_pair<T>(y[e + 2 * f], y[e + 2 * f + 1]);
             if (a.o_lo != 0) {
 #pragma unroll
               for (int f = 0; f < 4; ++f) {
-                lo[f] = pack2<T>(y[e + 2 * f] - __uint_as_float(hi[f] << 16),
+                lo[f] = pack_pair<T>(y[e + 2 * f] - __uint_as_float(hi[f] << 16),
                                  y[e + 2 * f + 1] - __uint_as_float(hi[f] & 0xFFFF0000u));
               }
             }
@@ -494,57 +435,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
-}
-
-// Joins the shares of split sequences: one warp per row and head.
-template <int OT>
-__global__ void __launch_bounds__(128) attention_join_kernel(const AttentionArgs a, int splits,
-                                                             const float* part_o,
-                                                             const float* part_lse) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.q_len;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (at >= rows) return;
-  const int i = static_cast<int>(at % a.q_len);
-  const int h = static_cast<int>(at / a.q_len % a.q_heads);
-  const int b = static_cast<int>(at / a.q_len / a.q_heads);
-  if (a.documents > 0) {  // rows of no document stay as they are
-    int lo = 0, hi = a.documents;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.q_offsets[mid + 1] > i) hi = mid;
-      else lo = mid + 1;
-    }
-    if (lo >= a.documents || a.q_offsets[lo] > i) return;
-  }
-  float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, part_lse[s * rows + at]);
-  const float base = top == -INFINITY ? 0.0f : top;
-  float y[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float w = expf(part_lse[s * rows + at] - base);
-    if (w == 0.0f) continue;  // an empty share wrote no o
-    sum += w;
-    for (int e = 0; e < 4; ++e) {
-      const int d = lane + 32 * e;
-      if (d < a.head_dim) y[e] += w * part_o[(s * rows + at) * a.head_dim + d];
-    }
-  }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t oo = b * a.o_stride[0] + i * a.o_stride[1] + h * a.o_stride[2];
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + 32 * e;
-    if (d >= a.head_dim) continue;
-    const float v = y[e] * inv;
-    if constexpr (OT == IE_DT_BF16X2) {
-      const float hi = __bfloat162float(__float2bfloat16_rn(v));
-      store_element<IE_DT_BF16>(a.o, oo + d, hi);
-      store_element<IE_DT_BF16>(a.o, oo + a.o_lo + d, v - hi);
-    } else {
-      store_element<OT>(a.o, oo + d, v);
-    }
-  }
-  if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.0f ? -INFINITY : base + logf(sum);
 }
 
 }  // namespace ie_cuda

@@ -7,8 +7,8 @@
 #include <cmath>
 #include <cstdint>
 
-#include "attention_kernels.cuh"
 #include "attention_prompt.cuh"
+#include "attention_step.cuh"
 #include "host_util.h"
 
 using namespace ie_cuda;
@@ -118,28 +118,63 @@ bool tma_readable(const void* p, int64_t head_dim, int64_t len, int64_t heads, i
   return true;
 }
 
-struct Plan {
-  int64_t tiles = 0;  // blocks of 256 query rows per head and batch row
-  int splits = 1;
-  size_t workspace = 0;
+constexpr int64_t kSms = 148;
+
+// Shares of each sequence's keys, their partial results in the workspace.
+size_t share_bytes(const ie_attention_desc* d, int splits) {
+  if (splits <= 1) return 0;
+  const int64_t rows = d->batch * d->q_heads * d->q_len * splits;
+  return static_cast<size_t>(round_up(rows * d->head_dim * 4, 256) + rows * 4);
+}
+
+// The step kernel's tiles: all heads of a kv head and all positions when that
+// is at most 32 rows, else 32 positions of one head (documents; unaligned
+// tensors of many rows).
+struct StepTiles {
+  int rows, heads;
+  int64_t tiles;
+  int splits;
 };
 
-// Blocks of the prompt kernel, and into how many shares each block's keys are
-// cut when the blocks alone leave more than half of the GPU idle.
-Plan plan_for(const ie_attention_desc* d, const ie_attention_mask* m) {
-  Plan p;
+bool few_rows(const ie_attention_desc* d, const ie_attention_mask* m) {
+  return (m == nullptr || m->documents == 0) && d->q_len * (d->q_heads / d->kv_heads) <= 32;
+}
+
+StepTiles step_tiles(const ie_attention_desc* d, const ie_attention_mask* m) {
+  StepTiles t{};
+  if (few_rows(d, m)) {
+    t.rows = static_cast<int>(d->q_len);
+    t.heads = d->q_heads / d->kv_heads;
+    t.tiles = 1;
+    // About four blocks for each of the two that an SM holds, so that ragged
+    // lengths even out, of at least 256 keys.
+    const int64_t units = d->batch * d->kv_heads;
+    const int64_t share = std::max<int64_t>(256, ceil_div(units * d->kv_len, 8 * kSms));
+    t.splits = static_cast<int>(std::min<int64_t>(ceil_div(d->kv_len, share), 1024));
+  } else {
+    const int64_t documents = m == nullptr ? 0 : m->documents;
+    t.rows = 32;
+    t.heads = 1;
+    t.tiles = documents > 0 ? d->q_len / 32 + documents : ceil_div(d->q_len, 32);
+    t.splits = 1;
+  }
+  return t;
+}
+
+// The prompt kernel's blocks of 256 query rows, and into how many shares each
+// block's keys are cut when the blocks alone leave half of the GPU idle.
+struct PromptTiles {
+  int64_t tiles;
+  int splits;
+};
+
+PromptTiles prompt_tiles(const ie_attention_desc* d, const ie_attention_mask* m) {
   const int64_t documents = m == nullptr ? 0 : m->documents;
-  p.tiles = documents > 0 ? d->q_len / 256 + documents : ceil_div(d->q_len, 256);
+  PromptTiles p{documents > 0 ? d->q_len / 256 + documents : ceil_div(d->q_len, 256), 1};
   const int64_t blocks = p.tiles * d->q_heads * d->batch;
   const int64_t key_tiles = ceil_div(d->kv_len, 128);
-  constexpr int64_t kSms = 148;
   if (documents == 0 && blocks * 2 <= kSms && key_tiles >= 8) {
     p.splits = static_cast<int>(std::min(kSms / blocks, key_tiles / 4));
-  }
-  if (p.splits > 1) {
-    const int64_t rows = d->batch * d->q_heads * d->q_len;
-    p.workspace = static_cast<size_t>(round_up(rows * p.splits * d->head_dim * 4, 256) +
-                                      rows * p.splits * 4);
   }
   return p;
 }
@@ -167,18 +202,105 @@ int launch_prompt(const PromptArgs& a, const CUtensorMap* maps, dim3 grid, cudaS
 }
 
 template <int OT>
-int launch_join(const PromptArgs& a, cudaStream_t s) {
+int launch_join(const AttentionArgs& a, int splits, const float* part_o, const float* part_lse,
+                cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.q_len;
   attention_join_kernel<OT><<<static_cast<unsigned>(ceil_div(rows, 4)), 128, 0, s>>>(
-      a, a.splits, a.part_o, a.part_lse);
+      a, splits, part_o, part_lse);
   return check_launch("attention join");
 }
 
-template <int T, int OT>
-void launch_simple(const AttentionArgs& a, cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((a.q_len + 3) / 4), static_cast<unsigned>(a.q_heads),
-                  static_cast<unsigned>(a.batch));
-  attention_simple_kernel<T, OT><<<grid, 128, 0, s>>>(a);
+int join(const ie_attention_desc* d, const AttentionArgs& a, int splits, const float* part_o,
+         const float* part_lse, cudaStream_t s) {
+  return d->o_type == IE_DT_BF16X2 ? launch_join<IE_DT_BF16X2>(a, splits, part_o, part_lse, s)
+         : d->o_type == IE_DT_BF16 ? launch_join<IE_DT_BF16>(a, splits, part_o, part_lse, s)
+                                   : launch_join<IE_DT_F16>(a, splits, part_o, part_lse, s);
+}
+
+template <int DP, int T, int MT, bool VEC>
+int launch_step(const StepArgs& a, dim3 grid, cudaStream_t s) {
+  auto kernel = attention_step_kernel<DP, T, MT, VEC>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             StepPlan<DP>::kSmem);
+  if (e != cudaSuccess) return fail(IE_RUNTIME, "attention: %s", cudaGetErrorString(e));
+  kernel<<<grid, kStepThreads, StepPlan<DP>::kSmem, s>>>(a);
+  return check_launch("attention");
+}
+
+template <int DP, int T>
+int launch_step(const StepArgs& a, dim3 grid, bool vec, cudaStream_t s) {
+  if (a.tile_rows * a.tile_heads <= 16) {
+    return vec ? launch_step<DP, T, 1, true>(a, grid, s) : launch_step<DP, T, 1, false>(a, grid, s);
+  }
+  return vec ? launch_step<DP, T, 2, true>(a, grid, s) : launch_step<DP, T, 2, false>(a, grid, s);
+}
+
+int run_step(const ie_attention_desc* d, const ie_attention_mask* m, const AttentionArgs& base,
+             bool vec, float* workspace, cudaStream_t s) {
+  StepArgs a{};
+  static_cast<AttentionArgs&>(a) = base;
+  const StepTiles t = step_tiles(d, m);
+  a.tile_rows = t.rows;
+  a.tile_heads = t.heads;
+  a.tiles = static_cast<int>(t.tiles);
+  a.splits = t.splits;
+  const int64_t rows = d->batch * d->q_heads * d->q_len * a.splits;
+  a.part_o = a.splits > 1 ? workspace : nullptr;
+  a.part_lse = a.splits > 1 ? workspace + round_up(rows * d->head_dim, 64) : nullptr;
+  const int64_t blocks = t.tiles * (d->q_heads / t.heads) * d->batch;
+  if (blocks > INT_MAX) return fail(IE_UNSUPPORTED, "Attention has too many rows");
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.splits));
+  const bool bf16 = d->type == IE_DT_BF16;
+  int rc;
+  if (d->head_dim <= 64) {
+    rc = bf16 ? launch_step<64, IE_DT_BF16>(a, grid, vec, s)
+              : launch_step<64, IE_DT_F16>(a, grid, vec, s);
+  } else {
+    rc = bf16 ? launch_step<128, IE_DT_BF16>(a, grid, vec, s)
+              : launch_step<128, IE_DT_F16>(a, grid, vec, s);
+  }
+  if (rc != IE_OK || a.splits == 1) return rc;
+  return join(d, a, a.splits, a.part_o, a.part_lse, s);
+}
+
+int run_prompt(const ie_attention_desc* d, const ie_attention_mask* m, const AttentionArgs& base,
+               float* workspace, cudaStream_t s) {
+  PromptArgs a{};
+  static_cast<AttentionArgs&>(a) = base;
+  const PromptTiles t = prompt_tiles(d, m);
+  const int64_t blocks = t.tiles * d->q_heads * d->batch;
+  if (blocks > INT_MAX) return fail(IE_UNSUPPORTED, "Attention has too many rows");
+  const bool bf16 = d->type == IE_DT_BF16;
+  CUtensorMap maps[3];
+  int rc = encode_rows(&maps[0], a.q, bf16, d->head_dim, d->q_len, d->q_heads, d->batch,
+                       d->q_stride);
+  if (rc == IE_OK) {
+    rc = encode_rows(&maps[1], a.k, bf16, d->head_dim, d->kv_len, d->kv_heads, d->batch,
+                     d->k_stride);
+  }
+  if (rc == IE_OK) {
+    rc = encode_rows(&maps[2], a.v, bf16, d->head_dim, d->kv_len, d->kv_heads, d->batch,
+                     d->v_stride);
+  }
+  if (rc != IE_OK) return rc;
+  a.tiles = static_cast<int>(t.tiles);
+  a.splits = t.splits;
+  const int64_t rows = d->batch * d->q_heads * d->q_len * a.splits;
+  a.part_o = a.splits > 1 ? workspace : nullptr;
+  a.part_lse = a.splits > 1 ? workspace + round_up(rows * d->head_dim, 64) : nullptr;
+  a.o_vec = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.o_lo % 8 == 0;
+  for (int i = 0; i < 3; ++i) a.o_vec = a.o_vec && a.o_stride[i] % 8 == 0;
+  a.wait_limit_ns = kWaitLimitNs;
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.splits));
+  if (d->head_dim <= 64) {
+    rc = bf16 ? launch_prompt<64, IE_DT_BF16>(a, maps, grid, s)
+              : launch_prompt<64, IE_DT_F16>(a, maps, grid, s);
+  } else {
+    rc = bf16 ? launch_prompt<128, IE_DT_BF16>(a, maps, grid, s)
+              : launch_prompt<128, IE_DT_F16>(a, maps, grid, s);
+  }
+  if (rc != IE_OK || a.splits == 1) return rc;
+  return join(d, a, a.splits, a.part_o, a.part_lse, s);
 }
 
 }  // namespace
@@ -201,7 +323,9 @@ extern "C" {
 size_t ie_cuda_attention_workspace_bytes(const ie_attention_desc* desc,
                                          const ie_attention_mask* mask) {
   if (check_attention(desc, mask) != IE_OK) return 0;
-  return plan_for(desc, mask).workspace;
+  // few rows always run on the step kernel; many rows that TMA cannot read are not split
+  return share_bytes(desc, few_rows(desc, mask) ? step_tiles(desc, mask).splits
+                                                : prompt_tiles(desc, mask).splits);
 }
 
 int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* mask, const void* q,
@@ -212,14 +336,21 @@ int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* ma
   if (q == nullptr || k == nullptr || v == nullptr || o == nullptr) {
     return fail(IE_INVALID_ARGUMENT, "null tensor or buffer");
   }
-  const Plan plan = plan_for(desc, mask);
-  if (plan.workspace > 0 &&
-      (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
-       workspace_bytes < plan.workspace)) {
+  const bool few = few_rows(desc, mask);
+  const bool kv_tma =
+      tma_readable(k, desc->head_dim, desc->kv_len, desc->kv_heads, desc->batch, desc->k_stride) &&
+      tma_readable(v, desc->head_dim, desc->kv_len, desc->kv_heads, desc->batch, desc->v_stride);
+  const bool tma = kv_tma && tma_readable(q, desc->head_dim, desc->q_len, desc->q_heads,
+                                          desc->batch, desc->q_stride);
+  const size_t need =
+      few ? share_bytes(desc, step_tiles(desc, mask).splits)
+          : tma ? share_bytes(desc, prompt_tiles(desc, mask).splits) : size_t{0};
+  if (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
+                   workspace_bytes < need)) {
     return fail(IE_INVALID_ARGUMENT, "Attention needs %zu bytes of 256-byte aligned workspace",
-                plan.workspace);
+                need);
   }
-  PromptArgs a{};
+  AttentionArgs a{};
   a.q = q;
   a.k = k;
   a.v = v;
@@ -248,51 +379,8 @@ int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* ma
     a.slopes = mask->slopes;
   }
   const cudaStream_t s = as_stream(stream);
-  const int64_t blocks = plan.tiles * a.q_heads * a.batch;
-  if (blocks <= INT_MAX &&
-      tma_readable(q, a.head_dim, a.q_len, a.q_heads, a.batch, a.q_stride) &&
-      tma_readable(k, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride) &&
-      tma_readable(v, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.v_stride)) {
-    const bool bf16 = desc->type == IE_DT_BF16;
-    CUtensorMap maps[3];
-    int rc2 = encode_rows(&maps[0], q, bf16, a.head_dim, a.q_len, a.q_heads, a.batch, a.q_stride);
-    if (rc2 == IE_OK) {
-      rc2 = encode_rows(&maps[1], k, bf16, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.k_stride);
-    }
-    if (rc2 == IE_OK) {
-      rc2 = encode_rows(&maps[2], v, bf16, a.head_dim, a.kv_len, a.kv_heads, a.batch, a.v_stride);
-    }
-    if (rc2 != IE_OK) return rc2;
-    a.tiles = static_cast<int>(plan.tiles);
-    a.splits = plan.splits;
-    a.part_o = static_cast<float*>(workspace);
-    a.part_lse = a.splits > 1 ? a.part_o + round_up(int64_t{1} * a.batch * a.q_heads * a.q_len *
-                                                        a.splits * a.head_dim, 64)
-                              : nullptr;
-    a.o_vec = reinterpret_cast<uintptr_t>(o) % 16 == 0 && a.o_lo % 8 == 0;
-    for (int i = 0; i < 3; ++i) a.o_vec = a.o_vec && a.o_stride[i] % 8 == 0;
-    a.wait_limit_ns = kWaitLimitNs;
-    const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.splits));
-    if (a.head_dim <= 64) {
-      rc2 = bf16 ? launch_prompt<64, IE_DT_BF16>(a, maps, grid, s)
-                 : launch_prompt<64, IE_DT_F16>(a, maps, grid, s);
-    } else {
-      rc2 = bf16 ? launch_prompt<128, IE_DT_BF16>(a, maps, grid, s)
-                 : launch_prompt<128, IE_DT_F16>(a, maps, grid, s);
-    }
-    if (rc2 != IE_OK || a.splits == 1) return rc2;
-    return desc->o_type == IE_DT_BF16X2 ? launch_join<IE_DT_BF16X2>(a, s)
-           : bf16                       ? launch_join<IE_DT_BF16>(a, s)
-                                        : launch_join<IE_DT_F16>(a, s);
-  }
-  if (desc->o_type == IE_DT_BF16X2) {
-    launch_simple<IE_DT_BF16, IE_DT_BF16X2>(a, s);
-  } else if (desc->type == IE_DT_BF16) {
-    launch_simple<IE_DT_BF16, IE_DT_BF16>(a, s);
-  } else {
-    launch_simple<IE_DT_F16, IE_DT_F16>(a, s);
-  }
-  return check_launch("attention");
+  if (few || !tma) return run_step(desc, mask, a, kv_tma, static_cast<float*>(workspace), s);
+  return run_prompt(desc, mask, a, static_cast<float*>(workspace), s);
 }
 
 }  // extern "C"
