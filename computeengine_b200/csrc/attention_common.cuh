@@ -6,6 +6,8 @@
 
 namespace ie_cuda {
 
+constexpr int kMaxSplits = 1024;  // shares of one sequence's keys
+
 struct AttentionArgs {
   const void* q;
   const void* k;
@@ -107,46 +109,53 @@ __device__ __forceinline__ bool tile_sequence(const AttentionArgs& a, int tile, 
   return false;
 }
 
-// Joins the shares of split sequences: one warp per row and head.
+// Joins the shares of split sequences: one block per row and head.  The
+// shares' weights are taken by all threads at once, then each warp sums every
+// fourth share.
 template <int OT>
 __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionArgs a, int splits,
                                                              const float* part_o,
                                                              const float* part_lse) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.q_len;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (at >= rows) return;
+  __shared__ float weight[kMaxSplits], warp_top[4], warp_total[4], warp_y[4][128];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t rows = int64_t{a.batch} * a.q_heads * a.q_len;
+  const int64_t at = blockIdx.x;
   const int i = static_cast<int>(at % a.q_len);
   const int h = static_cast<int>(at / a.q_len % a.q_heads);
-  const int b = static_cast<int>(at / a.q_len / a.q_heads);
-  if (a.documents > 0) {  // rows of no document stay as they are
-    int lo = 0, hi = a.documents;
-    while (lo < hi) {
-      const int mid = (lo + hi) / 2;
-      if (a.q_offsets[mid + 1] > i) hi = mid;
-      else lo = mid + 1;
-    }
-    if (lo >= a.documents || a.q_offsets[lo] > i) return;
-  }
+  const int64_t b = at / a.q_len / a.q_heads;
   float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, part_lse[s * rows + at]);
+  for (int s = threadIdx.x; s < splits; s += 128) {
+    weight[s] = part_lse[s * rows + at];
+    top = max_nan(top, weight[s]);
+  }
+  for (int w = 16; w > 0; w >>= 1) top = max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, w));
+  if (lane == 0) warp_top[warp] = top;
+  __syncthreads();
+  for (int w = 0; w < 4; ++w) top = max_nan(top, warp_top[w]);
   const float base = top == -INFINITY ? 0.0f : top;
-  float y[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sum = 0.0f;
-  for (int s = 0; s < splits; ++s) {
-    const float w = expf(part_lse[s * rows + at] - base);
-    if (w == 0.0f) continue;  // an empty share wrote no o
-    sum += w;
+  float total = 0.0f, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  const float* o = part_o + at * a.head_dim;
+#pragma unroll 4
+  for (int s = warp; s < splits; s += 4) {
+    const float w = expf(weight[s] - base);
+    total += w;
+#pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = lane + 32 * e;
-      if (d < a.head_dim) y[e] += w * part_o[(s * rows + at) * a.head_dim + d];
+      const float v = d < a.head_dim ? o[s * rows * a.head_dim + d] : 0.0f;
+      y[e] = fmaf(w, v, y[e]);
     }
   }
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  const int64_t oo = b * a.o_stride[0] + i * a.o_stride[1] + h * a.o_stride[2];
-  for (int e = 0; e < 4; ++e) {
-    const int d = lane + 32 * e;
-    if (d >= a.head_dim) continue;
-    const float v = y[e] * inv;
+  if (lane == 0) warp_total[warp] = total;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) warp_y[warp][lane + 32 * e] = y[e];
+  __syncthreads();
+  total = (warp_total[0] + warp_total[1]) + (warp_total[2] + warp_total[3]);
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  const int d = threadIdx.x;
+  if (d < a.head_dim) {
+    const float v = ((warp_y[0][d] + warp_y[1][d]) + (warp_y[2][d] + warp_y[3][d])) * inv;
+    const int64_t oo = b * a.o_stride[0] + i * a.o_stride[1] + h * a.o_stride[2];
     if constexpr (OT == IE_DT_BF16X2) {
       const float hi = __bfloat162float(__float2bfloat16_rn(v));
       store_element<IE_DT_BF16>(a.o, oo + d, hi);
@@ -155,7 +164,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionArgs
       store_element<OT>(a.o, oo + d, v);
     }
   }
-  if (a.lse != nullptr && lane == 0) a.lse[at] = sum == 0.0f ? -INFINITY : base + logf(sum);
+  if (a.lse != nullptr && d == 0) a.lse[at] = total == 0.0f ? -INFINITY : base + logf(total);
 }
 
 }  // namespace ie_cuda

@@ -1,13 +1,16 @@
 // Attention for few query rows (single tokens), and for tensors that TMA
 // cannot read.
 //
-// All query heads that read one kv head are rows of one tile, so K and V are
-// read once: 16 rows are one mma.sync m16n8k16 operand, two at most.  Bound by
-// the memory: a block's four warps take keys 16 at a time, each into its own
-// ring of asynchronous copies (no barrier between warps), with a running
-// maximum and sum per row; long sequences are cut into shares for many blocks.
-// The warps' results are joined in shared memory, the shares' by a second
-// kernel.
+// All query heads that read one kv head are columns of one tile, so K and V
+// are read once: S^T = K Q^T and O^T = V^T P^T with mma.sync m16n8k16, keys (and
+// then elements of the head) as its 16 rows and eight query rows as its
+// columns.  The other way round half of the operand would be empty for up to
+// eight rows, and the softmax would run over the empty half too (735 warp
+// instructions per 16 keys instead of about 250).  Bound by the memory: a
+// block's four warps take keys 16 at a time, each into its own ring of
+// asynchronous copies (no barrier between warps), with a running maximum and
+// sum per row; long sequences are cut into shares for many blocks.  The warps'
+// results are joined in shared memory, the shares' by a second kernel.
 #pragma once
 
 #include "attention_common.cuh"
@@ -20,7 +23,7 @@ constexpr int kStepKeys = 16;
 
 struct StepArgs : AttentionArgs {
   int tile_rows;    // query positions of a tile
-  int tile_heads;   // query heads of a tile; tile_rows * tile_heads <= 16 MT
+  int tile_heads;   // query heads of a tile; tile_rows * tile_heads <= 8 NT
   int tiles;        // tiles of positions per sequence (documents: upper bound in all)
   int splits;       // shares of each sequence's keys
   float* part_o;    // splits > 1: fp32 [splits][batch][q_heads][q_len][head_dim]
@@ -65,6 +68,13 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   }
 }
 
+// The transpose of an 8 x 8 matrix of 16-bit elements held across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(v));
+  return y;
+}
+
 // Byte of 16-byte chunk c of key row r in a tile of rows of DP elements: the
 // chunk's place is turned by the row, so eight rows' chunks share no bank.
 template <int DP>
@@ -72,12 +82,13 @@ __device__ __forceinline__ uint32_t step_at(int r, int c) {
   return static_cast<uint32_t>(r * StepPlan<DP>::kRow + ((c ^ (r & 7)) << 4));
 }
 
-// VEC: K and V in 16-byte aligned rows of a multiple of 8 elements.
-template <int DP, int T, int MT, bool VEC>
+// NT: columns / 8.  VEC: K and V in 16-byte aligned rows of a multiple of 8
+// elements.
+template <int DP, int T, int NT, bool VEC>
 __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const StepArgs a) {
   using P = StepPlan<DP>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float row_m[4][16 * MT], row_l[4][16 * MT];
+  __shared__ float row_m[4][8 * NT], row_l[4][8 * NT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int heads_per_kv = a.q_heads / a.kv_heads;
   const int head_tiles = a.q_heads / a.tile_heads;
@@ -103,187 +114,191 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
                       int64_t{seq.k0} * a.v_stride[1] + hk * a.v_stride[2];
   uint8_t* ring = smem + warp * kStepStages * P::kStage;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  const int chunks = (a.head_dim + 7) / 8;  // of a row that hold data
 
-  // copies K and V of keys key .. key + 15 into a stage; rows past `to` and
-  // elements past head_dim are zeros
-  auto fetch = [&](int stage, int key) {
+  // Copies K and V of the next 16 keys of this warp into a stage; rows past
+  // `to` and elements past head_dim are zeros.  A lane copies chunk lane %
+  // kChunks of the rows lane / kChunks + i * kRows.
+  constexpr int kStride = 4 * kStepKeys;
+  constexpr int kChunks = DP / 8, kRows = 32 / kChunks, kCopies = kStepKeys / kRows;
+  const int first = from + warp * kStepKeys;
+  const int my_row = lane / kChunks, my_chunk = lane % kChunks;
+  const bool my_data = my_chunk * 8 < a.head_dim;
+  const uint16_t* k_next = k + (my_data ? my_chunk * 8 : 0) + (first + my_row) * a.k_stride[1];
+  const uint16_t* v_next = v + (my_data ? my_chunk * 8 : 0) + (first + my_row) * a.v_stride[1];
+  int key_next = first;
+  auto fetch = [&](int stage) {
     const uint32_t at = ring_at + stage * P::kStage;
     if constexpr (VEC) {
 #pragma unroll
-      for (int i = 0; i < kStepKeys * DP / 8 / 32; ++i) {
-        const int e = i * 32 + lane, r = e / (DP / 8), c = e % (DP / 8);
-        const bool in = key + r < to && c < chunks;
-        const int64_t j = in ? key + r : 0;
-        const int bytes = in ? 16 : 0, cc = in ? c : 0;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at + step_at<DP>(r, c)),
-                     "l"(k + j * a.k_stride[1] + cc * 8), "r"(bytes)
+      for (int i = 0; i < kCopies; ++i) {
+        const int r = my_row + i * kRows;
+        const bool in = key_next + r < to && my_data;
+        const int bytes = in ? 16 : 0;
+        const uint16_t* kp = in ? k_next + i * kRows * a.k_stride[1] : k;
+        const uint16_t* vp = in ? v_next + i * kRows * a.v_stride[1] : v;
+        const uint32_t s = at + step_at<DP>(r, my_chunk);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s), "l"(kp), "r"(bytes)
                      : "memory");
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                         at + kStepKeys * P::kRow + step_at<DP>(r, c)),
-                     "l"(v + j * a.v_stride[1] + cc * 8), "r"(bytes)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(s + kStepKeys * P::kRow),
+                     "l"(vp), "r"(bytes)
                      : "memory");
       }
+      k_next += kStride * a.k_stride[1];
+      v_next += kStride * a.v_stride[1];
     } else {
       uint8_t* p = ring + stage * P::kStage;
       for (int e = lane; e < kStepKeys * DP; e += 32) {
         const int r = e / DP, d = e % DP;
-        const bool in = key + r < to && d < a.head_dim;
-        const int64_t j = in ? key + r : 0;
+        const bool in = key_next + r < to && d < a.head_dim;
+        const int64_t j = in ? key_next + r : 0;
         uint16_t* at_k = reinterpret_cast<uint16_t*>(p + step_at<DP>(r, d / 8)) + d % 8;
         at_k[0] = in ? k[j * a.k_stride[1] + d] : uint16_t{0};
         at_k[kStepKeys * DP] = in ? v[j * a.v_stride[1] + d] : uint16_t{0};
       }
       __syncwarp();
     }
+    key_next += kStride;
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  const int first = from + warp * kStepKeys;
-  constexpr int kStride = 4 * kStepKeys;
 #pragma unroll
-  for (int s = 0; s < kStepStages - 1; ++s) fetch(s, first + s * kStride);
+  for (int s = 0; s < kStepStages - 1; ++s) fetch(s);
 
-  // ---- Q as mma operands: this thread's rows are lane / 4 and lane / 4 + 8 of
-  // each 16-row tile, row r being head h0 + r / tile_rows, position row0 + r % tile_rows
-  uint32_t q[MT][DP / 16][4];
-  int seen[MT][2], head[MT][2], place[MT][2];
+  // ---- Q^T as mma operand: column lane / 4 of each tile of eight is query row
+  // n, head h0 + n / tile_rows and position row0 + n % tile_rows
+  uint32_t q[NT][DP / 16][2];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int n = 0; n < NT; ++n) {
+    const int r = 8 * n + lane / 4;
+    const int pos = row0 + r % a.tile_rows;
+    const bool valid = r < rows && pos < seq.q1;
+    const uint16_t* qr = static_cast<const uint16_t*>(a.q) + seq.batch * a.q_stride[0] +
+                         int64_t{valid ? pos : row0} * a.q_stride[1] +
+                         (valid ? h0 + r / a.tile_rows : h0) * a.q_stride[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = 16 * m + lane / 4 + 8 * i;
-      const int pos = row0 + r % a.tile_rows;
-      const bool valid = r < rows && pos < seq.q1;
-      head[m][i] = valid ? h0 + r / a.tile_rows : h0;
-      seen[m][i] = valid ? min(to, seq.seen(pos, a.causal)) : 0;
-      place[m][i] = valid ? seq.place(pos) : 0;
-      const uint16_t* qr = static_cast<const uint16_t*>(a.q) + seq.batch * a.q_stride[0] +
-                           int64_t{valid ? pos : row0} * a.q_stride[1] +
-                           head[m][i] * a.q_stride[2];
+    for (int s = 0; s < DP / 16; ++s) {
 #pragma unroll
-      for (int s = 0; s < DP / 16; ++s) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int d = 16 * s + 8 * half + 2 * (lane & 3);
-          const uint32_t lo = valid && d < a.head_dim ? qr[d] : 0u;
-          const uint32_t hi = valid && d + 1 < a.head_dim ? qr[d + 1] : 0u;
-          q[m][s][2 * half + i] = lo | hi << 16;
-        }
+      for (int half = 0; half < 2; ++half) {
+        const int d = 16 * s + 8 * half + 2 * (lane & 3);
+        const uint32_t lo = valid && d < a.head_dim ? qr[d] : 0u;
+        const uint32_t hi = valid && d + 1 < a.head_dim ? qr[d + 1] : 0u;
+        q[n][s][half] = lo | hi << 16;
       }
     }
   }
+  // ---- this thread's softmax rows: columns 2 (lane % 4) and the next
   constexpr float kLog2e = 1.4426950408889634f;
   const float scale = a.scale * kLog2e;
   const bool cap = a.softcap > 0.0f;
   const float cap_in = cap ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
   const float cap_out = a.softcap * kLog2e;
-  float slope[MT][2];
+  const bool bias = a.slopes != nullptr;
+  float slope[NT][2], place[NT][2];
+  int seen[NT][2];
+  float o[NT][DP / 16][4], top[NT][2], sum[NT][2];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      slope[m][i] = a.slopes == nullptr ? 0.0f : a.slopes[head[m][i]] * kLog2e;
+      const int r = 8 * n + 2 * (lane & 3) + i;
+      const int pos = row0 + r % a.tile_rows;
+      const bool valid = r < rows && pos < seq.q1;
+      seen[n][i] = valid ? min(to, seq.seen(pos, a.causal)) : 0;
+      place[n][i] = valid ? static_cast<float>(seq.place(pos)) : 0.0f;
+      slope[n][i] = valid && bias ? a.slopes[h0 + r / a.tile_rows] * kLog2e : 0.0f;
+      top[n][i] = -INFINITY;
+      sum[n][i] = 0.0f;
+    }
+#pragma unroll
+    for (int d = 0; d < DP / 16; ++d) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[n][d][e] = 0.0f;
     }
   }
 
-  float o[MT][DP / 8][4], top[MT][2], sum[MT][2];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      top[m][i] = -INFINITY;
-      sum[m][i] = 0.0f;
-    }
-#pragma unroll
-    for (int n = 0; n < DP / 8; ++n) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[m][n][e] = 0.0f;
-    }
-  }
-
+  // ldmatrix rows of this lane: K as it lies (keys 0-7, 8-15, then the next
+  // eight elements), V transposed (elements 0-7, 8-15, then the next keys)
+  const int k_row = lane & 15, k_half = lane >> 4;
+  const int v_row = (lane & 7) + (lane >> 4) * 8, v_half = lane >> 3 & 1;
   int stage = 0;
   for (int key = first; key < to; key += kStride) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStepStages - 2) : "memory");
     __syncwarp();
-    fetch((stage + kStepStages - 1) % kStepStages, key + (kStepStages - 1) * kStride);
+    fetch(stage == 0 ? kStepStages - 1 : stage - 1);
     const uint32_t k_at = ring_at + stage * P::kStage, v_at = k_at + kStepKeys * P::kRow;
-    stage = (stage + 1) % kStepStages;
-    float s[MT][2][4];
+    stage = stage == kStepStages - 1 ? 0 : stage + 1;
+    float s[NT][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[m][n][e] = 0.0f;
-      }
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
     }
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) {
-      // matrices: keys 0-7 and 8-15, each with the two halves of 16 elements
-      uint32_t b[4];
-      ldmatrix4<false>(b, k_at + step_at<DP>((lane & 7) + (lane >> 4) * 8, 2 * d + (lane >> 3 & 1)));
+      uint32_t m[4];
+      ldmatrix4<false>(m, k_at + step_at<DP>(k_row, 2 * d + k_half));
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        mma_16816<T>(s[m][0], q[m][d], b[0], b[1]);
-        mma_16816<T>(s[m][1], q[m][d], b[2], b[3]);
-      }
+      for (int n = 0; n < NT; ++n) mma_16816<T>(s[n], m, q[n][d][0], q[n][d][1]);
     }
-    uint32_t p[MT][4];
+    // s[n][2 half + i]: key lane / 4 + 8 half, row column i
+    uint32_t p[NT][2];
+    const int j0 = key + lane / 4;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
+    for (int n = 0; n < NT; ++n) {
+      float t[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float t = top[m][i];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = key + 8 * n + 2 * (lane & 3) + e;
-            float x = s[m][n][2 * i + e];
-            if (cap) {
-              x = cap_out - __fdividef(2.0f * cap_out, 1.0f + ex2(x * cap_in));
-            } else {
-              x *= scale;
-            }
-            x -= slope[m][i] * fabsf(static_cast<float>(place[m][i] - j));
-            x = j < seen[m][i] ? x : -INFINITY;
-            s[m][n][2 * i + e] = x;
-            t = max_nan(t, x);
+        for (int half = 0; half < 2; ++half) {
+          float x = s[n][2 * half + i];
+          if (cap) {
+            x = cap_out - __fdividef(2.0f * cap_out, 1.0f + ex2(x * cap_in));
+          } else {
+            x *= scale;
           }
+          const int j = j0 + 8 * half;
+          if (bias) x -= slope[n][i] * fabsf(place[n][i] - static_cast<float>(j));
+          s[n][2 * half + i] = j < seen[n][i] ? x : -INFINITY;
         }
-        t = max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 1));
-        t = max_nan(t, __shfl_xor_sync(0xFFFFFFFFu, t, 2));
-        // as in the prompt kernel: the maximum in use moves when it grew by 2^8
-        const bool moved = !(t - top[m][i] <= 8.0f) && t != -INFINITY;
-        const float factor = moved && top[m][i] != -INFINITY ? ex2(top[m][i] - t) : 1.0f;
-        if (moved) top[m][i] = t;
-        if (__any_sync(0xFFFFFFFFu, moved)) {
-          sum[m][i] *= factor;
+        t[i] = max_nan(top[n][i], max_nan(s[n][i], s[n][2 + i]));
+      }
 #pragma unroll
-          for (int n = 0; n < DP / 8; ++n) {
-            o[m][n][2 * i] *= factor;
-            o[m][n][2 * i + 1] *= factor;
-          }
-        }
-        const float base = top[m][i] == -INFINITY ? 0.0f : top[m][i];
+      for (int w = 4; w < 32; w <<= 1) {
+        t[0] = max_nan(t[0], __shfl_xor_sync(0xFFFFFFFFu, t[0], w));
+        t[1] = max_nan(t[1], __shfl_xor_sync(0xFFFFFFFFu, t[1], w));
+      }
+      // as in the prompt kernel: the maximum in use moves when it grew by 2^8
+      bool moved[2];
+      float factor[2], base[2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float p0 = ex2(s[m][n][2 * i] - base), p1 = ex2(s[m][n][2 * i + 1] - base);
-          sum[m][i] += p0 + p1;
-          p[m][2 * n + i] = pack_pair<T>(p0, p1);
+      for (int i = 0; i < 2; ++i) {
+        moved[i] = !(t[i] - top[n][i] <= 8.0f) && t[i] != -INFINITY;
+        factor[i] = moved[i] && top[n][i] != -INFINITY ? ex2(top[n][i] - t[i]) : 1.0f;
+        if (moved[i]) top[n][i] = t[i];
+        base[i] = top[n][i] == -INFINITY ? 0.0f : top[n][i];
+      }
+      if (__any_sync(0xFFFFFFFFu, moved[0] || moved[1])) {
+        sum[n][0] *= factor[0];
+        sum[n][1] *= factor[1];
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][d][e] *= factor[e & 1];
         }
+      }
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const float p0 = ex2(s[n][2 * half] - base[0]), p1 = ex2(s[n][2 * half + 1] - base[1]);
+        sum[n][0] += p0;
+        sum[n][1] += p1;
+        p[n][half] = transpose8(pack_pair<T>(p0, p1));
       }
     }
 #pragma unroll
     for (int d = 0; d < DP / 16; ++d) {
-      // matrices: keys 0-7 and 8-15 of 8 elements, then of the next 8
-      uint32_t b[4];
-      ldmatrix4<true>(b, v_at + step_at<DP>((lane & 7) + (lane >> 3 & 1) * 8, 2 * d + (lane >> 4)));
+      uint32_t m[4];
+      ldmatrix4<true>(m, v_at + step_at<DP>(v_row, 2 * d + v_half));
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        mma_16816<T>(o[m][2 * d], p[m], b[0], b[1]);
-        mma_16816<T>(o[m][2 * d + 1], p[m], b[2], b[3]);
-      }
+      for (int n = 0; n < NT; ++n) mma_16816<T>(o[n][d], m, p[n][0], p[n][1]);
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -292,21 +307,22 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
   // ---- join the warps: [warp][row][DP] fp32 over the rings
   float* all_o = reinterpret_cast<float*>(smem);
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
+  for (int n = 0; n < NT; ++n) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      float l = sum[m][i];
-      l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-      l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
-      const int r = 16 * m + lane / 4 + 8 * i;
-      if ((lane & 3) == 0) {
-        row_m[warp][r] = top[m][i];
+      float l = sum[n][i];
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, w);
+      const int r = 8 * n + 2 * (lane & 3) + i;
+      if (lane < 4) {
+        row_m[warp][r] = top[n][i];
         row_l[warp][r] = l;
       }
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        *reinterpret_cast<float2*>(all_o + (warp * 16 * MT + r) * DP + 8 * n + 2 * (lane & 3)) =
-            make_float2(o[m][n][2 * i], o[m][n][2 * i + 1]);
+      for (int d = 0; d < DP / 16; ++d) {
+        float* to_o = all_o + (warp * 8 * NT + r) * DP + 16 * d + lane / 4;
+        to_o[0] = o[n][d][i];
+        to_o[8] = o[n][d][2 + i];
       }
     }
   }
@@ -316,9 +332,11 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
     const int pos = row0 + r % a.tile_rows, h = h0 + r / a.tile_rows;
     if (pos >= seq.q1) continue;
     float t = -INFINITY;
+#pragma unroll
     for (int w = 0; w < 4; ++w) t = max_nan(t, row_m[w][r]);
     const float base = t == -INFINITY ? 0.0f : t;
     float f[4], l = 0.0f;
+#pragma unroll
     for (int w = 0; w < 4; ++w) {
       f[w] = row_m[w][r] == -INFINITY ? 0.0f : ex2(row_m[w][r] - base);
       if (f[w] != 0.0f) l += f[w] * row_l[w][r];
@@ -336,8 +354,9 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
     }
     for (int d = lane; d < a.head_dim; d += 32) {
       float y = 0.0f;
+#pragma unroll
       for (int w = 0; w < 4; ++w) {
-        if (f[w] != 0.0f) y += f[w] * all_o[(w * 16 * MT + r) * DP + d];
+        if (f[w] != 0.0f) y += f[w] * all_o[(w * 8 * NT + r) * DP + d];
       }
       y *= inv;
       if (a.splits > 1) {

@@ -146,11 +146,12 @@ StepTiles step_tiles(const ie_attention_desc* d, const ie_attention_mask* m) {
     t.rows = static_cast<int>(d->q_len);
     t.heads = d->q_heads / d->kv_heads;
     t.tiles = 1;
-    // About four blocks for each of the two that an SM holds, so that ragged
-    // lengths even out, of at least 256 keys.
+    // Two blocks per SM at once; with ragged lengths three times as many, which
+    // evens them out.  Shares of at least 256 keys.
     const int64_t units = d->batch * d->kv_heads;
-    const int64_t share = std::max<int64_t>(256, ceil_div(units * d->kv_len, 8 * kSms));
-    t.splits = static_cast<int>(std::min<int64_t>(ceil_div(d->kv_len, share), 1024));
+    const int64_t blocks = (m != nullptr && m->kv_lens != nullptr ? 6 : 2) * kSms;
+    const int64_t share = std::max<int64_t>(256, ceil_div(units * d->kv_len, blocks));
+    t.splits = static_cast<int>(std::min<int64_t>(ceil_div(d->kv_len, share), kMaxSplits));
   } else {
     const int64_t documents = m == nullptr ? 0 : m->documents;
     t.rows = 32;
@@ -205,7 +206,7 @@ template <int OT>
 int launch_join(const AttentionArgs& a, int splits, const float* part_o, const float* part_lse,
                 cudaStream_t s) {
   const int64_t rows = static_cast<int64_t>(a.batch) * a.q_heads * a.q_len;
-  attention_join_kernel<OT><<<static_cast<unsigned>(ceil_div(rows, 4)), 128, 0, s>>>(
+  attention_join_kernel<OT><<<static_cast<unsigned>(rows), 128, 0, s>>>(
       a, splits, part_o, part_lse);
   return check_launch("attention join");
 }
@@ -217,9 +218,9 @@ int join(const ie_attention_desc* d, const AttentionArgs& a, int splits, const f
                                    : launch_join<IE_DT_F16>(a, splits, part_o, part_lse, s);
 }
 
-template <int DP, int T, int MT, bool VEC>
+template <int DP, int T, int NT, bool VEC>
 int launch_step(const StepArgs& a, dim3 grid, cudaStream_t s) {
-  auto kernel = attention_step_kernel<DP, T, MT, VEC>;
+  auto kernel = attention_step_kernel<DP, T, NT, VEC>;
   const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              StepPlan<DP>::kSmem);
   if (e != cudaSuccess) return fail(IE_RUNTIME, "attention: %s", cudaGetErrorString(e));
@@ -227,12 +228,17 @@ int launch_step(const StepArgs& a, dim3 grid, cudaStream_t s) {
   return check_launch("attention");
 }
 
+template <int DP, int T, int NT>
+int launch_step(const StepArgs& a, dim3 grid, bool vec, cudaStream_t s) {
+  return vec ? launch_step<DP, T, NT, true>(a, grid, s) : launch_step<DP, T, NT, false>(a, grid, s);
+}
+
 template <int DP, int T>
 int launch_step(const StepArgs& a, dim3 grid, bool vec, cudaStream_t s) {
-  if (a.tile_rows * a.tile_heads <= 16) {
-    return vec ? launch_step<DP, T, 1, true>(a, grid, s) : launch_step<DP, T, 1, false>(a, grid, s);
-  }
-  return vec ? launch_step<DP, T, 2, true>(a, grid, s) : launch_step<DP, T, 2, false>(a, grid, s);
+  const int rows = a.tile_rows * a.tile_heads;
+  return rows <= 8    ? launch_step<DP, T, 1>(a, grid, vec, s)
+         : rows <= 16 ? launch_step<DP, T, 2>(a, grid, vec, s)
+                      : launch_step<DP, T, 4>(a, grid, vec, s);
 }
 
 int run_step(const ie_attention_desc* d, const ie_attention_mask* m, const AttentionArgs& base,
