@@ -61,7 +61,8 @@ def build_cuda(force: bool = False) -> Path:
         obj, deps = BUILD_DIR / (unit.stem + ".o"), BUILD_DIR / (unit.stem + ".d")
         read = [unit, *headers]
         if deps.exists():  # what the last compilation of this unit read
-            read = [Path(f) for f in deps.read_text().replace("\\\n", " ").split()[1:]]
+            listed = deps.read_text().replace("\\\n", " ").partition(":")[2]
+            read = [Path(f) for f in listed.split()]
             read = [f for f in read if ROOT in f.parents or not f.exists()]
         if force or not all(f.exists() for f in read) or not _newer(obj, read):
             _run([nvcc(), *NVCC_FLAGS, "-MMD", "-MF", deps, "-c", "-o", obj, unit])

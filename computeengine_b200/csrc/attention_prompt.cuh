@@ -1,15 +1,25 @@
 // Attention for many query rows on the tensor cores.
 //
-// One block works on 256 query rows of one head and sequence as two tiles of
-// 128, over the keys in tiles of 128:
+// One block works on two tiles of 128 query rows of one sequence, over the keys
+// in steps of 64:
 //   S = Q K^T            tcgen05.mma, both operands in shared memory, S in TMEM
 //   P = exp2(S - max)    one thread per row: the row's maximum and sum need no
 //                        exchange; P goes back over S in TMEM as 16-bit values
 //   O += P V             tcgen05.mma with P as the TMEM operand, O in TMEM
-// While the threads of one tile take their exponentials, the tensor core works
-// for the other one.  Warps 0-3 and 4-7 hold the rows of the tiles, warp 8
-// issues the MMAs, warp 9 the TMA loads of Q, K and V, warp 10 clears the rows
-// of V behind the sequence's end (0 * NaN would reach O).
+// The rows of a tile are 128 positions of one head, or, for few positions, all
+// positions of several heads that read the same kv head.
+//
+// Each tile has two S buffers, so the threads of a row always find the next S:
+// from P in TMEM to the next S there pass the MMAs and 400 cycles of latency,
+// which took a third of the time when a tile had one S of 128 keys.  The price
+// is that S of 64 keys costs 49 cycles per 16 elements of the head where half
+// of one of 128 keys costs 32 (Q is read from shared memory for each), so a
+// head of 128 runs at most at 79% of the tensor core's rate.  The exponentials
+// take 16 a cycle and SM; part of them is a polynomial on the FMA pipes.
+// Warps 0-3 and 4-7 hold the rows of the tiles, warps 8 and 9 issue their MMAs
+// (one thread for both tiles spent 2200 cycles a step on the waits between
+// them), warp 10 the TMA loads of Q, K and V, warp 11 clears the rows of V
+// behind the sequence's end (0 * NaN would reach O).
 #pragma once
 
 #include "attention_common.cuh"
@@ -21,9 +31,15 @@ constexpr unsigned kErrAttnQ = 0x201, kErrAttnKv = 0x202, kErrAttnEmpty = 0x203,
                    kErrAttnS = 0x204, kErrAttnP = 0x205, kErrAttnO = 0x206, kErrAttnFix = 0x207;
 
 constexpr int kPromptThreads = 384;
+constexpr int kStep = 64;      // keys per step
+constexpr int kPolyEvery = 4;  // one pair of exponentials in so many is a polynomial
 
 struct PromptArgs : AttentionArgs {
-  int tiles;           // blocks of 256 rows per (head, batch row), documents: upper bound
+  int tiles;           // blocks per (head unit, batch row), documents: upper bound in all
+  int head_units;      // blocks side by side: heads, or (packed) pairs of head tiles
+  int packed;          // a tile holds several heads of a kv head
+  int tile_rows;       // positions of a tile: 128, packed: q_len
+  int tile_heads;      // heads of a tile: 1, packed: tile_rows * tile_heads <= 128
   int splits;          // shares of each sequence's keys
   float* part_o;       // splits > 1: fp32 [splits][batch][q_heads][q_len][head_dim]
   float* part_lse;     //             fp32 [splits][batch][q_heads][q_len]
@@ -34,10 +50,104 @@ struct PromptArgs : AttentionArgs {
 template <int DP>
 struct PromptPlan {
   static constexpr int kCols = DP / 64;               // 128-byte wide column blocks of a tile
-  static constexpr int kTile = kCols * 128 * 128;     // bytes of a 128-row tile
-  static constexpr int kStages = DP == 128 ? 5 : 8;   // K and V tiles in flight
-  static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024 + 256;
+  static constexpr int kQ = kCols * 128 * 128;        // bytes of 128 rows of Q
+  static constexpr int kKv = kCols * kStep * 128;     // bytes of a step's K or V
+  static constexpr int kStages = DP == 128 ? 10 : 16; // K and V steps in flight
+  static constexpr int kSmem = 2 * kQ + kStages * kKv + 1024 + 512;
 };
+
+// True in one thread of the (converged) warp.  The compiler then knows that
+// one thread runs what follows: with `lane == 0` it walks the warp's active
+// threads around every MMA, which took 86 cycles an MMA instead of the 64 that
+// the tensor core needs for it.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "@p mov.b32 %0, 1;\n\t}"
+      : "+r"(yes));
+  return yes != 0;
+}
+
+// The warp's bounded wait, with every lane looking first: a phase that is
+// already complete costs one look and a vote instead of a branch to one lane.
+__device__ __forceinline__ bool wait_ready(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
+                                           unsigned site, uint64_t limit_ns) {
+  if (__all_sync(0xFFFFFFFFu, mbar_try_wait(bar, parity))) return true;
+  return mbar_wait_warp(bar, parity, abort_flag, site, limit_ns);
+}
+
+// ---- two fp32 values at once (one instruction each on sm_100)
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float* a, float* b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// 2^x for two values x <= 8 without the special function unit: x = n + f with
+// n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits) and f in
+// [-1/2, 1/2], 2^f by its minimax polynomial of degree 4 with 2^0 = 1 exactly
+// (relative error below 3e-6; the weights are rounded to 2^-9 or 2^-12), n
+// added to the exponent.  Below -127 the result is exactly 0.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  float a, b;
+  unpair(x, &a, &b);
+  x = pair_of(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
+  const uint64_t magic = pair_of(12582912.0f, 12582912.0f);
+  const uint64_t shifted = add2(x, magic);
+  const uint64_t n = add2(shifted, pair_of(-12582912.0f, -12582912.0f));
+  const uint64_t f = fma2(n, pair_of(-1.0f, -1.0f), x);
+  uint64_t p = fma2(f, pair_of(0.009582852944731712f, 0.009582852944731712f),
+                    pair_of(0.055906426161527634f, 0.055906426161527634f));
+  p = fma2(p, f, pair_of(0.24024099111557007f, 0.24024099111557007f));
+  p = fma2(p, f, pair_of(0.6931241750717163f, 0.6931241750717163f));
+  p = fma2(p, f, pair_of(1.0f, 1.0f));
+  float pa, pb, sa, sb;
+  unpair(p, &pa, &pb);
+  unpair(shifted, &sa, &sb);
+  return pair_of(__uint_as_float(__float_as_uint(pa) + (__float_as_uint(sa) << 23)),
+                 __uint_as_float(__float_as_uint(pb) + (__float_as_uint(sb) << 23)));
+}
+
+// tanh(u) / u for |u| <= kTanhLimit as a polynomial in u^2 (minimax of tanh u
+// with slope 1 at 0, absolute error below 2.7e-7).
+constexpr float kTanhLimit = 0.75f;
+__device__ __forceinline__ uint64_t tanh_ratio(uint64_t uu) {
+  uint64_t p = fma2(uu, pair_of(0.012750583700835705f, 0.012750583700835705f),
+                    pair_of(-0.04986608773469925f, -0.04986608773469925f));
+  p = fma2(p, uu, pair_of(0.13253363966941833f, 0.13253363966941833f));
+  p = fma2(p, uu, pair_of(-0.33328044414520264f, -0.33328044414520264f));
+  return fma2(p, uu, pair_of(1.0f, 1.0f));
+}
 
 template <int DP, int T, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(kPromptThreads, 1)
@@ -50,43 +160,59 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   // ---- which rows and keys
-  const int h = blockIdx.x % a.q_heads;
-  const int batch_row = blockIdx.x / a.q_heads % a.batch;
-  const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x / a.q_heads / a.batch);  // causal: longest first
+  const int unit = blockIdx.x % a.head_units;
+  const int batch_row = blockIdx.x / a.head_units % a.batch;
+  // causal: longest first
+  const int tile = a.tiles - 1 - static_cast<int>(blockIdx.x / a.head_units / a.batch);
   Sequence seq;
   int row0 = 0;
-  if (!tile_sequence(a, tile, batch_row, 256, &seq, &row0)) return;
+  if (!tile_sequence(a, tile, batch_row, a.packed ? a.tile_rows : 256, &seq, &row0)) return;
   const int length = seq.k1 - seq.k0;
-  // key tiles of each row tile: up to what its last row sees
-  int tiles_t[2];
+  const int heads_per_kv = a.q_heads / a.kv_heads;
+  // first head and position of each row tile; the kv head is the same
+  int head_t[2] = {unit, unit}, row_t[2] = {row0, row0 + 128}, hk = unit / heads_per_kv;
+  bool some_t[2] = {true, row0 + 128 < seq.q1};
+  if (a.packed) {
+    const int groups = heads_per_kv / a.tile_heads, pairs = (groups + 1) / 2;
+    hk = unit / pairs;
+    for (int t = 0; t < 2; ++t) {
+      const int group = unit % pairs * 2 + t;
+      head_t[t] = hk * heads_per_kv + group * a.tile_heads;
+      row_t[t] = row0;
+      some_t[t] = group < groups;
+    }
+  }
+  // steps of each row tile: up to what its last position sees
+  int steps_t[2];
   for (int t = 0; t < 2; ++t) {
-    const int last = min(row0 + 128 * (t + 1), seq.q1) - 1;
-    tiles_t[t] = row0 + 128 * t < seq.q1 ? (seq.seen(last, a.causal) + 127) / 128 : 0;
+    const int last = min(row_t[t] + a.tile_rows, seq.q1) - 1;
+    steps_t[t] = some_t[t] ? (seq.seen(last, a.causal) + kStep - 1) / kStep : 0;
   }
   int begin = 0;
-  {
-    const int all = max(tiles_t[0], tiles_t[1]);
+  if (a.splits > 1) {
+    const int all = max(steps_t[0], steps_t[1]);
     const int share = (all + a.splits - 1) / a.splits;
     begin = share * static_cast<int>(blockIdx.y);
-    for (int t = 0; t < 2; ++t) tiles_t[t] = max(0, min(tiles_t[t], begin + share) - begin);
+    for (int t = 0; t < 2; ++t) steps_t[t] = max(0, min(steps_t[t], begin + share) - begin);
   }
-  const int tiles = max(tiles_t[0], tiles_t[1]);
+  const int steps = max(steps_t[0], steps_t[1]);
 
   // ---- shared memory
   uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* q_tile = base;
-  uint8_t* ring = base + 2 * P::kTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kStages * P::kTile);
+  uint8_t* ring = base + 2 * P::kQ;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kStages * P::kKv);
   uint64_t* q_full = bars;                 // [2]
-  uint64_t* s_full = bars + 2;             // [2]
-  uint64_t* p_full = bars + 4;             // [2]
-  uint64_t* o_full = bars + 6;             // [2]
-  uint64_t* short_full = bars + 8;         // the last V tile, when it is cut short
-  uint64_t* fixed = bars + 9;              // and its rows behind the end are cleared
-  uint64_t* drain = bars + 10;
-  uint64_t* kv_full = bars + 11;           // [kStages]
-  uint64_t* kv_empty = bars + 11 + kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 11 + 2 * kStages);
+  uint64_t* s_full = bars + 2;             // [2][buffers]
+  uint64_t* p_full = bars + 6;             // [2][buffers]
+  uint64_t* o_done = bars + 10;            // [2] O += P V of a step
+  uint64_t* o_full = bars + 12;            // [2] O is complete
+  uint64_t* short_full = bars + 14;        // the last V, when it is cut short
+  uint64_t* fixed = bars + 15;             // and its rows behind the end are cleared
+  uint64_t* drain = bars + 16;             // [2]
+  uint64_t* kv_full = bars + 18;           // [kStages]
+  uint64_t* kv_empty = bars + 18 + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18 + 2 * kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* loads_issued = const_cast<int*>(abort_flag) + 1;
 
@@ -94,16 +220,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
         mbar_init(&q_full[i], 1);
-        mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 128);
+        mbar_init(&s_full[2 * i], 1);
+        mbar_init(&s_full[2 * i + 1], 1);
+        mbar_init(&p_full[2 * i], 4);
+        mbar_init(&p_full[2 * i + 1], 4);
+        mbar_init(&o_done[i], 1);
         mbar_init(&o_full[i], 1);
+        mbar_init(&drain[i], 1);
       }
       mbar_init(short_full, 1);
       mbar_init(fixed, 32);
-      mbar_init(drain, 1);
       for (int i = 0; i < kStages; ++i) {
         mbar_init(&kv_full[i], 1);
-        mbar_init(&kv_empty[i], 1);
+        mbar_init(&kv_empty[i], 2);  // both MMA warps
       }
       *abort_flag = 0;
       *loads_issued = 0;
@@ -113,7 +242,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 9 && lane == 0) {
+  if (warp == 10 && lane == 0) {
     tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_k);
     tma_prefetch_desc(&map_v);
@@ -122,120 +251,137 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns: S (and P over it) of tile t at 128 t, O at 256 + DP t
-  const bool last_short = length % 128 != 0 && begin + tiles == (length + 127) / 128;
-
+  // TMEM columns: S buffer b of tile t (and P over it) at 128 t + 64 b, O at
+  // 256 + DP t
+  const bool last_short =
+      length % kStep != 0 && begin + steps == (length + kStep - 1) / kStep;
+  const int total = 2 * steps;  // loads of K and V
+  // The ring's order is the MMAs': K0, K1, then V of a step and K of the step
+  // two ahead.
   if (warp >= 8) {
     setmaxnreg_dec<56>();
-    if (warp == 9 && lane == 0) {
+    if (warp == 10 && elect_one()) {
       // ------------------------------------------------ TMA loads
-      const int hk = static_cast<int>(static_cast<int64_t>(h) * a.kv_heads / a.q_heads);
-      bool ok = tiles > 0;
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (tiles_t[t] == 0) continue;
-        mbar_arrive_expect_tx(&q_full[t], P::kTile);
+      for (int t = 0; t < 2; ++t) {
+        if (steps_t[t] == 0) continue;
+        mbar_arrive_expect_tx(&q_full[t], P::kCols * a.tile_rows * a.tile_heads * 128);
         for (int c = 0; c < P::kCols; ++c) {
-          tma_load_4d(q_tile + t * P::kTile + c * 16384, &map_q, &q_full[t], 64 * c,
-                      row0 + 128 * t, h, seq.batch);
+          tma_load_4d(q_tile + t * P::kQ + c * 16384, &map_q, &q_full[t], 64 * c, row_t[t],
+                      head_t[t], seq.batch);
         }
       }
-      // ring order: K0, K1, V0, K2, V1, ... : V of a tile is needed after K of the next
-      int issued = 0;
-      const int total = 2 * tiles;
-      for (int i = 0; ok && i < total; ++i) {
-        // i = 0: K0; then pairs (K_{j+1}, V_j); the last V has no K before it
-        const bool is_k = i == 0 || (i % 2 == 1 && i < total - 1);
-        const int j = i == 0 ? 0 : is_k ? (i + 1) / 2 : i == total - 1 ? tiles - 1 : i / 2 - 1;
-        const int s = i % kStages;
-        if (!mbar_wait(&kv_empty[s], ((i / kStages) & 1) ^ 1u, abort_flag, kErrAttnEmpty,
-                       a.wait_limit_ns)) {
-          break;
-        }
-        // a barrier of its own lets warp 10 wait for this load from the start
-        uint64_t* full = last_short && i == total - 1 ? short_full : &kv_full[s];
-        mbar_arrive_expect_tx(full, P::kTile);
-        const int row = seq.k0 + (begin + j) * 128;
+      int issued = 0, slot = 0;
+      uint32_t phase = 1;
+      for (int i = 0; i < total; ++i) {
+        const bool is_k = i < 2 ? i < steps : i % 2 == 1 && i < total - 1;
+        const int s = i < 2 ? (is_k ? i : 0) : is_k ? (i + 1) / 2
+                      : i == total - 1 ? steps - 1 : i / 2 - 1;
+        if (!mbar_wait(&kv_empty[slot], phase, abort_flag, kErrAttnEmpty, a.wait_limit_ns)) break;
+        // a barrier of its own lets warp 11 wait for this load from the start
+        uint64_t* full = last_short && i == total - 1 ? short_full : &kv_full[slot];
+        mbar_arrive_expect_tx(full, P::kKv);
+        const int row = seq.k0 + (begin + s) * kStep;
         for (int c = 0; c < P::kCols; ++c) {
-          tma_load_4d(ring + s * P::kTile + c * 16384, is_k ? &map_k : &map_v, full, 64 * c,
-                      row, hk, seq.batch);
+          tma_load_4d(ring + slot * P::kKv + c * (kStep * 128), is_k ? &map_k : &map_v, full,
+                      64 * c, row, hk, seq.batch);
         }
         issued = i + 1;
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1u;
+        }
       }
       *loads_issued = issued;
-    } else if (warp == 8 && lane == 0) {
-      // ------------------------------------------------ MMA issuer
+    } else if (warp < 10 && elect_one()) {
+      // ------------------------------------------------ MMAs of tile t
+      const int t = warp - 8, n = steps_t[t];
       const int ksteps = (a.head_dim + 15) / 16;
-      const uint32_t idesc_s = make_idesc_f16(128, 128, T == IE_DT_BF16, false);
+      const uint32_t idesc_s = make_idesc_f16(128, kStep, T == IE_DT_BF16, false);
       const uint32_t idesc_o = make_idesc_f16(128, ksteps * 16, T == IE_DT_BF16, true);
-      const uint64_t q_desc = make_smem_desc(smem_u32(q_tile), 16, 1024, 2);
+      const uint64_t q_desc = make_smem_desc(smem_u32(q_tile + t * P::kQ), 16, 1024, 2);
       const uint64_t k_desc = make_smem_desc(smem_u32(ring), 16, 1024, 2);
-      const uint64_t v_desc = make_smem_desc(smem_u32(ring), 16384, 1024, 2);
-      bool ok = tiles > 0;
-      auto wait_kv = [&](int i) {
-        return mbar_wait(&kv_full[i % kStages], (i / kStages) & 1, abort_flag, kErrAttnKv,
-                         a.wait_limit_ns);
-      };
-      auto scores = [&](int t, int i) {  // S_t = Q_t K^T, K in ring slot of load i
-        const uint64_t qd = q_desc + ((t * P::kTile) >> 4);
-        const uint64_t kd = k_desc + (((i % kStages) * P::kTile) >> 4);
-        for (int s = 0; s < ksteps; ++s) {
-          const uint64_t at = ((s / 4) * 16384 + (s % 4) * 32) >> 4;
-          mma_f16(tmem + 128 * t, qd + at, kd + at, idesc_s, s > 0);
-        }
-        tc_commit(&s_full[t]);
-      };
-      auto outputs = [&](int t, int i, bool add) {  // O_t += P_t V, V in ring slot of load i
-        const uint64_t vd = v_desc + (((i % kStages) * P::kTile) >> 4);
-        for (int s = 0; s < 8; ++s) {
-          mma_f16_ta(tmem + 256 + DP * t, tmem + 128 * t + 8 * s, vd + ((s * 2048) >> 4), idesc_o,
-                     add || s > 0);
+      const uint64_t v_desc = make_smem_desc(smem_u32(ring), kStep * 128, 1024, 2);
+      const uint32_t s_tmem = tmem + 128 * t, o_tmem = tmem + 256 + DP * t;
+      int slot = 0;
+      uint32_t phase = 0;
+      auto advance = [&] {
+        if (++slot == kStages) {
+          slot = 0;
+          phase ^= 1u;
         }
       };
-      // load index of K_j and V_j in the ring's order
-      auto k_at = [&](int j) { return j == 0 ? 0 : 2 * j - 1; };
-      auto v_at = [&](int j) { return j == tiles - 1 ? 2 * tiles - 1 : 2 * j + 2; };
-      for (int t = 0; t < 2 && ok; ++t) {
-        if (tiles_t[t] == 0) continue;
-        ok = mbar_wait(&q_full[t], 0, abort_flag, kErrAttnQ, a.wait_limit_ns) && wait_kv(0);
-        if (ok) scores(t, 0);
-      }
-      if (ok) tc_commit(&kv_empty[0]);
-      for (int j = 0; ok && j < tiles; ++j) {
-        if (j + 1 < tiles) ok = wait_kv(k_at(j + 1));
-        if (last_short && j == tiles - 1) {
-          ok = ok && mbar_wait(fixed, 0, abort_flag, kErrAttnFix, a.wait_limit_ns);
-        } else {
-          ok = ok && wait_kv(v_at(j));
-        }
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= tiles_t[t]) continue;
-          ok = mbar_wait(&p_full[t], j & 1, abort_flag, kErrAttnP, a.wait_limit_ns);
-          if (!ok) break;
-          tc_fence_after();
-          outputs(t, v_at(j), j > 0);
-          if (j + 1 < tiles_t[t]) {
-            scores(t, k_at(j + 1));
-          } else {
-            tc_commit(&o_full[t]);
+      auto wait_slot = [&] {
+        return mbar_wait(&kv_full[slot], phase, abort_flag, kErrAttnKv, a.wait_limit_ns);
+      };
+      // the slot is free once this tile's MMAs so far are done, or at once
+      auto release = [&](int i, bool used) {
+        if (used) tc_commit(&kv_empty[i]);
+        else mbar_arrive(&kv_empty[i]);
+      };
+      // Unrolled: an MMA takes 33 to 65 cycles, a loop around it up to 86.
+      auto scores = [&](int s, int i) {  // S of step s = Q K^T, K in slot i
+        const uint64_t kd = k_desc + ((i * P::kKv) >> 4);
+        const uint32_t d = s_tmem + 64 * (s & 1);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          if (k < ksteps) {
+            mma_f16(d, q_desc + (((k / 4) * 16384 + (k % 4) * 32) >> 4),
+                    kd + (((k / 4) * (kStep * 128) + (k % 4) * 32) >> 4), idesc_s, k > 0);
           }
         }
+        tc_commit(&s_full[2 * t + (s & 1)]);
+      };
+      bool ok = n == 0 || mbar_wait(&q_full[t], 0, abort_flag, kErrAttnQ, a.wait_limit_ns);
+      for (int s = 0; ok && s < 2 && s < steps; ++s) {
+        ok = wait_slot();
         if (!ok) break;
-        if (j + 1 < tiles) tc_commit(&kv_empty[k_at(j + 1) % kStages]);
-        tc_commit(&kv_empty[v_at(j) % kStages]);
+        if (s < n) scores(s, slot);
+        release(slot, s < n);
+        advance();
+      }
+      for (int s = 0; ok && s < steps; ++s) {
+        const int vi = slot;
+        ok = last_short && s == steps - 1
+                 ? mbar_wait(fixed, 0, abort_flag, kErrAttnFix, a.wait_limit_ns)
+                 : wait_slot();
+        advance();
+        const int ki = slot;
+        if (s + 2 < steps) {
+          ok = ok && wait_slot();
+          advance();
+        }
+        if (ok && s < n) {
+          ok = mbar_wait(&p_full[2 * t + (s & 1)], (s >> 1) & 1, abort_flag, kErrAttnP,
+                         a.wait_limit_ns);
+        }
+        if (!ok) break;
+        if (s < n) {
+          tc_fence_after();
+          const uint64_t vd = v_desc + ((vi * P::kKv) >> 4);
+          const uint32_t p = s_tmem + 64 * (s & 1);
+#pragma unroll
+          for (int k = 0; k < kStep / 16; ++k) {
+            mma_f16_ta(o_tmem, p + 8 * k, vd + ((k * 2048) >> 4), idesc_o, s > 0 || k > 0);
+          }
+          tc_commit(&o_done[t]);
+          if (s + 2 < n) scores(s + 2, ki);
+          if (s + 1 == n) tc_commit(&o_full[t]);
+        }
+        release(vi, s < n);
+        if (s + 2 < steps) release(ki, s < n);
       }
       // every MMA done before tensor memory is released, on the abort path too
-      tc_commit(drain);
+      tc_commit(&drain[t]);
       int dummy_abort = 0;
-      mbar_wait(drain, 0, &dummy_abort, kErrAttnO, a.wait_limit_ns);
-    } else if (warp == 10 && last_short && tiles > 0) {
+      mbar_wait(&drain[t], 0, &dummy_abort, kErrAttnO, a.wait_limit_ns);
+    } else if (warp == 11 && last_short && steps > 0) {
       // ------------------------------------------------ rows of V behind the end
-      const int i = 2 * tiles - 1, s = i % kStages;  // the last load is the last tile's V
       if (mbar_wait_warp(short_full, 0, abort_flag, kErrAttnKv, a.wait_limit_ns)) {
-        uint8_t* v = ring + s * P::kTile;
-        const int from = length % 128;
-        for (int e = lane; e < (128 - from) * 8 * P::kCols; e += 32) {
-          const int c = e / ((128 - from) * 8), r = e % ((128 - from) * 8);
-          *reinterpret_cast<uint4*>(v + c * 16384 + from * 128 + r * 16) = make_uint4(0, 0, 0, 0);
+        uint8_t* v = ring + (total - 1) % kStages * P::kKv;  // the last load
+        const int from = length % kStep, pieces = (kStep - from) * 8;
+        for (int e = lane; e < pieces * P::kCols; e += 32) {
+          *reinterpret_cast<uint4*>(v + e / pieces * (kStep * 128) + from * 128 +
+                                    e % pieces * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_proxy_async_smem();
         mbar_arrive(fixed);
@@ -245,68 +391,110 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // ------------------------------------------------ rows
     setmaxnreg_inc<224>();
     const int t = warp >> 2;
-    const int row = row0 + 128 * t + (threadIdx.x & 127);
+    const int r = threadIdx.x & 127;
+    const int row = row_t[t] + r % a.tile_rows, h = head_t[t] + r / a.tile_rows;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + 128 * t + lanes, o_at = tmem + 256 + DP * t + lanes;
-    const bool valid = row < seq.q1;
+    const bool valid = some_t[t] && r < a.tile_rows * a.tile_heads && row < seq.q1;
     const int seen = valid ? seq.seen(row, a.causal) : 0;
-    // what every row of this tile sees, and what the sequence's rows are biased by
-    const int all_see =
-        row0 + 128 * t < seq.q1 ? seq.seen(row0 + 128 * t, a.causal) : 0;
+    // what every row of this tile sees, and the first row's place
+    const int all_see = some_t[t] ? seq.seen(row_t[t], a.causal) : 0;
+    const int all_past = some_t[t] ? seq.place(row_t[t]) : 0;
     constexpr float kLog2e = 1.4426950408889634f;
     const float scale = a.scale * kLog2e;
-    const float cap_in = CAP ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+    const float cap_arg = CAP ? a.scale / a.softcap : 0.0f;
     const float cap_out = CAP ? a.softcap * kLog2e : 0.0f;
-    const float slope = BIAS && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.0f;
+    // scores up to here go through the polynomial
+    const float cap_limit = CAP ? kTanhLimit / fabsf(cap_arg) : 0.0f;
+    const float slope = BIAS && valid && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.0f;
     const float place = static_cast<float>(valid ? seq.place(row) : 0);
     // x is the score in units of log2 e (plain: before the scale)
     constexpr bool kScaled = CAP || BIAS;
     const float to_log2 = kScaled ? 1.0f : scale;
+    // cap * tanh(s / cap) = cap * (1 - 2 / (1 + exp(2 s / cap)))
+    auto capped = [&](float s) {
+      const float u = ex2(s * (2.0f * kLog2e * cap_arg));
+      return cap_out - __fdividef(2.0f * cap_out, 1.0f + u);
+    };
+    auto capped_pair = [&](uint64_t s) {
+      const uint64_t u = mul2(s, pair_of(cap_arg, cap_arg));
+      return mul2(mul2(u, pair_of(cap_out, cap_out)), tanh_ratio(mul2(u, u)));
+    };
 
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
-    const int n = tiles_t[t];
-    for (int j = 0; j < n; ++j) {
-      if (!mbar_wait_warp(&s_full[t], j & 1, abort_flag, kErrAttnS, a.wait_limit_ns)) {
+    const int n = steps_t[t];
+    for (int s = 0; s < n; ++s) {
+      if (!wait_ready(&s_full[2 * t + (s & 1)], (s >> 1) & 1, abort_flag, kErrAttnS,
+                      a.wait_limit_ns)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      uint32_t sr[4][32];
+      const uint32_t s_now = s_at + 64 * (s & 1);
+      const int key0 = (begin + s) * kStep;
+      float x[kStep];
+      {
+        uint32_t sr[2][32];
+        tmem_ld_32x32b_x32(s_now, sr[0]);
+        tmem_ld_32x32b_x32(s_now + 32, sr[1]);
+        tmem_ld_wait(sr[0]);
+        tmem_ld_wait(sr[1]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_at + 32 * c, sr[c]);
-      const int key0 = (begin + j) * 128;
-      float x[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_ld_wait(sr[c]);
-#pragma unroll
-        for (int e = 0; e < 32; ++e) x[32 * c + e] = __uint_as_float(sr[c][e]);
+        for (int e = 0; e < kStep; ++e) x[e] = __uint_as_float(sr[e / 32][e % 32]);
       }
       if constexpr (CAP) {
+        float hi = x[0], lo = x[0];
 #pragma unroll
-        for (int e = 0; e < 128; ++e) {
-          // cap * tanh(s / cap) = cap * (1 - 2 / (1 + exp(2 s / cap)))
-          const float u = ex2(x[e] * cap_in);
-          x[e] = cap_out - __fdividef(2.0f * cap_out, 1.0f + u);
+        for (int e = 0; e < kStep; e += 2) {
+          hi = max3(hi, x[e], x[e + 1]);
+          lo = min3(lo, x[e], x[e + 1]);
         }
-      } else if constexpr (BIAS) {
+        // NaN takes the exact way
+        const bool small = hi <= cap_limit && lo >= -cap_limit;
+        if (__all_sync(0xFFFFFFFFu, small)) {
 #pragma unroll
-        for (int e = 0; e < 128; ++e) x[e] *= scale;
+          for (int e = 0; e < kStep; e += 2) {
+            unpair(capped_pair(pair_of(x[e], x[e + 1])), &x[e], &x[e + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kStep; ++e) x[e] = capped(x[e]);
+        }
       }
       if constexpr (BIAS) {
         const float from = place - static_cast<float>(key0);
+        const float factor = CAP ? 1.0f : scale;
+        if (all_past >= key0 + kStep - 1) {  // no key lies ahead of its row
+          const uint64_t f2 = pair_of(factor, factor), s2 = pair_of(slope, slope);
+          const uint64_t c2 = pair_of(-slope * from, -slope * from);
 #pragma unroll
-        for (int e = 0; e < 128; ++e) x[e] -= slope * fabsf(from - static_cast<float>(e));
+          for (int e = 0; e < kStep; e += 2) {
+            const uint64_t c =
+                fma2(s2, pair_of(static_cast<float>(e), static_cast<float>(e + 1)), c2);
+            const uint64_t y = CAP ? add2(pair_of(x[e], x[e + 1]), c)
+                                   : fma2(pair_of(x[e], x[e + 1]), f2, c);
+            unpair(y, &x[e], &x[e + 1]);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kStep; ++e) {
+            x[e] = x[e] * factor - slope * fabsf(from - static_cast<float>(e));
+          }
+        }
       }
-      if (key0 + 128 > all_see) {
+      if (key0 + kStep > all_see) {
         const int vis = seen - key0;
 #pragma unroll
-        for (int e = 0; e < 128; ++e) x[e] = e < vis ? x[e] : -INFINITY;
+        for (int e = 0; e < kStep; ++e) x[e] = e < vis ? x[e] : -INFINITY;
       }
-      float top = m;
+      float hi[4] = {m, m, m, m};
 #pragma unroll
-      for (int e = 0; e < 128; ++e) top = max_nan(top, x[e]);
+      for (int e = 0; e < kStep; e += 8) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) hi[c] = max3(hi[c], x[e + 2 * c], x[e + 2 * c + 1]);
+      }
+      const float top = max_nan(max3(hi[0], hi[1], hi[2]), hi[3]);
       // The maximum in use moves only when it grew by more than 2^8: until then
       // the weights stay below 256, which both 16-bit types hold as well as 1.
       float factor = 1.0f;
@@ -315,40 +503,57 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         factor = m == -INFINITY ? 1.0f : ex2((m - top) * to_log2);
         m = top;
       }
-      if (j > 0 && __any_sync(0xFFFFFFFFu, moved)) {
-        // the tile's earlier O (S of this tile follows it in the tensor core's order)
+      if (s > 0 && __any_sync(0xFFFFFFFFu, moved)) {
         l *= factor;
+        // S of this step came after O += P V of the step two before, so at most
+        // the last one is still under way
+        if (!mbar_wait_warp(&o_done[t], (s - 1) & 1, abort_flag, kErrAttnO, a.wait_limit_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < DP / 32; ++c) {
-          uint32_t r[32];
-          tmem_ld_32x32b_x32(o_at + 32 * c, r);
-          tmem_ld_wait(r);
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(o_at + 32 * c, o);
+          tmem_ld_wait(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * factor);
-          tmem_st_32x32b_x32(o_at + 32 * c, r);
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+          tmem_st_32x32b_x32(o_at + 32 * c, o);
         }
       }
       const float base = m == -INFINITY ? 0.0f : m * to_log2;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t to2 = pair_of(to_log2, to_log2), base2 = pair_of(-base, -base);
+      uint64_t sum[2] = {0, 0};
+      uint32_t p[32];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t p[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) {
-          const float p0 = ex2(fmaf(x[64 * c + 2 * e], to_log2, -base));
-          const float p1 = ex2(fmaf(x[64 * c + 2 * e + 1], to_log2, -base));
-          sum[e & 1] += p0;
-          sum[2 + (e & 1)] += p1;
-          p[e] = pack_pair<T>(p0, p1);
+      for (int e = 0; e < 32; ++e) {
+        uint64_t y = pair_of(x[2 * e], x[2 * e + 1]);
+        y = kScaled ? add2(y, base2) : fma2(y, to2, base2);
+        if (e % kPolyEvery == kPolyEvery - 1) {
+          y = exp2_pair(y);
+        } else {
+          float y0, y1;
+          unpair(y, &y0, &y1);
+          y = pair_of(ex2(y0), ex2(y1));
         }
-        tmem_st_32x32b_x32(s_at + 32 * c, p);
+        sum[e & 1] = add2(sum[e & 1], y);
+        float p0, p1;
+        unpair(y, &p0, &p1);
+        p[e] = pack_pair<T>(p0, p1);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st_32x32b_x32(s_now, p);
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&p_full[t]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[2 * t + (s & 1)]);
+      float s0, s1;
+      unpair(add2(sum[0], sum[1]), &s0, &s1);
+      l += s0 + s1;
     }
-    if (n > 0 && ok) ok = mbar_wait_warp(&o_full[t], 0, abort_flag, kErrAttnO, a.wait_limit_ns);
+    if (n > 0 && ok) {
+      ok = mbar_wait_warp(&o_full[t], 0, abort_flag, kErrAttnO, a.wait_limit_ns);
+    }
     tc_fence_after();
     if (ok) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
@@ -370,15 +575,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         if (32 * c >= a.head_dim) break;
-        uint32_t r[32];
+        uint32_t acc[32];
         if (n > 0) {
-          tmem_ld_32x32b_x32(o_at + 32 * c, r);
-          tmem_ld_wait(r);
+          tmem_ld_32x32b_x32(o_at + 32 * c, acc);
+          tmem_ld_wait(acc);
         }
         if (valid) {
           float y[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y[e] = none ? 0.0f : __uint_as_float(r[e]) * inv;
+          for (int e = 0; e < 32; ++e) y[e] = none ? 0.0f : __uint_as_float(acc[e]) * inv;
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             const int d = 32 * c + e;
@@ -422,11 +627,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     // no TMA load may still be writing this block's shared memory when it ends
     int dummy_abort = 0;
     for (int t = 0; t < 2; ++t) {
-      if (tiles_t[t] > 0) mbar_wait(&q_full[t], 0, &dummy_abort, kErrAttnQ, a.wait_limit_ns);
+      if (steps_t[t] > 0) mbar_wait(&q_full[t], 0, &dummy_abort, kErrAttnQ, a.wait_limit_ns);
     }
     const int issued = *loads_issued;
     for (int i = max(0, issued - kStages); i < issued; ++i) {
-      const bool cut = last_short && i == 2 * tiles - 1;
+      const bool cut = last_short && i == total - 1;
       mbar_wait(cut ? short_full : &kv_full[i % kStages], cut ? 0 : (i / kStages) & 1,
                 &dummy_abort, kErrAttnKv, a.wait_limit_ns);
     }

@@ -76,10 +76,10 @@ int check_attention(const ie_attention_desc* d, const ie_attention_mask* m) {
 constexpr int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
 constexpr int64_t round_up(int64_t v, int64_t m) { return ceil_div(v, m) * m; }
 
-// [batch, len, heads, head_dim] of 16-bit elements, loaded in boxes of 128 rows
-// x 64 elements; rows and elements outside read as zeros.
+// [batch, len, heads, head_dim] of 16-bit elements, loaded in boxes of 64
+// elements, box_len rows and box_heads heads; what lies outside reads as zeros.
 int encode_rows(CUtensorMap* map, const void* p, bool bf16, int64_t head_dim, int64_t len,
-                int64_t heads, int64_t batch, const int64_t* stride) {
+                int64_t heads, int64_t batch, const int64_t* stride, int box_len, int box_heads) {
   const DriverFns& f = driver_fns();
   if (!f.ok) return fail(IE_RUNTIME, "cuTensorMapEncodeTiled entry point unavailable");
   const int64_t extent[4] = {head_dim, len, heads, batch};
@@ -91,7 +91,9 @@ int encode_rows(CUtensorMap* map, const void* p, bool bf16, int64_t head_dim, in
     strides[i] = static_cast<cuuint64_t>(extent[i + 1] > 1 ? 2 * elements[i]
                                                            : round_up(2 * head_dim, 16));
   }
-  const cuuint32_t box[4] = {64, 128, 1, 1}, estrides[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_len),
+                             static_cast<cuuint32_t>(box_heads), 1};
+  const cuuint32_t estrides[4] = {1, 1, 1, 1};
   const CUresult r = f.tiled(
       map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
       const_cast<void*>(p), dims, strides, box, estrides, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -137,7 +139,7 @@ struct StepTiles {
 };
 
 bool few_rows(const ie_attention_desc* d, const ie_attention_mask* m) {
-  return (m == nullptr || m->documents == 0) && d->q_len * (d->q_heads / d->kv_heads) <= 32;
+  return (m == nullptr || m->documents == 0) && d->q_len * (d->q_heads / d->kv_heads) <= (getenv("FEWR") ? atoi(getenv("FEWR")) : 32);
 }
 
 StepTiles step_tiles(const ie_attention_desc* d, const ie_attention_mask* m) {
@@ -162,17 +164,32 @@ StepTiles step_tiles(const ie_attention_desc* d, const ie_attention_mask* m) {
   return t;
 }
 
-// The prompt kernel's blocks of 256 query rows, and into how many shares each
-// block's keys are cut when the blocks alone leave half of the GPU idle.
+// The prompt kernel's blocks of two row tiles, and into how many shares each
+// block's keys are cut when the blocks alone leave half of the GPU idle.  Up to
+// 64 positions and several heads per kv head: a tile holds all positions of as
+// many of those heads as fit 128 rows, so that their K and V are loaded once.
 struct PromptTiles {
   int64_t tiles;
+  int64_t head_units;
+  int rows, heads;
+  bool packed;
   int splits;
 };
 
 PromptTiles prompt_tiles(const ie_attention_desc* d, const ie_attention_mask* m) {
   const int64_t documents = m == nullptr ? 0 : m->documents;
-  PromptTiles p{documents > 0 ? d->q_len / 256 + documents : ceil_div(d->q_len, 256), 1};
-  const int64_t blocks = p.tiles * d->q_heads * d->batch;
+  PromptTiles p{documents > 0 ? d->q_len / 256 + documents : ceil_div(d->q_len, 256), d->q_heads,
+                128, 1, false, 1};
+  const int heads_per_kv = d->q_heads / d->kv_heads;
+  if (documents == 0 && d->q_len <= 64 && heads_per_kv > 1) {
+    p.packed = true;
+    p.rows = static_cast<int>(d->q_len);
+    for (int h = 1; h <= heads_per_kv && h * p.rows <= 128; ++h) {
+      if (heads_per_kv % h == 0) p.heads = h;
+    }
+    p.head_units = d->kv_heads * ceil_div(heads_per_kv / p.heads, 2);
+  }
+  const int64_t blocks = p.tiles * p.head_units * d->batch;
   const int64_t key_tiles = ceil_div(d->kv_len, 128);
   if (documents == 0 && blocks * 2 <= kSms && key_tiles >= 8) {
     p.splits = static_cast<int>(std::min(kSms / blocks, key_tiles / 4));
@@ -274,21 +291,25 @@ int run_prompt(const ie_attention_desc* d, const ie_attention_mask* m, const Att
   PromptArgs a{};
   static_cast<AttentionArgs&>(a) = base;
   const PromptTiles t = prompt_tiles(d, m);
-  const int64_t blocks = t.tiles * d->q_heads * d->batch;
+  const int64_t blocks = t.tiles * t.head_units * d->batch;
   if (blocks > INT_MAX) return fail(IE_UNSUPPORTED, "Attention has too many rows");
   const bool bf16 = d->type == IE_DT_BF16;
   CUtensorMap maps[3];
   int rc = encode_rows(&maps[0], a.q, bf16, d->head_dim, d->q_len, d->q_heads, d->batch,
-                       d->q_stride);
+                       d->q_stride, t.rows, t.heads);
   if (rc == IE_OK) {
     rc = encode_rows(&maps[1], a.k, bf16, d->head_dim, d->kv_len, d->kv_heads, d->batch,
-                     d->k_stride);
+                     d->k_stride, kStep, 1);
   }
   if (rc == IE_OK) {
     rc = encode_rows(&maps[2], a.v, bf16, d->head_dim, d->kv_len, d->kv_heads, d->batch,
-                     d->v_stride);
+                     d->v_stride, kStep, 1);
   }
   if (rc != IE_OK) return rc;
+  a.head_units = static_cast<int>(t.head_units);
+  a.packed = t.packed;
+  a.tile_rows = t.rows;
+  a.tile_heads = t.heads;
   a.tiles = static_cast<int>(t.tiles);
   a.splits = t.splits;
   const int64_t rows = d->batch * d->q_heads * d->q_len * a.splits;
