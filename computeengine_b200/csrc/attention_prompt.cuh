@@ -52,8 +52,9 @@ struct PromptPlan {
   static constexpr int kCols = DP / 64;               // 128-byte wide column blocks of a tile
   static constexpr int kQ = kCols * 128 * 128;        // bytes of 128 rows of Q
   static constexpr int kKv = kCols * kStep * 128;     // bytes of a step's K or V
-  static constexpr int kStages = DP == 128 ? 10 : 16; // K and V steps in flight
-  static constexpr int kSmem = 2 * kQ + kStages * kKv + 1024 + 512;
+  static constexpr int kSlot = 2 * kKv;               // V of a step, K of the step two ahead
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kSmem = 2 * kQ + kStages * kSlot + 1024 + 512;
 };
 
 // True in one thread of the (converged) warp.  The compiler then knows that
@@ -68,6 +69,26 @@ __device__ __forceinline__ bool elect_one() {
       "@p mov.b32 %0, 1;\n\t}"
       : "+r"(yes));
   return yes != 0;
+}
+
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
 }
 
 // The warp's bounded wait, with every lane looking first: a phase that is
@@ -201,51 +222,68 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint8_t* base = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* q_tile = base;
   uint8_t* ring = base + 2 * P::kQ;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kStages * P::kKv);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kStages * P::kSlot);
   uint64_t* q_full = bars;                 // [2]
   uint64_t* s_full = bars + 2;             // [2][buffers]
   uint64_t* p_full = bars + 6;             // [2][buffers]
-  uint64_t* o_done = bars + 10;            // [2] O += P V of a step
-  uint64_t* o_full = bars + 12;            // [2] O is complete
-  uint64_t* short_full = bars + 14;        // the last V, when it is cut short
-  uint64_t* fixed = bars + 15;             // and its rows behind the end are cleared
-  uint64_t* drain = bars + 16;             // [2]
-  uint64_t* kv_full = bars + 18;           // [kStages]
-  uint64_t* kv_empty = bars + 18 + kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18 + 2 * kStages);
+  uint64_t* short_full = bars + 10;        // the last V, when it is cut short
+  uint64_t* fixed = bars + 11;             // and its rows behind the end are cleared
+  uint64_t* drain = bars + 12;             // [2]
+  uint64_t* kv_full = bars + 14;           // [kStages]
+  uint64_t* kv_empty = bars + 14 + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14 + 2 * kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* loads_issued = const_cast<int*>(abort_flag) + 1;
 
-  if (warp == 8) {
-    if (lane == 0) {
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&q_full[i], 1);
-        mbar_init(&s_full[2 * i], 1);
-        mbar_init(&s_full[2 * i + 1], 1);
-        mbar_init(&p_full[2 * i], 4);
-        mbar_init(&p_full[2 * i + 1], 4);
-        mbar_init(&o_done[i], 1);
-        mbar_init(&o_full[i], 1);
-        mbar_init(&drain[i], 1);
-      }
-      mbar_init(short_full, 1);
-      mbar_init(fixed, 32);
-      for (int i = 0; i < kStages; ++i) {
-        mbar_init(&kv_full[i], 1);
-        mbar_init(&kv_empty[i], 2);  // both MMA warps
-      }
-      *abort_flag = 0;
-      *loads_issued = 0;
-      fence_mbar_init();
+  const bool last_short =
+      length % kStep != 0 && begin + steps == (length + kStep - 1) / kStep;
+  // A slot of the ring holds what a tile's MMAs wait for together: K of the
+  // first two steps, then V of a step and K of the step two ahead.
+  const int slots = steps > 0 ? steps + 1 : 0;
+  auto load_slot = [&](int i, int slot) {
+    // a barrier of its own lets warp 11 wait for the last load from the start
+    uint64_t* full = last_short && i == slots - 1 ? short_full : &kv_full[slot];
+    const int first = i == 0 ? 0 : i - 1, second = i + 1;  // steps of the two halves
+    mbar_arrive_expect_tx(full, second < steps ? 2 * P::kKv : P::kKv);
+    uint8_t* to = ring + slot * P::kSlot;
+    for (int c = 0; c < P::kCols; ++c) {
+      tma_load_4d(to + c * (kStep * 128), i == 0 ? &map_k : &map_v, full, 64 * c,
+                  seq.k0 + (begin + first) * kStep, hk, seq.batch);
     }
-    __syncwarp();
+    for (int c = 0; c < P::kCols && second < steps; ++c) {
+      tma_load_4d(to + P::kKv + c * (kStep * 128), &map_k, full, 64 * c,
+                  seq.k0 + (begin + second) * kStep, hk, seq.batch);
+    }
+  };
+  if (warp == 8) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
-  }
-  if (warp == 10 && lane == 0) {
-    tma_prefetch_desc(&map_q);
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
+  } else if (warp == 10) {
+    // barriers 0 .. 13 + 2 kStages in their order above, one per lane
+    for (int i = lane; i < 14 + 2 * kStages; i += 32) {
+      mbar_init(&bars[i], i >= 6 && i < 10 ? 4           // p_full: a lane of each warp
+                          : i == 11        ? 32          // fixed
+                          : i >= 14 + kStages ? 2        // kv_empty: both MMA warps
+                                              : 1);
+    }
+    if (lane == 0) {
+      *abort_flag = 0;
+      *loads_issued = 0;
+    }
+    fence_mbar_init();
+    __syncwarp();
+    if (elect_one()) {  // the first loads need no other warp
+      for (int i = 0; i < min(slots, kStages); ++i) {
+        if (i < 2 && steps_t[i] > 0) {
+          mbar_arrive_expect_tx(&q_full[i], P::kCols * a.tile_rows * a.tile_heads * 128);
+          for (int c = 0; c < P::kCols; ++c) {
+            tma_load_4d(q_tile + i * P::kQ + c * 16384, &map_q, &q_full[i], 64 * c, row_t[i],
+                        head_t[i], seq.batch);
+          }
+        }
+        load_slot(i, i);
+      }
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -253,38 +291,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const uint32_t tmem = *tmem_slot;
   // TMEM columns: S buffer b of tile t (and P over it) at 128 t + 64 b, O at
   // 256 + DP t
-  const bool last_short =
-      length % kStep != 0 && begin + steps == (length + kStep - 1) / kStep;
-  const int total = 2 * steps;  // loads of K and V
-  // The ring's order is the MMAs': K0, K1, then V of a step and K of the step
-  // two ahead.
+
   if (warp >= 8) {
-    setmaxnreg_dec<56>();
+    setmaxnreg_dec<120>();
     if (warp == 10 && elect_one()) {
       // ------------------------------------------------ TMA loads
-      for (int t = 0; t < 2; ++t) {
-        if (steps_t[t] == 0) continue;
-        mbar_arrive_expect_tx(&q_full[t], P::kCols * a.tile_rows * a.tile_heads * 128);
-        for (int c = 0; c < P::kCols; ++c) {
-          tma_load_4d(q_tile + t * P::kQ + c * 16384, &map_q, &q_full[t], 64 * c, row_t[t],
-                      head_t[t], seq.batch);
-        }
-      }
-      int issued = 0, slot = 0;
-      uint32_t phase = 1;
-      for (int i = 0; i < total; ++i) {
-        const bool is_k = i < 2 ? i < steps : i % 2 == 1 && i < total - 1;
-        const int s = i < 2 ? (is_k ? i : 0) : is_k ? (i + 1) / 2
-                      : i == total - 1 ? steps - 1 : i / 2 - 1;
+      int issued = min(slots, kStages), slot = 0;
+      uint32_t phase = 0;
+      for (int i = kStages; i < slots; ++i) {
         if (!mbar_wait(&kv_empty[slot], phase, abort_flag, kErrAttnEmpty, a.wait_limit_ns)) break;
-        // a barrier of its own lets warp 11 wait for this load from the start
-        uint64_t* full = last_short && i == total - 1 ? short_full : &kv_full[slot];
-        mbar_arrive_expect_tx(full, P::kKv);
-        const int row = seq.k0 + (begin + s) * kStep;
-        for (int c = 0; c < P::kCols; ++c) {
-          tma_load_4d(ring + slot * P::kKv + c * (kStep * 128), is_k ? &map_k : &map_v, full,
-                      64 * c, row, hk, seq.batch);
-        }
+        load_slot(i, slot);
         issued = i + 1;
         if (++slot == kStages) {
           slot = 0;
@@ -310,17 +326,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           phase ^= 1u;
         }
       };
-      auto wait_slot = [&] {
-        return mbar_wait(&kv_full[slot], phase, abort_flag, kErrAttnKv, a.wait_limit_ns);
-      };
       // the slot is free once this tile's MMAs so far are done, or at once
       auto release = [&](int i, bool used) {
         if (used) tc_commit(&kv_empty[i]);
         else mbar_arrive(&kv_empty[i]);
       };
       // Unrolled: an MMA takes 33 to 65 cycles, a loop around it up to 86.
-      auto scores = [&](int s, int i) {  // S of step s = Q K^T, K in slot i
-        const uint64_t kd = k_desc + ((i * P::kKv) >> 4);
+      auto scores = [&](int s, uint32_t k_offset) {  // S of step s = Q K^T
+        const uint64_t kd = k_desc + (k_offset >> 4);
         const uint32_t d = s_tmem + 64 * (s & 1);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
@@ -329,27 +342,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                     kd + (((k / 4) * (kStep * 128) + (k % 4) * 32) >> 4), idesc_s, k > 0);
           }
         }
-        tc_commit(&s_full[2 * t + (s & 1)]);
       };
       bool ok = n == 0 || mbar_wait(&q_full[t], 0, abort_flag, kErrAttnQ, a.wait_limit_ns);
-      for (int s = 0; ok && s < 2 && s < steps; ++s) {
-        ok = wait_slot();
-        if (!ok) break;
-        if (s < n) scores(s, slot);
-        release(slot, s < n);
-        advance();
-      }
-      for (int s = 0; ok && s < steps; ++s) {
-        const int vi = slot;
-        ok = last_short && s == steps - 1
-                 ? mbar_wait(fixed, 0, abort_flag, kErrAttnFix, a.wait_limit_ns)
-                 : wait_slot();
-        advance();
-        const int ki = slot;
-        if (s + 2 < steps) {
-          ok = ok && wait_slot();
+      if (ok && steps > 0) {
+        ok = mbar_wait(&kv_full[0], 0, abort_flag, kErrAttnKv, a.wait_limit_ns);
+        if (ok) {
+          for (int s = 0; s < 2; ++s) {
+            if (s < n) scores(s, s * P::kKv);
+            if (n > 0) tc_commit(&s_full[2 * t + s]);
+          }
+          release(0, n > 0);
           advance();
         }
+      }
+      for (int s = 0; ok && s < steps; ++s) {
+        ok = last_short && s == steps - 1
+                 ? mbar_wait(fixed, 0, abort_flag, kErrAttnFix, a.wait_limit_ns)
+                 : mbar_wait(&kv_full[slot], phase, abort_flag, kErrAttnKv, a.wait_limit_ns);
         if (ok && s < n) {
           ok = mbar_wait(&p_full[2 * t + (s & 1)], (s >> 1) & 1, abort_flag, kErrAttnP,
                          a.wait_limit_ns);
@@ -357,18 +366,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         if (!ok) break;
         if (s < n) {
           tc_fence_after();
-          const uint64_t vd = v_desc + ((vi * P::kKv) >> 4);
+          const uint64_t vd = v_desc + ((slot * P::kSlot) >> 4);
           const uint32_t p = s_tmem + 64 * (s & 1);
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k) {
             mma_f16_ta(o_tmem, p + 8 * k, vd + ((k * 2048) >> 4), idesc_o, s > 0 || k > 0);
           }
-          tc_commit(&o_done[t]);
-          if (s + 2 < n) scores(s + 2, ki);
-          if (s + 1 == n) tc_commit(&o_full[t]);
+          if (s + 2 < n) scores(s + 2, slot * P::kSlot + P::kKv);
+          // S of step s + 2 is there, or (behind the last) just O += P V of step s
+          tc_commit(&s_full[2 * t + (s & 1)]);
         }
-        release(vi, s < n);
-        if (s + 2 < steps) release(ki, s < n);
+        release(slot, s < n);
+        advance();
       }
       // every MMA done before tensor memory is released, on the abort path too
       tc_commit(&drain[t]);
@@ -377,7 +386,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     } else if (warp == 11 && last_short && steps > 0) {
       // ------------------------------------------------ rows of V behind the end
       if (mbar_wait_warp(short_full, 0, abort_flag, kErrAttnKv, a.wait_limit_ns)) {
-        uint8_t* v = ring + (total - 1) % kStages * P::kKv;  // the last load
+        uint8_t* v = ring + (slots - 1) % kStages * P::kSlot;  // the last load
         const int from = length % kStep, pieces = (kStep - from) * 8;
         for (int e = lane; e < pieces * P::kCols; e += 32) {
           *reinterpret_cast<uint4*>(v + e / pieces * (kStep * 128) + from * 128 +
@@ -389,7 +398,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     // ------------------------------------------------ rows
-    setmaxnreg_inc<224>();
+    setmaxnreg_inc<192>();
     const int t = warp >> 2;
     const int r = threadIdx.x & 127;
     const int row = row_t[t] + r % a.tile_rows, h = head_t[t] + r / a.tile_rows;
@@ -424,6 +433,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     const int n = steps_t[t];
+#pragma unroll 1
     for (int s = 0; s < n; ++s) {
       if (!wait_ready(&s_full[2 * t + (s & 1)], (s >> 1) & 1, abort_flag, kErrAttnS,
                       a.wait_limit_ns)) {
@@ -444,14 +454,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         for (int e = 0; e < kStep; ++e) x[e] = __uint_as_float(sr[e / 32][e % 32]);
       }
       if constexpr (CAP) {
-        float hi = x[0], lo = x[0];
+        float hi[2] = {x[0], x[0]}, lo[2] = {x[0], x[0]};
 #pragma unroll
-        for (int e = 0; e < kStep; e += 2) {
-          hi = max3(hi, x[e], x[e + 1]);
-          lo = min3(lo, x[e], x[e + 1]);
+        for (int e = 0; e < kStep; e += 4) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            hi[c] = max3(hi[c], x[e + 2 * c], x[e + 2 * c + 1]);
+            lo[c] = min3(lo[c], x[e + 2 * c], x[e + 2 * c + 1]);
+          }
         }
         // NaN takes the exact way
-        const bool small = hi <= cap_limit && lo >= -cap_limit;
+        const bool small = max_nan(hi[0], hi[1]) <= cap_limit &&
+                           min3(lo[0], lo[1], lo[1]) >= -cap_limit;
         if (__all_sync(0xFFFFFFFFu, small)) {
 #pragma unroll
           for (int e = 0; e < kStep; e += 2) {
@@ -505,21 +519,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       if (s > 0 && __any_sync(0xFFFFFFFFu, moved)) {
         l *= factor;
-        // S of this step came after O += P V of the step two before, so at most
-        // the last one is still under way
-        if (!mbar_wait_warp(&o_done[t], (s - 1) & 1, abort_flag, kErrAttnO, a.wait_limit_ns)) {
+        // the next step's S comes after O += P V of the step before this one
+        if (!wait_ready(&s_full[2 * t + ((s + 1) & 1)], ((s + 1) >> 1) & 1, abort_flag, kErrAttnO,
+                        a.wait_limit_ns)) {
           ok = false;
           break;
         }
         tc_fence_after();
 #pragma unroll 1
-        for (int c = 0; c < DP / 32; ++c) {
-          uint32_t o[32];
-          tmem_ld_32x32b_x32(o_at + 32 * c, o);
+        for (int c = 0; c < DP / 16; ++c) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(o_at + 16 * c, o);
           tmem_ld_wait(o);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-          tmem_st_32x32b_x32(o_at + 32 * c, o);
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+          tmem_st_32x32b_x16(o_at + 16 * c, o);
         }
       }
       const float base = m == -INFINITY ? 0.0f : m * to_log2;
@@ -552,7 +566,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       l += s0 + s1;
     }
     if (n > 0 && ok) {
-      ok = mbar_wait_warp(&o_full[t], 0, abort_flag, kErrAttnO, a.wait_limit_ns);
+      // what follows the last step's O += P V
+      ok = wait_ready(&s_full[2 * t + ((n + 1) & 1)], ((n + 1) >> 1) & 1, abort_flag, kErrAttnO,
+                      a.wait_limit_ns);
     }
     tc_fence_after();
     if (ok) {
@@ -571,7 +587,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const int64_t oo = static_cast<int64_t>(seq.batch) * a.o_stride[0] +
                          static_cast<int64_t>(row) * a.o_stride[1] +
                          static_cast<int64_t>(h) * a.o_stride[2];
-      float* part = a.splits > 1 ? a.part_o + (blockIdx.y * part_rows + at) * a.head_dim : nullptr;
+      const float* part = a.splits > 1 ? a.part_o + (blockIdx.y * part_rows + at) * a.head_dim
+                                       : nullptr;
+      // 32 columns at a time through the warp's share of the tile's Q (its MMAs
+      // are done): a row's pieces are written side by side by neighbouring
+      // threads, not by the one thread that holds the row.
+      uint8_t* stage = q_tile + t * P::kQ + (warp & 3) * 4096;
+      // 32 rows of `pieces` 16-byte pieces each; row r of `to` is lane r's
+      auto write_rows = [&](int pieces, uint64_t to, int limit) {
+        __syncwarp();
+        const int c = lane % pieces;
+#pragma unroll 1
+        for (int r0 = lane / pieces; r0 < 32; r0 += 32 / pieces) {
+          const uint64_t to_r = __shfl_sync(0xFFFFFFFFu, to, r0);
+          const bool write = __shfl_sync(0xFFFFFFFFu, static_cast<int>(valid), r0) != 0;
+          if (write && c < limit) {
+            *reinterpret_cast<uint4*>(to_r + 16 * c) =
+                *reinterpret_cast<const uint4*>(stage + (r0 * pieces + (c ^ (r0 & (pieces - 1)))) * 16);
+          }
+        }
+        __syncwarp();
+      };
+      auto put = [&](int pieces, int c, uint4 v) {
+        *reinterpret_cast<uint4*>(stage + (lane * pieces + (c ^ (lane & (pieces - 1)))) * 16) = v;
+      };
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
         if (32 * c >= a.head_dim) break;
@@ -580,39 +619,51 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           tmem_ld_32x32b_x32(o_at + 32 * c, acc);
           tmem_ld_wait(acc);
         }
-        if (valid) {
-          float y[32];
+        float y[32];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) y[e] = none ? 0.0f : __uint_as_float(acc[e]) * inv;
+        for (int e = 0; e < 32; ++e) y[e] = none ? 0.0f : __uint_as_float(acc[e]) * inv;
+        const int left = a.head_dim - 32 * c;  // a multiple of 8
+        if (a.splits > 1) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            const int d = 32 * c + e;
-            if (d >= a.head_dim) break;  // head_dim is a multiple of 8 here
-            if (a.splits > 1) {
-              for (int f = 0; f < 8; ++f) part[d + f] = y[e + f];
-              continue;
+          for (int e = 0; e < 8; ++e) {
+            put(8, e, make_uint4(__float_as_uint(y[4 * e]), __float_as_uint(y[4 * e + 1]),
+                                 __float_as_uint(y[4 * e + 2]), __float_as_uint(y[4 * e + 3])));
+          }
+          write_rows(8, reinterpret_cast<uint64_t>(part + 32 * c), left / 4);
+          continue;
+        }
+        uint16_t* o = static_cast<uint16_t*>(a.o) + oo + 32 * c;
+        uint32_t hi[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) hi[e] = pack_pair<T>(y[2 * e], y[2 * e + 1]);
+        if (a.o_vec) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            put(4, e, make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]));
+          }
+          write_rows(4, reinterpret_cast<uint64_t>(o), left / 8);
+        } else if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            if (e < left) o[e] = static_cast<uint16_t>(hi[e / 2] >> (16 * (e & 1)));
+          }
+        }
+        if (a.o_lo != 0) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            hi[e] = pack_pair<T>(y[2 * e] - __uint_as_float(hi[e] << 16),
+                                 y[2 * e + 1] - __uint_as_float(hi[e] & 0xFFFF0000u));
+          }
+          if (a.o_vec) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              put(4, e, make_uint4(hi[4 * e], hi[4 * e + 1], hi[4 * e + 2], hi[4 * e + 3]));
             }
-            uint32_t hi[4], lo[4];
+            write_rows(4, reinterpret_cast<uint64_t>(o + a.o_lo), left / 8);
+          } else if (valid) {
 #pragma unroll
-            for (int f = 0; f < 4; ++f) hi[f] = pack_pair<T>(y[e + 2 * f], y[e + 2 * f + 1]);
-            if (a.o_lo != 0) {
-#pragma unroll
-              for (int f = 0; f < 4; ++f) {
-                lo[f] = pack_pair<T>(y[e + 2 * f] - __uint_as_float(hi[f] << 16),
-                                 y[e + 2 * f + 1] - __uint_as_float(hi[f] & 0xFFFF0000u));
-              }
-            }
-            uint16_t* o = static_cast<uint16_t*>(a.o) + oo + d;
-            if (a.o_vec) {
-              *reinterpret_cast<uint4*>(o) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-              if (a.o_lo != 0) {
-                *reinterpret_cast<uint4*>(o + a.o_lo) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-              }
-            } else {
-              for (int f = 0; f < 8; ++f) {
-                o[f] = static_cast<uint16_t>(hi[f / 2] >> (16 * (f & 1)));
-                if (a.o_lo != 0) o[a.o_lo + f] = static_cast<uint16_t>(lo[f / 2] >> (16 * (f & 1)));
-              }
+            for (int e = 0; e < 32; ++e) {
+              if (e < left) o[a.o_lo + e] = static_cast<uint16_t>(hi[e / 2] >> (16 * (e & 1)));
             }
           }
         }
@@ -631,7 +682,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
     const int issued = *loads_issued;
     for (int i = max(0, issued - kStages); i < issued; ++i) {
-      const bool cut = last_short && i == total - 1;
+      const bool cut = last_short && i == slots - 1;
       mbar_wait(cut ? short_full : &kv_full[i % kStages], cut ? 0 : (i / kStages) & 1,
                 &dummy_abort, kErrAttnKv, a.wait_limit_ns);
     }
