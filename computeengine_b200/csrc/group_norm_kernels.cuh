@@ -16,7 +16,6 @@
 
 #include <cooperative_groups.h>
 
-#include <type_traits>
 
 #include "element_types.cuh"
 
@@ -27,34 +26,43 @@ struct GroupNormArgs {
   const float* gamma;
   const float* beta;
   void* y;
-  int64_t pixels;  // h * w
-  int c, c_store, groups, act;
+  int pixels;  // h * w
+  int c, c_store, group_channels;
+  float low, high;  // of the clamp
   float eps;
   int range_groups;     // groups per channel range
   int ranges;           // channel ranges of an image
   int first_range;      // of this launch (two-kernel path)
   int64_t first_image;  // of this launch
   int blocks;           // pixel blocks per image and range
+  int share;            // pixels of a block
+  int cols[2], rows[2]; // threads over a range's vectors and pixels: inner, last range
   float2* partial;      // two-kernel path: mean and sum of squared differences,
                         // [image of this launch][range of this launch][block][range_groups]
   int launch_ranges;    // ranges of this launch
 };
 
 constexpr int kGnThreads = 256;
-constexpr int kGnBatch = 8;  // pixels per exact mean
+constexpr int kGnBatch = 4;  // pixels per exact mean
 
-__device__ __forceinline__ float activate(float v, int act) {
-  switch (act) {
-    case IE_ACT_RELU:
-      return v < 0.0f ? 0.0f : v;  // NaN stays
-    case IE_ACT_RELU6:
-      return v < 0.0f ? 0.0f : v > 6.0f ? 6.0f : v;
-    case IE_ACT_SILU:
-      return __fdividef(v, 1.0f + __expf(-v));
-    case IE_ACT_GELU:
-      return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-    default:
-      return v;
+// Kinds of activation: a clamp to [low, high] (none, ReLU, ReLU6), SiLU, GELU.
+enum { kActClamp = 0, kActSilu = 1, kActGelu = 2 };
+
+template <int ACT>
+__device__ __forceinline__ float activate(float v, float low, float high) {
+  if constexpr (ACT == kActClamp) {
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(low));  // NaN stays
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(high));
+    return v;
+  } else if constexpr (ACT == kActSilu) {
+    // v / (1 + 2^(-v log2 e)) on the special function unit: each of its two
+    // results is within two steps of fp32
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return v * r;
+  } else {
+    return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
   }
 }
 
@@ -110,6 +118,45 @@ __device__ __forceinline__ void store_item(void* y, int64_t at, int c_store, con
   }
 }
 
+// Two fp32 operations in one instruction (sm_100).
+__device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b1) {
+  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
+      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void fma_pair(float& d0, float& d1, float a0, float a1, float b0,
+                                         float b1) {  // d += a * b
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mov.b64 d, {%0, %1};\n\tfma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(d0), "+f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+template <int V>
+__device__ __forceinline__ void add_to(float (&a)[V], const float (&b)[V]) {  // a += b
+  if constexpr (V == 1) {
+    a[0] += b[0];
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) add_pair(a[e], a[e + 1], b[e], b[e + 1]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void add_squares(float (&a)[V], const float (&b)[V],
+                                            const float (&minus)[V]) {  // a += (b + minus)^2
+  if constexpr (V == 1) {
+    const float d = b[0] + minus[0];
+    a[0] += d * d;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      float d0 = b[e], d1 = b[e + 1];
+      add_pair(d0, d1, minus[e], minus[e + 1]);
+      fma_pair(a[e], a[e + 1], d0, d1, d0, d1);
+    }
+  }
+}
+
 // Running statistics of V channels over the pixels a thread has seen.
 template <int V>
 struct Running {
@@ -120,55 +167,43 @@ struct Running {
 #pragma unroll
     for (int e = 0; e < V; ++e) mean[e] = m2[e] = 0.0f;
   }
-  // A batch of k > 0 pixels, MAX at most (0: any number); get(i, f) reads
-  // pixel i, twice.
-  template <int MAX, class Get>
-  __device__ __forceinline__ void add(int k, const Get& get) {
-    float s[V], q[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) s[e] = q[e] = 0.0f;
-    auto sum = [&](int i) {
-      float f[V];
-      get(i, f);
-#pragma unroll
-      for (int e = 0; e < V; ++e) s[e] += f[e];
-    };
-    auto squares = [&](int i) {
-      float f[V];
-      get(i, f);
-#pragma unroll
-      for (int e = 0; e < V; ++e) q[e] += (f[e] - s[e]) * (f[e] - s[e]);
-    };
-    const float inv = 1.0f / static_cast<float>(k);
-    if constexpr (MAX > 0) {
-#pragma unroll
-      for (int i = 0; i < MAX; ++i) {
-        if (i < k) sum(i);
-      }
-    } else {
-#pragma unroll 4
-      for (int i = 0; i < k; ++i) sum(i);
-    }
-#pragma unroll
-    for (int e = 0; e < V; ++e) s[e] *= inv;
-    if constexpr (MAX > 0) {
-#pragma unroll
-      for (int i = 0; i < MAX; ++i) {
-        if (i < k) squares(i);
-      }
-    } else {
-#pragma unroll 4
-      for (int i = 0; i < k; ++i) squares(i);
-    }
+  // Joins k > 0 pixels with sum s and squares q about their mean.
+  __device__ __forceinline__ void join(int k, const float (&batch_mean)[V], const float (&q)[V]) {
     const float share = static_cast<float>(k) / static_cast<float>(n + k);
     const float weight = static_cast<float>(n) * share;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      const float d = n == 0 ? 0.0f : s[e] - mean[e];
-      mean[e] = n == 0 ? s[e] : mean[e] + d * share;
-      m2[e] += q[e] + d * d * weight;
+      const float d = n == 0 ? 0.0f : batch_mean[e] - mean[e];
+      mean[e] = n == 0 ? batch_mean[e] : fmaf(d, share, mean[e]);
+      m2[e] += fmaf(d * d, weight, q[e]);
     }
     n += k;
+  }
+  // A whole batch in registers.
+  __device__ __forceinline__ void add(const float (&f)[kGnBatch][V]) {
+    float s[V], q[V], minus[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      s[e] = f[0][e];
+      q[e] = 0.0f;
+    }
+#pragma unroll
+    for (int i = 1; i < kGnBatch; ++i) add_to<V>(s, f[i]);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      s[e] *= 1.0f / kGnBatch;
+      minus[e] = -s[e];
+    }
+#pragma unroll
+    for (int i = 0; i < kGnBatch; ++i) add_squares<V>(q, f[i], minus);
+    join(kGnBatch, s, q);
+  }
+  // One pixel.
+  __device__ __forceinline__ void add(const float (&f)[V]) {
+    float q[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) q[e] = 0.0f;
+    join(1, f, q);
   }
 };
 
@@ -177,161 +212,169 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Joins the threads' channels into the groups of the block's channel range:
-// out[g] = (mean, sum of squared differences).  Thread t holds the channels
-// (t % cols) * V .. of the range, rows = threads per column; scratch holds
-// (2 * V + 2) * threads floats.  First every channel's rows are joined in
-// slices, so that all threads take part; then a warp joins a group's channels.
-// (A single group wider than the threads' columns: every thread's channels are
-// that group's.)
+// Sums each thread's V channels into the groups of the block's channel range:
+// out[g], in an order that is always the same.  Thread t holds the channels
+// (t % cols) * V .. of the range, rows = threads per column.  First slices of
+// the rows of each channel are summed by all threads, then a warp sums a
+// group.  scratch holds (V + 1) * threads floats.  (A single group wider than
+// the threads' columns: group_channels is what the columns hold.)
 template <int V>
-__device__ __forceinline__ void join_threads(const Running<V>& r, int cols, int rows,
-                                             int group_channels, int groups, float* scratch,
-                                             float2* out) {
-  const int width = cols * V;
-  float* mean = scratch;                   // [rows][width]
-  float* m2 = mean + V * kGnThreads;       // [rows][width]
-  float* count = m2 + V * kGnThreads;      // [rows][cols]
-  float* joined = count + kGnThreads;      // [slices][cols]
-  const int t = threadIdx.x;
-  if (t < cols * rows) {
-    const int at = t / cols * width + t % cols * V;
+__device__ __forceinline__ void group_sums(const float (&v)[V], int cols, int rows,
+                                           int group_channels, int groups, float* scratch,
+                                           float* out) {
+  const int width = cols * V, t = threadIdx.x, lane = t & 31;
+  if (t < cols * rows) {  // [rows][width]
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      mean[at + e] = r.mean[e];
-      m2[at + e] = r.m2[e];
-    }
-    count[t] = static_cast<float>(r.n);
+    for (int e = 0; e < V; ++e) scratch[t * V + e] = v[e];
   }
   __syncthreads();
-  // slices of whole rows; a slice's result replaces its first row
-  const int slices = max(1, min(rows, kGnThreads / width));
-  const int deep = (rows + slices - 1) / slices;
-  for (int i = t; i < slices * width; i += kGnThreads) {
-    const int slice = i / width, ch = i - slice * width, col = ch / V;
-    const int from = slice * deep, to = min(rows, from + deep);
-    float n = 0.0f, s = 0.0f, q = 0.0f;
-    for (int k = from; k < to; ++k) {
-      n += count[k * cols + col];
-      s += count[k * cols + col] * mean[k * width + ch];
+  float* partial = scratch;  // [slices][width]
+  int slices = 1;
+  if (width >= kGnThreads) {  // a channel's sum replaces its first row
+    for (int ch = t; ch < width; ch += kGnThreads) {
+      float s = scratch[ch];
+      for (int k = 1; k < rows; ++k) s += scratch[k * width + ch];
+      scratch[ch] = s;
     }
-    const float mu = n > 0.0f ? s / n : 0.0f;
-    for (int k = from; k < to; ++k) {
-      const float w = count[k * cols + col], d = mean[k * width + ch] - mu;
-      if (w > 0.0f) q += m2[k * width + ch] + w * d * d;
+  } else {
+    partial = scratch + V * kGnThreads;
+    slices = kGnThreads / width;
+    const int slice = t / width, ch = t - slice * width;
+    if (slice < slices) {
+      float s = 0.0f;
+#pragma unroll 4
+      for (int k = slice; k < rows; k += slices) s += scratch[k * width + ch];
+      partial[t] = s;
     }
-    if (from < rows) {
-      mean[from * width + ch] = mu;
-      m2[from * width + ch] = q;
-    }
-    joined[slice * cols + col] = n;  // the same from each of the column's channels
   }
   __syncthreads();
-  const int lane = t & 31;
+  // lanes over the group's channels, and over slices when they are few
+  int lanes = 1, shift = 0;
+  while (lanes < group_channels && lanes < 32) {
+    lanes <<= 1;
+    ++shift;
+  }
   for (int g = t >> 5; g < groups; g += kGnThreads / 32) {
-    const int entries = slices * group_channels;
-    float n = 0.0f, s = 0.0f, q = 0.0f;
-    for (int i = lane; i < entries; i += 32) {
-      const int slice = i / group_channels, ch = g * group_channels + i - slice * group_channels;
-      const float w = joined[slice * cols + ch / V];
-      if (w > 0.0f) {
-        n += w;
-        s += w * mean[slice * deep * width + ch];
-      }
+    float s = 0.0f;
+    for (int k = lane >> shift; k < slices; k += 32 >> shift) {
+      const float* row = partial + k * width + g * group_channels;
+      for (int ch = lane & (lanes - 1); ch < group_channels; ch += lanes) s += row[ch];
     }
-    n = warp_sum(n);
-    const float mu = warp_sum(s) / n;
-    for (int i = lane; i < entries; i += 32) {
-      const int slice = i / group_channels, ch = g * group_channels + i - slice * group_channels;
-      const float w = joined[slice * cols + ch / V];
-      const float d = w > 0.0f ? mean[slice * deep * width + ch] - mu : 0.0f;
-      if (w > 0.0f) q += m2[slice * deep * width + ch] + w * d * d;
-    }
-    q = warp_sum(q);
-    if (lane == 0) out[g] = make_float2(mu, q);
+    s = warp_sum(s);
+    if (lane == 0) out[g] = s;
   }
   __syncthreads();
+}
+
+// Joins the statistics of `blocks` pixel blocks, block k's at at(k), into the
+// mean and 1 / sigma of a group.
+template <class At>
+__device__ __forceinline__ float2 join_blocks(const GroupNormArgs& a, int group_channels,
+                                              const At& at) {
+  float s = 0.0f, q = 0.0f;
+  for (int k = 0; k < a.blocks; ++k) {
+    const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
+    if (w > 0) s += static_cast<float>(w) * at(k).x;
+  }
+  const float mu = a.blocks == 1 ? at(0).x : s / static_cast<float>(a.pixels);
+  for (int k = 0; k < a.blocks; ++k) {
+    const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
+    if (w <= 0) continue;
+    const float2 o = at(k);
+    const float d = o.x - mu;
+    q += o.y + static_cast<float>(w) * static_cast<float>(group_channels) * d * d;
+  }
+  const float size = static_cast<float>(a.pixels) * static_cast<float>(group_channels);
+  return make_float2(mu, 1.0f / sqrtf(q / size + a.eps));
 }
 
 // Geometry shared by the kernels: the block's channel range.
 struct Range {
   int c0, channels, cols, rows, group_channels;
-  __device__ __forceinline__ Range(const GroupNormArgs& a, int range, int v) {
-    group_channels = a.c / a.groups;
-    c0 = range * a.range_groups * group_channels;
+  __device__ __forceinline__ Range(const GroupNormArgs& a, int range) {
+    const int last = range == a.ranges - 1;  // carries the padding channels
+    group_channels = a.group_channels;
     channels = a.range_groups * group_channels;
-    // the last range carries the padding channels
-    const int stored = range == a.ranges - 1 ? a.c_store - c0 : channels;
-    cols = (stored + v - 1) / v;
-    rows = max(1, kGnThreads / cols);
+    c0 = range * channels;
+    cols = a.cols[last];
+    rows = a.rows[last];
   }
 };
+
+// mul and add of the V channels from c: gamma / sigma, and beta less the mean's
+// share of it.  stat: mean and 1 / sigma of the range's groups; the thread's
+// first channel is `inner` channels into group `first`.
+template <int V>
+__device__ __forceinline__ void channel_affine(const GroupNormArgs& a, int c, int first, int inner,
+                                               const float2* stat, float (&mul)[V],
+                                               float (&add)[V]) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const bool in = c + e < a.c;
+    const float2 st = in ? stat[first] : make_float2(0.0f, 0.0f);
+    mul[e] = in && a.gamma != nullptr ? st.y * a.gamma[c + e] : st.y;
+    add[e] = fmaf(-st.x, mul[e], in && a.beta != nullptr ? a.beta[c + e] : 0.0f);
+    if (++inner == a.group_channels) {
+      inner = 0;
+      ++first;
+    }
+  }
+}
 
 // Normalizes, activates and stores one item; channels past c become zero
 // (mul and add are zero there, but x may hold anything).
 template <int YT, int V, int ACT>
 __device__ __forceinline__ void finish_item(const GroupNormArgs& a, float (&f)[V],
                                             const float (&mul)[V], const float (&add)[V],
-                                            int64_t pixel, int c) {
+                                            uint8_t* y, int valid) {
 #pragma unroll
-  for (int e = 0; e < V; ++e) f[e] = activate(fmaf(f[e], mul[e], add[e]), ACT);
-  if (c + V > a.c) {
+  for (int e = 0; e < V; ++e) f[e] = activate<ACT>(fmaf(f[e], mul[e], add[e]), a.low, a.high);
+  if (valid < V) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = c + e < a.c ? f[e] : 0.0f;
+    for (int e = 0; e < V; ++e) f[e] = e < valid ? f[e] : 0.0f;
   }
-  store_item<YT, V>(a.y, channel_at<YT>(pixel, a.c_store, c), a.c_store, f);
-}
-
-// Runs body(std::integral_constant<int, act>) for the activation, so that the
-// choice is made once and not per element.
-template <class Body>
-__device__ __forceinline__ void with_activation(int act, const Body& body) {
-  switch (act) {
-    case IE_ACT_RELU: body(std::integral_constant<int, IE_ACT_RELU>()); break;
-    case IE_ACT_RELU6: body(std::integral_constant<int, IE_ACT_RELU6>()); break;
-    case IE_ACT_SILU: body(std::integral_constant<int, IE_ACT_SILU>()); break;
-    case IE_ACT_GELU: body(std::integral_constant<int, IE_ACT_GELU>()); break;
-    default: body(std::integral_constant<int, IE_ACT_NONE>()); break;
-  }
+  store_item<YT, V>(y, 0, a.c_store, f);
 }
 
 // One cluster per (image, channel range); each block holds its pixels' items
 // in shared memory.  The copies are issued at once, so the whole range is in
 // flight; a thread reads back only what it copied itself.
-template <int XT, int YT, int V>
+template <int XT, int YT, int V, int ACT>
 __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const GroupNormArgs a) {
   namespace cg = cooperative_groups;
   constexpr int kItem = Item<XT, V>::kBytes * (XT == IE_DT_BF16X2 ? 2 : 1);
   static_assert(Item<XT, V>::kBytes == 16, "16-byte copies");
   extern __shared__ __align__(16) uint8_t smem[];
-  float2* own = reinterpret_cast<float2*>(smem);  // [range_groups] of this block
-  float2* stat = own + a.range_groups;            // [range_groups] mean, 1 / sigma
-  float* scratch = reinterpret_cast<float*>(stat + a.range_groups);
-  uint8_t* items = reinterpret_cast<uint8_t*>(scratch + (2 * V + 2) * kGnThreads);
+  float2* own = reinterpret_cast<float2*>(smem);    // [range_groups] of this block
+  float2* stat = own + a.range_groups;              // [range_groups] mean, 1 / sigma
+  float2* others = stat + a.range_groups;           // [blocks][range_groups]
+  float* sums = reinterpret_cast<float*>(others + a.blocks * a.range_groups);  // [range_groups]
+  float* scratch = sums + a.range_groups;
+  uint8_t* items = reinterpret_cast<uint8_t*>(scratch + (V + 1) * kGnThreads);
   items += (16 - reinterpret_cast<uintptr_t>(items) % 16) % 16;
 
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = a.blocks > 1 ? static_cast<int>(cluster.block_rank()) : 0;
-  const int unit = static_cast<int>(blockIdx.x) / a.blocks;
-  const int range = unit % a.ranges;
-  const int64_t image = unit / a.ranges;
-  const Range r(a, range, V);
-  const int col = threadIdx.x % r.cols, row = threadIdx.x / r.cols;
-  const bool works = row < r.rows;
-  const int64_t share = (a.pixels + a.blocks - 1) / a.blocks;
-  const int64_t from = rank * share;
-  const int count = static_cast<int>(max(int64_t{0}, min(a.pixels, from + share) - from));
+  const uint32_t unit = blockIdx.x / static_cast<uint32_t>(a.blocks);
+  const int64_t image = unit / static_cast<uint32_t>(a.ranges);
+  const int range = static_cast<int>(unit - image * a.ranges);
+  const Range r(a, range);
+  const int row = threadIdx.x / r.cols, col = threadIdx.x - row * r.cols;
+  const int from = rank * a.share;
+  const int count = max(0, min(a.pixels, from + a.share) - from);
   const int64_t p0 = image * a.pixels + from;
   const int c = r.c0 + col * V;
 
   uint8_t* mine = items + threadIdx.x * 16;
   constexpr int kStep = kGnThreads * kItem;
-  if (works) {
-    const uint8_t* x = static_cast<const uint8_t*>(a.x);
-    int i = 0;
-    for (int p = row; p < count; p += r.rows, ++i) {
-      const uint8_t* from_x = x + channel_at<XT>(p0 + p, a.c_store, c) * element_bytes(XT);
-      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(mine + i * kStep));
+  const int n = row < r.rows && row < count ? (count - row + r.rows - 1) / r.rows : 0;
+  {
+    const int64_t x_step = static_cast<int64_t>(r.rows) * channel_at<XT>(1, a.c_store, 0) *
+                           element_bytes(XT);
+    const uint8_t* from_x = static_cast<const uint8_t*>(a.x) +
+                            channel_at<XT>(p0 + row, a.c_store, c) * element_bytes(XT);
+    uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(mine));
+    for (int i = 0; i < n; ++i, from_x += x_step, to += kStep) {
       asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from_x) : "memory");
       if constexpr (XT == IE_DT_BF16X2) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + kGnThreads * 16),
@@ -340,12 +383,8 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
       }
     }
   }
-  float g[V], b[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    g[e] = works && a.gamma != nullptr && c + e < a.c ? a.gamma[c + e] : 1.0f;
-    b[e] = works && a.beta != nullptr && c + e < a.c ? a.beta[c + e] : 0.0f;
-  }
+  // the thread's place among the groups, while the copies are under way
+  const int first = col * V / r.group_channels, inner = col * V - first * r.group_channels;
   asm volatile("cp.async.wait_all;" ::: "memory");
 
   auto item = [&](int i, float(&f)[V]) {
@@ -354,179 +393,223 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
     if constexpr (XT == IE_DT_BF16X2) it.lo = load_bytes<16>(mine + i * kStep + kGnThreads * 16);
     item_floats<XT, V>(it, f);
   };
-  const int n = works && row < count ? (count - row + r.rows - 1) / r.rows : 0;
-  Running<V> run;
-  if (n > 0) run.template add<0>(n, item);
-  join_threads<V>(run, r.cols, r.rows, r.group_channels, a.range_groups, scratch, own);
-
-  // the blocks' statistics, in rank order
-  if (a.blocks > 1) cluster.sync();
-  for (int gi = threadIdx.x; gi < a.range_groups; gi += kGnThreads) {
-    float total = 0.0f, s = 0.0f, q = 0.0f, mu = own[gi].x;
-    if (a.blocks > 1) {
-      for (int k = 0; k < a.blocks; ++k) {
-        const float w = static_cast<float>(
-            max(int64_t{0}, min(a.pixels, (k + 1) * share) - k * share));
-        const float2 o = *cluster.map_shared_rank(own + gi, k);
-        total += w;
-        if (w > 0.0f) s += w * o.x;
-      }
-      mu = s / total;
-    }
-    for (int k = 0; k < a.blocks; ++k) {
-      const float w = static_cast<float>(
-          max(int64_t{0}, min(a.pixels, (k + 1) * share) - k * share));
-      if (w == 0.0f) continue;
-      const float2 o = a.blocks > 1 ? *cluster.map_shared_rank(own + gi, k) : own[gi];
-      const float d = o.x - mu;
-      q += o.y + w * static_cast<float>(r.group_channels) * d * d;
-    }
-    const float size = static_cast<float>(a.pixels) * static_cast<float>(r.group_channels);
-    stat[gi] = make_float2(mu, 1.0f / sqrtf(q / size + a.eps));
-  }
-  if (a.blocks > 1) {
-    cluster.sync();  // no block leaves while another reads its statistics
-  } else {
-    __syncthreads();
-  }
+  // the block's mean of each group, then the squares about it
+  float v[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const int gi = (c + e - r.c0) / r.group_channels;
-    const float2 st = works && c + e < a.c ? stat[gi] : make_float2(0.0f, 0.0f);
-    g[e] *= st.y;
-    b[e] = fmaf(-st.x, g[e], b[e]);  // the mean goes into the addend
+  for (int e = 0; e < V; ++e) v[e] = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    float f[V];
+    item(i, f);
+    add_to<V>(v, f);
   }
-  with_activation(a.act, [&](auto act) {
-#pragma unroll 1
+  group_sums<V>(v, r.cols, r.rows, r.group_channels, a.range_groups, scratch, sums);
+  const float inv = 1.0f / (static_cast<float>(count) * static_cast<float>(r.group_channels));
+  {
+    float minus[V];
+    int g = first, in_group = inner;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {  // padding channels: the group's that would follow
+      minus[e] = -sums[min(g, a.range_groups - 1)] * inv;
+      v[e] = 0.0f;
+      if (++in_group == r.group_channels) {
+        in_group = 0;
+        ++g;
+      }
+    }
+#pragma unroll 4
     for (int i = 0; i < n; ++i) {
       float f[V];
       item(i, f);
-      finish_item<YT, V, decltype(act)::value>(a, f, g, b,
-                                               p0 + row + static_cast<int64_t>(i) * r.rows, c);
+      add_squares<V>(v, f, minus);
     }
-  });
+  }
+  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) own[g].x = sums[g] * inv;
+  __syncthreads();
+  group_sums<V>(v, r.cols, r.rows, r.group_channels, a.range_groups, scratch, sums);
+  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) own[g].y = sums[g];
+
+  // the blocks' statistics, in rank order
+  if (a.blocks > 1) {
+    cluster.sync();
+    const int all = a.blocks * a.range_groups;
+    for (int i = threadIdx.x; i < all; i += kGnThreads) {
+      const int k = i / a.range_groups;
+      others[i] = *cluster.map_shared_rank(own + (i - k * a.range_groups), k);
+    }
+    cluster.barrier_arrive();  // waited for at the end: no block leaves while others read
+  }
+  __syncthreads();
+  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) {
+    stat[g] = join_blocks(a, r.group_channels, [&](int k) {
+      return a.blocks > 1 ? others[k * a.range_groups + g] : own[g];
+    });
+  }
+  __syncthreads();
+  float g[V], b[V];
+  if (n > 0) channel_affine<V>(a, c, first, inner, stat, g, b);
+  uint8_t* y = static_cast<uint8_t*>(a.y) +
+               channel_at<YT>(p0 + row, a.c_store, c) * element_bytes(YT);
+  const int64_t y_step = static_cast<int64_t>(r.rows) * channel_at<YT>(1, a.c_store, 0) *
+                         element_bytes(YT);
+#pragma unroll(ACT == kActGelu ? 1 : 2)
+  for (int i = 0; i < n; ++i, y += y_step) {
+    float f[V];
+    item(i, f);
+    finish_item<YT, V, ACT>(a, f, g, b, y, a.c - c);
+  }
+  if (a.blocks > 1) cluster.barrier_wait();
 }
 
 // Statistics of one block of pixels of an image and channel range.
 template <int XT, int V>
 __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const GroupNormArgs a) {
   extern __shared__ __align__(16) uint8_t smem[];
-  float* scratch = reinterpret_cast<float*>(smem);
-  float2* own = reinterpret_cast<float2*>(scratch + (2 * V + 2) * kGnThreads);
-  const int block = blockIdx.x % a.blocks;
-  const int64_t unit = blockIdx.x / a.blocks;
-  const int range = a.first_range + static_cast<int>(unit % a.launch_ranges);
-  const int64_t image = a.first_image + unit / a.launch_ranges;
-  const Range r(a, range, V);
+  float* sums = reinterpret_cast<float*>(smem);  // [range_groups]
+  float* scratch = sums + a.range_groups;
+  const uint32_t unit = blockIdx.x / static_cast<uint32_t>(a.blocks);
+  const int block = static_cast<int>(blockIdx.x - unit * a.blocks);
+  const uint32_t of_launch = unit / static_cast<uint32_t>(a.launch_ranges);
+  const int range = a.first_range + static_cast<int>(unit - of_launch * a.launch_ranges);
+  const int64_t image = a.first_image + of_launch;
+  const Range r(a, range);
   const int all = (r.channels + V - 1) / V;  // padding channels have no statistics
   const int cols = min(all, kGnThreads), rows = kGnThreads / cols;
-  const int col = threadIdx.x % cols, row = threadIdx.x / cols;
-  const int64_t share = (a.pixels + a.blocks - 1) / a.blocks;
-  const int64_t from = block * share;
-  const int64_t count = max(int64_t{0}, min(a.pixels, from + share) - from);
+  const int row = threadIdx.x / cols, col = threadIdx.x - row * cols;
+  const int from = block * a.share;
+  const int count = max(0, min(a.pixels, from + a.share) - from);
   const int64_t p0 = image * a.pixels + from;
   Running<V> run;
   // more columns than threads: the range is one group
-  for (int at = col; row < rows && at < all; at += cols) {
+  for (int at = col; row < rows && row < count && at < all; at += cols) {
     const int c = r.c0 + at * V;
-    for (int64_t p = row; p < count; p += kGnBatch * rows) {
-      const int64_t left = (count - p + rows - 1) / rows;
-      const int k = left < kGnBatch ? static_cast<int>(left) : kGnBatch;
-      Item<XT, V> it[kGnBatch];
+    constexpr int K = XT == IE_DT_BF16X2 ? 1 : 2;  // batches in flight
+    const int64_t step = static_cast<int64_t>(rows) * channel_at<XT>(1, a.c_store, 0);
+    int64_t from_x = channel_at<XT>(p0 + row, a.c_store, c);
+    int left = (count - row + rows - 1) / rows;  // pixels of this thread
+    for (; left >= K * kGnBatch; left -= K * kGnBatch) {
+      Item<XT, V> it[K * kGnBatch];
 #pragma unroll
-      for (int e = 0; e < kGnBatch; ++e) {
-        if (e < k) {
-          it[e] = load_item<XT, V>(a.x, channel_at<XT>(p0 + p + int64_t{e} * rows, a.c_store, c),
-                                   a.c_store);
-        }
+      for (int e = 0; e < K * kGnBatch; ++e, from_x += step) {
+        it[e] = load_item<XT, V>(a.x, from_x, a.c_store);
       }
-      run.template add<kGnBatch>(k, [&](int e, float(&f)[V]) { item_floats<XT, V>(it[e], f); });
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float f[kGnBatch][V];
+#pragma unroll
+        for (int e = 0; e < kGnBatch; ++e) item_floats<XT, V>(it[k * kGnBatch + e], f[e]);
+        run.add(f);
+      }
+    }
+    for (; left > 0; --left, from_x += step) {
+      float f[V];
+      item_floats<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store), f);
+      run.add(f);
     }
   }
-  join_threads<V>(run, cols, rows, all > cols ? cols * V : r.group_channels, a.range_groups,
-                  scratch, own);
-  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) {
-    a.partial[(unit * a.blocks + block) * a.range_groups + g] = own[g];
+  // the block's mean of each group, then each channel's squares about it
+  const int group_channels = all > cols ? cols * V : r.group_channels;
+  float v[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) v[e] = run.n > 0 ? run.mean[e] * static_cast<float>(run.n) : 0.0f;
+  group_sums<V>(v, cols, rows, group_channels, a.range_groups, scratch, sums);
+  const float inv = 1.0f / (static_cast<float>(count) * static_cast<float>(r.group_channels));
+  int g = col * V / group_channels, inner = col * V - g * group_channels;
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    const float d = run.mean[e] - sums[min(g, a.range_groups - 1)] * inv;
+    v[e] = run.n > 0 ? fmaf(d * d, static_cast<float>(run.n), run.m2[e]) : 0.0f;
+    if (++inner == group_channels) {
+      inner = 0;
+      ++g;
+    }
+  }
+  // [unit][group][block], so that a warp reads a group's blocks side by side
+  float2* to = a.partial + static_cast<int64_t>(unit) * a.range_groups * a.blocks + block;
+  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) {
+    to[static_cast<int64_t>(i) * a.blocks].x = sums[i] * inv;
+  }
+  __syncthreads();
+  group_sums<V>(v, cols, rows, group_channels, a.range_groups, scratch, sums);
+  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) {
+    to[static_cast<int64_t>(i) * a.blocks].y = sums[i];
   }
 }
 
 // Joins the blocks' statistics (every block of the launch for itself) and
 // normalizes.  Blocks run over the pixels from the end, which L2 still holds.
-template <int XT, int YT, int V>
-__global__ void __launch_bounds__(kGnThreads, 2) group_norm_apply_kernel(const GroupNormArgs a,
+template <int XT, int YT, int V, int ACT>
+__global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 : 4)
+    group_norm_apply_kernel(const GroupNormArgs a,
                                                                       int apply_blocks) {
   extern __shared__ __align__(16) uint8_t smem[];
   float2* stat = reinterpret_cast<float2*>(smem);
-  const int block = apply_blocks - 1 - static_cast<int>(blockIdx.x % apply_blocks);
-  const int64_t unit = blockIdx.x / apply_blocks;
-  const int range = a.first_range + static_cast<int>(unit % a.launch_ranges);
-  const int64_t image = a.first_image + unit / a.launch_ranges;
-  const Range r(a, range, V);
-  const int64_t part = (a.pixels + a.blocks - 1) / a.blocks;
+  const uint32_t unit = blockIdx.x / static_cast<uint32_t>(apply_blocks);
+  const int block = apply_blocks - 1 - static_cast<int>(blockIdx.x - unit * apply_blocks);
+  const uint32_t of_launch = unit / static_cast<uint32_t>(a.launch_ranges);
+  const int range = a.first_range + static_cast<int>(unit - of_launch * a.launch_ranges);
+  const int64_t image = a.first_image + of_launch;
+  const Range r(a, range);
   const int lane = threadIdx.x & 31;
   for (int g = threadIdx.x >> 5; g < a.range_groups; g += kGnThreads / 32) {
-    const float2* p = a.partial + unit * a.blocks * a.range_groups + g;
+    const float2* p = a.partial + (static_cast<int64_t>(unit) * a.range_groups + g) * a.blocks;
     float s = 0.0f, q = 0.0f;
     for (int k = lane; k < a.blocks; k += 32) {
-      const float w =
-          static_cast<float>(max(int64_t{0}, min(a.pixels, (k + 1) * part) - k * part));
-      if (w > 0.0f) s += w * p[k * a.range_groups].x;
+      const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
+      if (w > 0) s += static_cast<float>(w) * p[k].x;
     }
     const float mu = warp_sum(s) / static_cast<float>(a.pixels);
     for (int k = lane; k < a.blocks; k += 32) {
-      const float w =
-          static_cast<float>(max(int64_t{0}, min(a.pixels, (k + 1) * part) - k * part));
-      if (w == 0.0f) continue;
-      const float2 o = p[k * a.range_groups];
+      const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
+      if (w <= 0) continue;
+      const float2 o = p[k];
       const float d = o.x - mu;
-      q += o.y + w * static_cast<float>(r.group_channels) * d * d;
+      q += o.y + static_cast<float>(w) * static_cast<float>(r.group_channels) * d * d;
     }
     q = warp_sum(q);
     const float size = static_cast<float>(a.pixels) * static_cast<float>(r.group_channels);
     if (lane == 0) stat[g] = make_float2(mu, 1.0f / sqrtf(q / size + a.eps));
   }
   __syncthreads();
-  const int64_t share = (a.pixels + apply_blocks - 1) / apply_blocks;
-  const int64_t from = block * share;
-  const int64_t count = max(int64_t{0}, min(a.pixels, from + share) - from);
+  const int share = (a.pixels + apply_blocks - 1) / apply_blocks;
+  const int from = block * share;
+  const int count = max(0, min(a.pixels, from + share) - from);
   const int64_t p0 = image * a.pixels + from;
   // padding channels may make the last range wider than the block
   for (int col0 = 0; col0 < r.cols; col0 += kGnThreads) {
     const int cols = min(r.cols - col0, kGnThreads), rows = kGnThreads / cols;
-    const int col = col0 + threadIdx.x % cols, row = threadIdx.x / cols;
-    if (row >= rows) continue;
+    const int row = threadIdx.x / cols, col = col0 + threadIdx.x - row * cols;
+    if (row >= rows || row >= count) continue;
     const int c = r.c0 + col * V;
+    const int first = col * V / r.group_channels;
     float mul[V], add[V];
+    channel_affine<V>(a, c, first, col * V - first * r.group_channels, stat, mul, add);
+    constexpr int K = ACT == kActGelu || XT == IE_DT_BF16X2 ? 2 : 4;
+    const int64_t x_step = static_cast<int64_t>(rows) * channel_at<XT>(1, a.c_store, 0);
+    const int64_t y_step = static_cast<int64_t>(rows) * channel_at<YT>(1, a.c_store, 0) *
+                           element_bytes(YT);
+    int64_t from_x = channel_at<XT>(p0 + row, a.c_store, c);
+    uint8_t* y = static_cast<uint8_t*>(a.y) +
+                 channel_at<YT>(p0 + row, a.c_store, c) * element_bytes(YT);
+    int left = (count - row + rows - 1) / rows;
+    for (; left >= K; left -= K) {
+      Item<XT, V> it[K];
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      mul[e] = add[e] = 0.0f;
-      if (c + e < a.c) {
-        const float2 st = stat[(c + e - r.c0) / r.group_channels];
-        mul[e] = a.gamma == nullptr ? st.y : st.y * a.gamma[c + e];
-        // the mean goes into the addend
-        add[e] = fmaf(-st.x, mul[e], a.beta == nullptr ? 0.0f : a.beta[c + e]);
+      for (int e = 0; e < K; ++e, from_x += x_step) {
+        it[e] = load_item<XT, V>(a.x, from_x, a.c_store);
+      }
+#pragma unroll
+      for (int e = 0; e < K; ++e, y += y_step) {
+        float f[V];
+        item_floats<XT, V>(it[e], f);
+        finish_item<YT, V, ACT>(a, f, mul, add, y, a.c - c);
       }
     }
-    constexpr int K = XT == IE_DT_BF16X2 ? 2 : 4;
-    with_activation(a.act, [&](auto act) {
-      for (int64_t p = row; p < count; p += K * rows) {
-        Item<XT, V> it[K];
-#pragma unroll
-        for (int e = 0; e < K; ++e) {
-          if (p + int64_t{e} * rows < count) {
-            it[e] = load_item<XT, V>(a.x, channel_at<XT>(p0 + p + int64_t{e} * rows, a.c_store, c),
-                                     a.c_store);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < K; ++e) {
-          if (p + int64_t{e} * rows >= count) break;
-          float f[V];
-          item_floats<XT, V>(it[e], f);
-          finish_item<YT, V, decltype(act)::value>(a, f, mul, add, p0 + p + int64_t{e} * rows, c);
-        }
-      }
-    });
+    for (; left > 0; --left, from_x += x_step, y += y_step) {
+      float f[V];
+      item_floats<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store), f);
+      finish_item<YT, V, ACT>(a, f, mul, add, y, a.c - c);
+    }
   }
 }
 

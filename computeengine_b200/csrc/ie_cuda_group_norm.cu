@@ -37,9 +37,10 @@ int check_group_norm(const ie_group_norm_desc* d) {
       return fail(IE_INVALID_ARGUMENT, "split tensors hold a multiple of 16 channels per plane");
     }
   }
-  if (d->c_store > (1 << 20) || d->h > INT_MAX || d->w > INT_MAX || d->h * d->w > INT_MAX ||
-      d->n > 65535) {
-    return fail(IE_UNSUPPORTED, "GroupNorm size out of range (c_store <= 2^20, h * w < 2^31, "
+  constexpr int64_t kMaxPixels = 1 << 30;
+  if (d->c_store > (1 << 20) || d->h > kMaxPixels || d->w > kMaxPixels ||
+      d->h * d->w > kMaxPixels || d->n > 65535) {
+    return fail(IE_UNSUPPORTED, "GroupNorm size out of range (c_store <= 2^20, h * w <= 2^30, "
                                 "n < 2^16)");
   }
   return IE_OK;
@@ -51,7 +52,7 @@ constexpr int64_t kSms = 148;
 constexpr int64_t kSmemPerSm = 227 * 1024;
 // Bytes of x that the two-kernel path normalizes per pair of launches: with
 // the y they become they stay in the 126 MB L2 between the two reads.
-constexpr int64_t kWaveBytes = 48 << 20;
+constexpr int64_t kWaveBytes = 72 << 20;
 
 int64_t item_bytes(int x_type, int v) {
   return int64_t{v} * element_bytes(x_type) * (x_type == IE_DT_BF16X2 ? 2 : 1);
@@ -99,7 +100,7 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
     for (int blocks = 1; blocks <= 16; blocks *= 2) {
       const int64_t share = ceil_div(pixels, blocks);
       const int64_t held = ceil_div(share, rows) * kGnThreads * item_bytes(d->x_type, v);
-      const int64_t smem = held + (2 * v + 2) * kGnThreads * 4 + 16 * g + 32;
+      const int64_t smem = held + (v + 1) * kGnThreads * 4 + (20 + 8 * blocks) * g + 32;
       if (smem > kSmemPerSm || (blocks > 1 && share * (blocks - 1) >= pixels)) continue;
       const int64_t per_sm = std::min<int64_t>(4, (kSmemPerSm + 1024) / (smem + 1024));
       const int64_t total = d->n * ranges * blocks;
@@ -108,8 +109,11 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
       // one wave: no SM can do better than its own share of the bandwidth
       const double busy = static_cast<double>(std::min<int64_t>(total, kSms)) / kSms;
       const double bytes = static_cast<double>(d->n * pixels * d->c) * static_cast<double>(xb + yb);
+      // with few blocks on an SM, one's loads, arithmetic and stores leave the
+      // memory idle in turn (measured: one block per SM reaches half of it)
+      const double overlap = per_sm == 1 ? 2.0 : per_sm == 2 ? 1.4 : per_sm == 3 ? 1.15 : 1.0;
       const double ns = latency + std::max(latency * static_cast<double>(waves - 1),
-                                           waste * bytes / (6500.0 * busy));
+                                           waste * overlap * bytes / (6500.0 * busy));
       if (ns < best_ns) {
         best_ns = ns;
         best.cluster = true;
@@ -157,7 +161,7 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
       std::max<int64_t>(1, std::min(2 * kSms / units, ceil_div(pixels, kGnBatch * rows))));
   best.apply_blocks = static_cast<int>(
       std::max<int64_t>(1, std::min(2 * kSms / units, ceil_div(pixels, 4 * rows))));
-  best.smem = (2 * v + 2) * kGnThreads * 4 + 8 * best.range_groups;
+  best.smem = (v + 1) * kGnThreads * 4 + 4 * best.range_groups;
   best.workspace = units * best.blocks * best.range_groups * static_cast<int64_t>(sizeof(float2));
   return best;
 }
@@ -186,9 +190,9 @@ int allow_smem(Kernel kernel, int64_t smem, bool wide_cluster) {
   return e == cudaSuccess ? IE_OK : fail(IE_RUNTIME, "group_norm: %s", cudaGetErrorString(e));
 }
 
-template <int XT, int YT, int V>
+template <int XT, int YT, int V, int ACT>
 int launch_cluster(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
-  auto kernel = group_norm_cluster_kernel<XT, YT, V>;
+  auto kernel = group_norm_cluster_kernel<XT, YT, V, ACT>;
   const int rc = allow_smem(kernel, p.smem, p.blocks > 8);
   if (rc != IE_OK) return rc;
   cudaLaunchConfig_t cfg{};
@@ -210,10 +214,10 @@ int launch_cluster(const GroupNormArgs& a, const Plan& p, int64_t images, cudaSt
   return check_launch("group_norm");
 }
 
-template <int XT, int YT, int V>
+template <int XT, int YT, int V, int ACT>
 int launch_two(GroupNormArgs a, const Plan& p, int64_t images, cudaStream_t s) {
   auto stats = group_norm_stats_kernel<XT, V>;
-  auto apply = group_norm_apply_kernel<XT, YT, V>;
+  auto apply = group_norm_apply_kernel<XT, YT, V, ACT>;
   const int64_t apply_smem = 8 * p.range_groups;
   int rc = allow_smem(stats, p.smem, false);
   if (rc == IE_OK) rc = allow_smem(apply, apply_smem, false);
@@ -235,31 +239,40 @@ int launch_two(GroupNormArgs a, const Plan& p, int64_t images, cudaStream_t s) {
   return rc;
 }
 
-template <int XT, int YT>
+template <int XT, int YT, int ACT>
 int launch(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
   constexpr int V = XT == IE_DT_F32 ? 4 : 8;
-  if (p.v == 1) return launch_two<XT, YT, 1>(a, p, images, s);
-  return p.cluster ? launch_cluster<XT, YT, V>(a, p, images, s)
-                   : launch_two<XT, YT, V>(a, p, images, s);
+  if (p.v == 1) return launch_two<XT, YT, 1, ACT>(a, p, images, s);
+  return p.cluster ? launch_cluster<XT, YT, V, ACT>(a, p, images, s)
+                   : launch_two<XT, YT, V, ACT>(a, p, images, s);
+}
+
+template <int XT, int YT>
+int launch(int act, GroupNormArgs a, const Plan& p, int64_t images, cudaStream_t s) {
+  if (act == IE_ACT_SILU) return launch<XT, YT, kActSilu>(a, p, images, s);
+  if (act == IE_ACT_GELU) return launch<XT, YT, kActGelu>(a, p, images, s);
+  a.low = act == IE_ACT_NONE ? -INFINITY : 0.0f;
+  a.high = act == IE_ACT_RELU6 ? 6.0f : INFINITY;
+  return launch<XT, YT, kActClamp>(a, p, images, s);
 }
 
 template <int XT>
-int launch(int y_type, const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
+int launch(int y_type, int act, const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
   switch (y_type) {
-    case IE_DT_F32: return launch<XT, IE_DT_F32>(a, p, images, s);
-    case IE_DT_BF16: return launch<XT, IE_DT_BF16>(a, p, images, s);
-    case IE_DT_F16: return launch<XT, IE_DT_F16>(a, p, images, s);
-    default: return launch<XT, IE_DT_BF16X2>(a, p, images, s);
+    case IE_DT_F32: return launch<XT, IE_DT_F32>(act, a, p, images, s);
+    case IE_DT_BF16: return launch<XT, IE_DT_BF16>(act, a, p, images, s);
+    case IE_DT_F16: return launch<XT, IE_DT_F16>(act, a, p, images, s);
+    default: return launch<XT, IE_DT_BF16X2>(act, a, p, images, s);
   }
 }
 
-int launch(int x_type, int y_type, const GroupNormArgs& a, const Plan& p, int64_t images,
-           cudaStream_t s) {
+int launch(int x_type, int y_type, int act, const GroupNormArgs& a, const Plan& p,
+           int64_t images, cudaStream_t s) {
   switch (x_type) {
-    case IE_DT_F32: return launch<IE_DT_F32>(y_type, a, p, images, s);
-    case IE_DT_BF16: return launch<IE_DT_BF16>(y_type, a, p, images, s);
-    case IE_DT_F16: return launch<IE_DT_F16>(y_type, a, p, images, s);
-    default: return launch<IE_DT_BF16X2>(y_type, a, p, images, s);
+    case IE_DT_F32: return launch<IE_DT_F32>(y_type, act, a, p, images, s);
+    case IE_DT_BF16: return launch<IE_DT_BF16>(y_type, act, a, p, images, s);
+    case IE_DT_F16: return launch<IE_DT_F16>(y_type, act, a, p, images, s);
+    default: return launch<IE_DT_BF16X2>(y_type, act, a, p, images, s);
   }
 }
 
@@ -301,17 +314,23 @@ int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const
   a.gamma = gamma;
   a.beta = beta;
   a.y = y;
-  a.pixels = desc->h * desc->w;
+  a.pixels = static_cast<int>(desc->h * desc->w);
   a.c = static_cast<int>(desc->c);
   a.c_store = static_cast<int>(desc->c_store);
-  a.groups = static_cast<int>(desc->groups);
-  a.act = desc->act;
+  a.group_channels = static_cast<int>(desc->c / desc->groups);
   a.eps = desc->eps;
   a.range_groups = p.range_groups;
   a.ranges = p.ranges;
   a.blocks = p.blocks;
+  a.share = static_cast<int>(ceil_div(a.pixels, p.blocks));
+  for (int last = 0; last < 2; ++last) {
+    const int64_t channels = int64_t{p.range_groups} * a.group_channels;
+    const int64_t stored = last ? desc->c_store - (p.ranges - 1) * channels : channels;
+    a.cols[last] = static_cast<int>(ceil_div(stored, p.v));
+    a.rows[last] = std::max(1, kGnThreads / a.cols[last]);
+  }
   a.partial = static_cast<float2*>(workspace);
-  return launch(desc->x_type, desc->y_type, a, p, desc->n, as_stream(stream));
+  return launch(desc->x_type, desc->y_type, desc->act, a, p, desc->n, as_stream(stream));
 }
 
 }  // extern "C"
