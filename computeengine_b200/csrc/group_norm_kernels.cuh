@@ -9,9 +9,8 @@
 // therefore costs no precision and results do not depend on timing.
 //
 // group_norm_cluster_kernel: a channel range of an image is held in the shared
-// memory of one block or a cluster of up to 16, so x is read once.
-// group_norm_stats_kernel, group_norm_apply_kernel: for images that do not fit;
-// the second read of x comes out of L2.
+// memory of one block or a cluster of up to 8, so x is read once.
+// group_norm_stats_kernel, group_norm_apply_kernel: for images that do not fit.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -32,37 +31,54 @@ struct GroupNormArgs {
   float eps;
   int range_groups;     // groups per channel range
   int ranges;           // channel ranges of an image
-  int first_range;      // of this launch (two-kernel path)
-  int64_t first_image;  // of this launch
   int blocks;           // pixel blocks per image and range
   int share;            // pixels of a block
+  int parts, part_share;  // two-kernel path: clusters of blocks, and their pixels
   int cols[2], rows[2]; // threads over a range's vectors and pixels: inner, last range
   float2* partial;      // two-kernel path: mean and sum of squared differences,
-                        // [image of this launch][range of this launch][block][range_groups]
-  int launch_ranges;    // ranges of this launch
+                        // [image][range][range_groups][part]
 };
 
 constexpr int kGnThreads = 256;
 constexpr int kGnBatch = 4;  // pixels per exact mean
+constexpr int kGnCluster = 4;  // blocks of the statistics kernel joined before memory
 
 // Kinds of activation: a clamp to [low, high] (none, ReLU, ReLU6), SiLU, GELU.
 enum { kActClamp = 0, kActSilu = 1, kActGelu = 2 };
 
-template <int ACT>
-__device__ __forceinline__ float activate(float v, float low, float high) {
+template <int ACT, int V>
+__device__ __forceinline__ void activate(float (&v)[V], float low, float high) {
   if constexpr (ACT == kActClamp) {
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(low));  // NaN stays
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(v), "f"(high));
-    return v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      asm("max.NaN.f32 %0, %1, %2;" : "=f"(v[e]) : "f"(v[e]), "f"(low));  // NaN stays
+      asm("min.NaN.f32 %0, %1, %2;" : "=f"(v[e]) : "f"(v[e]), "f"(high));
+    }
   } else if constexpr (ACT == kActSilu) {
-    // v / (1 + 2^(-v log2 e)) on the special function unit: each of its two
-    // results is within two steps of fp32
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(v * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return v * r;
+    // v / (1 + 2^(-v log2 e)) on the special function unit, within a few steps
+    // of fp32.  It takes 16 results a cycle and SM, which exponential and
+    // reciprocal for each value would make the bound; so two values share the
+    // reciprocal of their denominators' product (held below overflow: from
+    // 2^60 on v / 2^60 is below every type's last place).
+    float d[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float x = v[e] * -1.4426950408889634f;
+      asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(60.0f));
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(x));
+      d[e] = 1.0f + x;
+    }
+#pragma unroll
+    for (int e = 0; e < V; e += 2) {
+      const float other = e + 1 < V ? d[e + 1] : 1.0f;
+      float r;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d[e] * other));
+      v[e] *= r * other;
+      if (e + 1 < V) v[e + 1] *= r * d[e];
+    }
   } else {
-    return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.5f * v[e] * (1.0f + erff(v[e] * 0.70710678118654752f));
   }
 }
 
@@ -89,17 +105,92 @@ __device__ __forceinline__ Item<T, V> load_item(const void* x, int64_t at, int c
   return i;
 }
 
-template <int T, int V>
-__device__ __forceinline__ void item_floats(const Item<T, V>& i, float (&f)[V]) {
-  if constexpr (T == IE_DT_BF16X2) {
-    float l[V];
-    to_floats<IE_DT_BF16, V>(i.v, f);
-    to_floats<IE_DT_BF16, V>(i.lo, l);
-#pragma unroll
-    for (int e = 0; e < V; ++e) f[e] += l[e];
-  } else {
-    to_floats<T, V>(i.v, f);
+// Two fp32 values in one register pair, two operations per instruction (sm_100).
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+// V channels as pairs; V == 1: the second of the one pair is zero.
+template <int V>
+struct Pairs {
+  static constexpr int kCount = (V + 1) / 2;
+  uint64_t p[kCount];
+
+  __device__ __forceinline__ float operator[](int e) const {
+    const float2 f = floats_of(p[e / 2]);
+    return e % 2 == 0 ? f.x : f.y;
   }
+  __device__ __forceinline__ void set(const float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) p[i] = pair_of(f[2 * i], 2 * i + 1 < V ? f[2 * i + 1] : 0.0f);
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) p[i] = 0;
+  }
+  __device__ __forceinline__ void add(const Pairs& o) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) p[i] = add2(p[i], o.p[i]);
+  }
+  __device__ __forceinline__ void add_squares(const Pairs& o, const Pairs& minus) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+      const uint64_t d = add2(o.p[i], minus.p[i]);
+      p[i] = fma2(d, d, p[i]);
+    }
+  }
+};
+
+template <int T, int V>
+__device__ __forceinline__ Pairs<V> item_pairs(const Item<T, V>& i) {
+  Pairs<V> r;
+  if constexpr (V == 1) {
+    float f[1];
+    to_floats<T == IE_DT_BF16X2 ? static_cast<int>(IE_DT_BF16) : T, 1>(i.v, f);
+    if constexpr (T == IE_DT_BF16X2) {
+      float l[1];
+      to_floats<IE_DT_BF16, 1>(i.lo, l);
+      f[0] += l[0];
+    }
+    r.set(f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V / 2; ++k) {
+      if constexpr (T == IE_DT_F32) {
+        r.p[k] = pair_of(__uint_as_float(i.v.r[2 * k]), __uint_as_float(i.v.r[2 * k + 1]));
+      } else {
+        const float2 f = unpack_pair<T>(i.v.r[k]);
+        r.p[k] = pair_of(f.x, f.y);
+        if constexpr (T == IE_DT_BF16X2) {
+          const float2 l = unpack_pair<T>(i.lo.r[k]);
+          r.p[k] = add2(r.p[k], pair_of(l.x, l.y));
+        }
+      }
+    }
+  }
+  return r;
 }
 
 template <int T, int V>
@@ -118,91 +209,56 @@ __device__ __forceinline__ void store_item(void* y, int64_t at, int c_store, con
   }
 }
 
-// Two fp32 operations in one instruction (sm_100).
-__device__ __forceinline__ void add_pair(float& a0, float& a1, float b0, float b1) {
-  asm("{\n\t.reg .b64 a, b;\n\tmov.b64 a, {%0, %1};\n\tmov.b64 b, {%2, %3};\n\t"
-      "add.rn.f32x2 a, a, b;\n\tmov.b64 {%0, %1}, a;\n\t}"
-      : "+f"(a0), "+f"(a1)
-      : "f"(b0), "f"(b1));
-}
-__device__ __forceinline__ void fma_pair(float& d0, float& d1, float a0, float a1, float b0,
-                                         float b1) {  // d += a * b
-  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-      "mov.b64 d, {%0, %1};\n\tfma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
-      : "+f"(d0), "+f"(d1)
-      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
-}
-template <int V>
-__device__ __forceinline__ void add_to(float (&a)[V], const float (&b)[V]) {  // a += b
-  if constexpr (V == 1) {
-    a[0] += b[0];
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; e += 2) add_pair(a[e], a[e + 1], b[e], b[e + 1]);
-  }
-}
-template <int V>
-__device__ __forceinline__ void add_squares(float (&a)[V], const float (&b)[V],
-                                            const float (&minus)[V]) {  // a += (b + minus)^2
-  if constexpr (V == 1) {
-    const float d = b[0] + minus[0];
-    a[0] += d * d;
-  } else {
-#pragma unroll
-    for (int e = 0; e < V; e += 2) {
-      float d0 = b[e], d1 = b[e + 1];
-      add_pair(d0, d1, minus[e], minus[e + 1]);
-      fma_pair(a[e], a[e + 1], d0, d1, d0, d1);
-    }
-  }
-}
-
 // Running statistics of V channels over the pixels a thread has seen.
 template <int V>
 struct Running {
-  float mean[V], m2[V];
+  Pairs<V> mean, m2;
   int n = 0;
 
   __device__ __forceinline__ Running() {
-#pragma unroll
-    for (int e = 0; e < V; ++e) mean[e] = m2[e] = 0.0f;
+    mean.zero();
+    m2.zero();
   }
-  // Joins k > 0 pixels with sum s and squares q about their mean.
-  __device__ __forceinline__ void join(int k, const float (&batch_mean)[V], const float (&q)[V]) {
-    const float share = static_cast<float>(k) / static_cast<float>(n + k);
-    const float weight = static_cast<float>(n) * share;
+  // Joins k > 0 pixels of the given mean and squares about it.
+  __device__ __forceinline__ void join(int k, const Pairs<V>& batch, const Pairs<V>& squares) {
+    if (n == 0) {
+      mean = batch;
+      m2 = squares;
+    } else {
+      const float share = static_cast<float>(k) / static_cast<float>(n + k);
+      const float weight = static_cast<float>(n) * share;
+      const uint64_t share2 = pair_of(share, share), weight2 = pair_of(weight, weight);
+      const uint64_t minus1 = pair_of(-1.0f, -1.0f);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const float d = n == 0 ? 0.0f : batch_mean[e] - mean[e];
-      mean[e] = n == 0 ? batch_mean[e] : fmaf(d, share, mean[e]);
-      m2[e] += fmaf(d * d, weight, q[e]);
+      for (int i = 0; i < Pairs<V>::kCount; ++i) {
+        const uint64_t d = fma2(mean.p[i], minus1, batch.p[i]);
+        mean.p[i] = fma2(d, share2, mean.p[i]);
+        m2.p[i] = add2(m2.p[i], fma2(mul2(d, d), weight2, squares.p[i]));
+      }
     }
     n += k;
   }
   // A whole batch in registers.
-  __device__ __forceinline__ void add(const float (&f)[kGnBatch][V]) {
-    float s[V], q[V], minus[V];
+  __device__ __forceinline__ void add(const Pairs<V> (&f)[kGnBatch]) {
+    Pairs<V> s = f[0], q, minus;
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      s[e] = f[0][e];
-      q[e] = 0.0f;
+    for (int i = 1; i < kGnBatch; ++i) s.add(f[i]);
+    const uint64_t inv = pair_of(1.0f / kGnBatch, 1.0f / kGnBatch);
+    const uint64_t minus_inv = pair_of(-1.0f / kGnBatch, -1.0f / kGnBatch);
+#pragma unroll
+    for (int i = 0; i < Pairs<V>::kCount; ++i) {
+      minus.p[i] = mul2(s.p[i], minus_inv);
+      s.p[i] = mul2(s.p[i], inv);
     }
+    q.zero();
 #pragma unroll
-    for (int i = 1; i < kGnBatch; ++i) add_to<V>(s, f[i]);
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      s[e] *= 1.0f / kGnBatch;
-      minus[e] = -s[e];
-    }
-#pragma unroll
-    for (int i = 0; i < kGnBatch; ++i) add_squares<V>(q, f[i], minus);
+    for (int i = 0; i < kGnBatch; ++i) q.add_squares(f[i], minus);
     join(kGnBatch, s, q);
   }
   // One pixel.
-  __device__ __forceinline__ void add(const float (&f)[V]) {
-    float q[V];
-#pragma unroll
-    for (int e = 0; e < V; ++e) q[e] = 0.0f;
+  __device__ __forceinline__ void add(const Pairs<V>& f) {
+    Pairs<V> q;
+    q.zero();
     join(1, f, q);
   }
 };
@@ -219,7 +275,7 @@ __device__ __forceinline__ float warp_sum(float v) {
 // group.  scratch holds (V + 1) * threads floats.  (A single group wider than
 // the threads' columns: group_channels is what the columns hold.)
 template <int V>
-__device__ __forceinline__ void group_sums(const float (&v)[V], int cols, int rows,
+__device__ __forceinline__ void group_sums(const Pairs<V>& v, int cols, int rows,
                                            int group_channels, int groups, float* scratch,
                                            float* out) {
   const int width = cols * V, t = threadIdx.x, lane = t & 31;
@@ -306,8 +362,9 @@ struct Range {
 // first channel is `inner` channels into group `first`.
 template <int V>
 __device__ __forceinline__ void channel_affine(const GroupNormArgs& a, int c, int first, int inner,
-                                               const float2* stat, float (&mul)[V],
-                                               float (&add)[V]) {
+                                               const float2* stat, Pairs<V>* mul_pairs,
+                                               Pairs<V>* add_pairs) {
+  float mul[V], add[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const bool in = c + e < a.c;
@@ -319,16 +376,24 @@ __device__ __forceinline__ void channel_affine(const GroupNormArgs& a, int c, in
       ++first;
     }
   }
+  mul_pairs->set(mul);
+  add_pairs->set(add);
 }
 
 // Normalizes, activates and stores one item; channels past c become zero
 // (mul and add are zero there, but x may hold anything).
 template <int YT, int V, int ACT>
-__device__ __forceinline__ void finish_item(const GroupNormArgs& a, float (&f)[V],
-                                            const float (&mul)[V], const float (&add)[V],
-                                            uint8_t* y, int valid) {
+__device__ __forceinline__ void finish_item(const GroupNormArgs& a, const Pairs<V>& x,
+                                            const Pairs<V>& mul, const Pairs<V>& add, uint8_t* y,
+                                            int valid) {
+  float f[V];
 #pragma unroll
-  for (int e = 0; e < V; ++e) f[e] = activate<ACT>(fmaf(f[e], mul[e], add[e]), a.low, a.high);
+  for (int i = 0; i < Pairs<V>::kCount; ++i) {
+    const float2 r = floats_of(fma2(x.p[i], mul.p[i], add.p[i]));
+    f[2 * i] = r.x;
+    if (2 * i + 1 < V) f[2 * i + 1] = r.y;
+  }
+  activate<ACT, V>(f, a.low, a.high);
   if (valid < V) {
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = e < valid ? f[e] : 0.0f;
@@ -387,22 +452,17 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
   const int first = col * V / r.group_channels, inner = col * V - first * r.group_channels;
   asm volatile("cp.async.wait_all;" ::: "memory");
 
-  auto item = [&](int i, float(&f)[V]) {
+  auto item = [&](int i) {
     Item<XT, V> it;
     it.v = load_bytes<16>(mine + i * kStep);
     if constexpr (XT == IE_DT_BF16X2) it.lo = load_bytes<16>(mine + i * kStep + kGnThreads * 16);
-    item_floats<XT, V>(it, f);
+    return item_pairs<XT, V>(it);
   };
   // the block's mean of each group, then the squares about it
-  float v[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = 0.0f;
+  Pairs<V> v;
+  v.zero();
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    float f[V];
-    item(i, f);
-    add_to<V>(v, f);
-  }
+  for (int i = 0; i < n; ++i) v.add(item(i));
   group_sums<V>(v, r.cols, r.rows, r.group_channels, a.range_groups, scratch, sums);
   const float inv = 1.0f / (static_cast<float>(count) * static_cast<float>(r.group_channels));
   {
@@ -411,18 +471,16 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
 #pragma unroll
     for (int e = 0; e < V; ++e) {  // padding channels: the group's that would follow
       minus[e] = -sums[min(g, a.range_groups - 1)] * inv;
-      v[e] = 0.0f;
       if (++in_group == r.group_channels) {
         in_group = 0;
         ++g;
       }
     }
+    Pairs<V> minus_pairs;
+    minus_pairs.set(minus);
+    v.zero();
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      float f[V];
-      item(i, f);
-      add_squares<V>(v, f, minus);
-    }
+    for (int i = 0; i < n; ++i) v.add_squares(item(i), minus_pairs);
   }
   for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) own[g].x = sums[g] * inv;
   __syncthreads();
@@ -446,17 +504,15 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
     });
   }
   __syncthreads();
-  float g[V], b[V];
-  if (n > 0) channel_affine<V>(a, c, first, inner, stat, g, b);
+  Pairs<V> g, b;
+  if (n > 0) channel_affine<V>(a, c, first, inner, stat, &g, &b);
   uint8_t* y = static_cast<uint8_t*>(a.y) +
                channel_at<YT>(p0 + row, a.c_store, c) * element_bytes(YT);
   const int64_t y_step = static_cast<int64_t>(r.rows) * channel_at<YT>(1, a.c_store, 0) *
                          element_bytes(YT);
 #pragma unroll(ACT == kActGelu ? 1 : 2)
   for (int i = 0; i < n; ++i, y += y_step) {
-    float f[V];
-    item(i, f);
-    finish_item<YT, V, ACT>(a, f, g, b, y, a.c - c);
+    finish_item<YT, V, ACT>(a, item(i), g, b, y, a.c - c);
   }
   if (a.blocks > 1) cluster.barrier_wait();
 }
@@ -464,14 +520,15 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
 // Statistics of one block of pixels of an image and channel range.
 template <int XT, int V>
 __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const GroupNormArgs a) {
+  namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* sums = reinterpret_cast<float*>(smem);  // [range_groups]
+  float2* own = reinterpret_cast<float2*>(smem);  // [range_groups] of this block
+  float* sums = reinterpret_cast<float*>(own + a.range_groups);  // [range_groups]
   float* scratch = sums + a.range_groups;
   const uint32_t unit = blockIdx.x / static_cast<uint32_t>(a.blocks);
   const int block = static_cast<int>(blockIdx.x - unit * a.blocks);
-  const uint32_t of_launch = unit / static_cast<uint32_t>(a.launch_ranges);
-  const int range = a.first_range + static_cast<int>(unit - of_launch * a.launch_ranges);
-  const int64_t image = a.first_image + of_launch;
+  const int64_t image = unit / static_cast<uint32_t>(a.ranges);
+  const int range = static_cast<int>(unit - image * a.ranges);
   const Range r(a, range);
   const int all = (r.channels + V - 1) / V;  // padding channels have no statistics
   const int cols = min(all, kGnThreads), rows = kGnThreads / cols;
@@ -495,26 +552,26 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const G
       }
 #pragma unroll
       for (int k = 0; k < K; ++k) {
-        float f[kGnBatch][V];
+        Pairs<V> f[kGnBatch];
 #pragma unroll
-        for (int e = 0; e < kGnBatch; ++e) item_floats<XT, V>(it[k * kGnBatch + e], f[e]);
+        for (int e = 0; e < kGnBatch; ++e) f[e] = item_pairs<XT, V>(it[k * kGnBatch + e]);
         run.add(f);
       }
     }
     for (; left > 0; --left, from_x += step) {
-      float f[V];
-      item_floats<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store), f);
-      run.add(f);
+      run.add(item_pairs<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store)));
     }
   }
   // the block's mean of each group, then each channel's squares about it
   const int group_channels = all > cols ? cols * V : r.group_channels;
-  float v[V];
+  Pairs<V> sum = run.mean;
+  const uint64_t seen = pair_of(static_cast<float>(run.n), static_cast<float>(run.n));
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = run.n > 0 ? run.mean[e] * static_cast<float>(run.n) : 0.0f;
-  group_sums<V>(v, cols, rows, group_channels, a.range_groups, scratch, sums);
+  for (int i = 0; i < Pairs<V>::kCount; ++i) sum.p[i] = mul2(sum.p[i], seen);
+  group_sums<V>(sum, cols, rows, group_channels, a.range_groups, scratch, sums);
   const float inv = 1.0f / (static_cast<float>(count) * static_cast<float>(r.group_channels));
   int g = col * V / group_channels, inner = col * V - g * group_channels;
+  float v[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const float d = run.mean[e] - sums[min(g, a.range_groups - 1)] * inv;
@@ -524,20 +581,49 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const G
       ++g;
     }
   }
-  // [unit][group][block], so that a warp reads a group's blocks side by side
-  float2* to = a.partial + static_cast<int64_t>(unit) * a.range_groups * a.blocks + block;
-  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) {
-    to[static_cast<int64_t>(i) * a.blocks].x = sums[i] * inv;
-  }
+  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) own[i].x = sums[i] * inv;
   __syncthreads();
-  group_sums<V>(v, cols, rows, group_channels, a.range_groups, scratch, sums);
-  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) {
-    to[static_cast<int64_t>(i) * a.blocks].y = sums[i];
+  sum.set(v);
+  group_sums<V>(sum, cols, rows, group_channels, a.range_groups, scratch, sums);
+  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) own[i].y = sums[i];
+  // A cluster's blocks are joined here, so that the second kernel's blocks,
+  // which each join them all, find few parts: [unit][group][part].
+  cg::cluster_group cluster = cg::this_cluster();
+  const int size = static_cast<int>(cluster.num_blocks());
+  cluster.sync();
+  const int part = block / size, first_pixel = part * a.part_share;
+  const int pixels = min(a.pixels, first_pixel + a.part_share) - first_pixel;
+  for (int i = static_cast<int>(cluster.block_rank()) * kGnThreads + threadIdx.x;
+       i < a.range_groups; i += kGnThreads * size) {
+    float s = 0.0f, q = 0.0f;
+    float2 o[kGnCluster];
+#pragma unroll
+    for (int k = 0; k < kGnCluster; ++k) {
+      o[k] = k < size ? *cluster.map_shared_rank(own + i, k) : make_float2(0.0f, 0.0f);
+    }
+#pragma unroll
+    for (int k = 0; k < kGnCluster; ++k) {
+      const int w = min(pixels, (k + 1) * a.share) - k * a.share;
+      if (k < size && w > 0) s += static_cast<float>(w) * o[k].x;
+    }
+    const float mu = s / static_cast<float>(pixels);
+#pragma unroll
+    for (int k = 0; k < kGnCluster; ++k) {
+      const int w = min(pixels, (k + 1) * a.share) - k * a.share;
+      const float d = o[k].x - mu;
+      if (k < size && w > 0) {
+        q += o[k].y + static_cast<float>(w) * static_cast<float>(r.group_channels) * d * d;
+      }
+    }
+    a.partial[(static_cast<int64_t>(unit) * a.range_groups + i) * a.parts + part] =
+        make_float2(mu, q);
   }
+  cluster.sync();  // no block leaves while another reads its statistics
 }
 
 // Joins the blocks' statistics (every block of the launch for itself) and
-// normalizes.  Blocks run over the pixels from the end, which L2 still holds.
+// normalizes.  Every block runs over its pixels from their end: the statistics
+// kernel's blocks, all on the GPU at once, read the ends last, so L2 holds them.
 template <int XT, int YT, int V, int ACT>
 __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 : 4)
     group_norm_apply_kernel(const GroupNormArgs a,
@@ -545,26 +631,30 @@ __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 :
   extern __shared__ __align__(16) uint8_t smem[];
   float2* stat = reinterpret_cast<float2*>(smem);
   const uint32_t unit = blockIdx.x / static_cast<uint32_t>(apply_blocks);
-  const int block = apply_blocks - 1 - static_cast<int>(blockIdx.x - unit * apply_blocks);
-  const uint32_t of_launch = unit / static_cast<uint32_t>(a.launch_ranges);
-  const int range = a.first_range + static_cast<int>(unit - of_launch * a.launch_ranges);
-  const int64_t image = a.first_image + of_launch;
+  const int block = static_cast<int>(blockIdx.x - unit * apply_blocks);
+  const int64_t image = unit / static_cast<uint32_t>(a.ranges);
+  const int range = static_cast<int>(unit - image * a.ranges);
   const Range r(a, range);
   const int lane = threadIdx.x & 31;
   for (int g = threadIdx.x >> 5; g < a.range_groups; g += kGnThreads / 32) {
-    const float2* p = a.partial + (static_cast<int64_t>(unit) * a.range_groups + g) * a.blocks;
+    const float2* p = a.partial + (static_cast<int64_t>(unit) * a.range_groups + g) * a.parts;
+    // up to 64 parts stay in registers between the mean and the squares
+    const float2 mine[2] = {lane < a.parts ? p[lane] : make_float2(0.0f, 0.0f),
+                            lane + 32 < a.parts ? p[lane + 32] : make_float2(0.0f, 0.0f)};
+    auto pixels_of = [&](int k) {
+      return static_cast<float>(max(0, min(a.pixels, (k + 1) * a.part_share) - k * a.part_share));
+    };
     float s = 0.0f, q = 0.0f;
-    for (int k = lane; k < a.blocks; k += 32) {
-      const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
-      if (w > 0) s += static_cast<float>(w) * p[k].x;
+    for (int k = lane, i = 0; k < a.parts; k += 32, ++i) {
+      if (pixels_of(k) > 0.0f) s += pixels_of(k) * (i == 0 ? mine[0] : i == 1 ? mine[1] : p[k]).x;
     }
     const float mu = warp_sum(s) / static_cast<float>(a.pixels);
-    for (int k = lane; k < a.blocks; k += 32) {
-      const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
-      if (w <= 0) continue;
-      const float2 o = p[k];
+    for (int k = lane, i = 0; k < a.parts; k += 32, ++i) {
+      const float2 o = i == 0 ? mine[0] : i == 1 ? mine[1] : p[k];
       const float d = o.x - mu;
-      q += o.y + static_cast<float>(w) * static_cast<float>(r.group_channels) * d * d;
+      if (pixels_of(k) > 0.0f) {
+        q += o.y + pixels_of(k) * static_cast<float>(r.group_channels) * d * d;
+      }
     }
     q = warp_sum(q);
     const float size = static_cast<float>(a.pixels) * static_cast<float>(r.group_channels);
@@ -582,15 +672,15 @@ __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 :
     if (row >= rows || row >= count) continue;
     const int c = r.c0 + col * V;
     const int first = col * V / r.group_channels;
-    float mul[V], add[V];
-    channel_affine<V>(a, c, first, col * V - first * r.group_channels, stat, mul, add);
+    Pairs<V> mul, add;
+    channel_affine<V>(a, c, first, col * V - first * r.group_channels, stat, &mul, &add);
     constexpr int K = ACT == kActGelu || XT == IE_DT_BF16X2 ? 2 : 4;
-    const int64_t x_step = static_cast<int64_t>(rows) * channel_at<XT>(1, a.c_store, 0);
-    const int64_t y_step = static_cast<int64_t>(rows) * channel_at<YT>(1, a.c_store, 0) *
+    const int64_t x_step = -static_cast<int64_t>(rows) * channel_at<XT>(1, a.c_store, 0);
+    const int64_t y_step = -static_cast<int64_t>(rows) * channel_at<YT>(1, a.c_store, 0) *
                            element_bytes(YT);
-    int64_t from_x = channel_at<XT>(p0 + row, a.c_store, c);
-    uint8_t* y = static_cast<uint8_t*>(a.y) +
-                 channel_at<YT>(p0 + row, a.c_store, c) * element_bytes(YT);
+    const int64_t last = p0 + count - 1 - row;
+    int64_t from_x = channel_at<XT>(last, a.c_store, c);
+    uint8_t* y = static_cast<uint8_t*>(a.y) + channel_at<YT>(last, a.c_store, c) * element_bytes(YT);
     int left = (count - row + rows - 1) / rows;
     for (; left >= K; left -= K) {
       Item<XT, V> it[K];
@@ -600,15 +690,12 @@ __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 :
       }
 #pragma unroll
       for (int e = 0; e < K; ++e, y += y_step) {
-        float f[V];
-        item_floats<XT, V>(it[e], f);
-        finish_item<YT, V, ACT>(a, f, mul, add, y, a.c - c);
+        finish_item<YT, V, ACT>(a, item_pairs<XT, V>(it[e]), mul, add, y, a.c - c);
       }
     }
     for (; left > 0; --left, from_x += x_step, y += y_step) {
-      float f[V];
-      item_floats<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store), f);
-      finish_item<YT, V, ACT>(a, f, mul, add, y, a.c - c);
+      finish_item<YT, V, ACT>(a, item_pairs<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store)), mul,
+                              add, y, a.c - c);
     }
   }
 }

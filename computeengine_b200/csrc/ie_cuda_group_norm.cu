@@ -50,10 +50,6 @@ constexpr int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
 
 constexpr int64_t kSms = 148;
 constexpr int64_t kSmemPerSm = 227 * 1024;
-// Bytes of x that the two-kernel path normalizes per pair of launches: with
-// the y they become they stay in the 126 MB L2 between the two reads.
-constexpr int64_t kWaveBytes = 72 << 20;
-
 int64_t item_bytes(int x_type, int v) {
   return int64_t{v} * element_bytes(x_type) * (x_type == IE_DT_BF16X2 ? 2 : 1);
 }
@@ -64,9 +60,8 @@ struct Plan {
   int range_groups = 1, ranges = 1;  // channel ranges of whole groups
   int blocks = 1;                    // per image and range: cluster size, or statistics blocks
   int64_t smem = 0;
-  // two-kernel path: (image, range) units of one pair of launches
-  int64_t wave_images = 1;
-  int wave_ranges = 1;
+  // two-kernel path
+  int joined = 1;  // statistics blocks of a cluster
   int apply_blocks = 1;
   int64_t workspace = 0;
 };
@@ -77,93 +72,91 @@ bool range_fits(const ie_group_norm_desc* d, int64_t g, int v) {
 }
 
 // The choice between one kernel that holds x in shared memory and two that
-// read it twice, and the split of the work, by an estimate of the time: blocks
-// run in waves over the SMs; a wave costs about 4 us of latencies (load, join,
-// store), more with the cluster's barriers, and all of them together no less
-// than the bytes at the measured 6.5 TB/s.  Pieces of a pixel narrower than
-// 128 bytes waste part of each DRAM access.
+// read it twice, and the split of an image's work.  It does not depend on the
+// number of images, so an image's result is the same in every batch.
+//
+// One kernel: channel ranges of whole groups, at least 64 bytes of a pixel (32
+// where that saves a larger cluster; narrower pieces waste part of each DRAM
+// access), cut into blocks of pixels of at most 32768 elements and half an SM's
+// shared memory, so that one block's loads cover another's arithmetic: 32
+// images of 56 x 56 x 256 fp32 take 59 us in clusters of 2, 70 us in clusters
+// of 8 and a quarter of the size.  Up to 8 blocks are a cluster; ranges too
+// large for that take two kernels, 256 blocks an image at most.
 Plan plan_for(const ie_group_norm_desc* d, int v) {
-  Plan best;
+  Plan p;
   const int64_t cg = d->c / d->groups, pixels = d->h * d->w;
   const int64_t xb = item_bytes(d->x_type, 1), yb = item_bytes(d->y_type, 1);
-  best.v = v;
-  double best_ns = 1e30;
-  for (int64_t g = 1; v > 1 && g <= d->groups; ++g) {
-    if (!range_fits(d, g, v)) continue;
-    const int64_t ranges = d->groups / g;
-    const int64_t stored = d->c_store - (ranges - 1) * g * cg;  // of the last range
+  p.v = v;
+  auto smem_for = [&](int64_t g, int blocks) {
+    const int64_t stored = d->c_store - (d->groups / g - 1) * g * cg;  // of the last range
     const int64_t cols = ceil_div(std::max(stored, g * cg), v);
-    if (cols > kGnThreads) break;
+    if (cols > kGnThreads) return int64_t{1} << 40;
     const int64_t rows = kGnThreads / cols;
-    const double segment = static_cast<double>(g * cg * xb);
-    const double waste = segment < 32 ? 2.0 : segment < 64 ? 1.5 : segment < 128 ? 1.15 : 1.0;
-    for (int blocks = 1; blocks <= 16; blocks *= 2) {
-      const int64_t share = ceil_div(pixels, blocks);
-      const int64_t held = ceil_div(share, rows) * kGnThreads * item_bytes(d->x_type, v);
-      const int64_t smem = held + (v + 1) * kGnThreads * 4 + (20 + 8 * blocks) * g + 32;
-      if (smem > kSmemPerSm || (blocks > 1 && share * (blocks - 1) >= pixels)) continue;
-      const int64_t per_sm = std::min<int64_t>(4, (kSmemPerSm + 1024) / (smem + 1024));
-      const int64_t total = d->n * ranges * blocks;
-      const int64_t waves = ceil_div(total, kSms * per_sm);
-      const double latency = blocks > 8 ? 5500.0 : blocks > 1 ? 4500.0 : 4000.0;
-      // one wave: no SM can do better than its own share of the bandwidth
-      const double busy = static_cast<double>(std::min<int64_t>(total, kSms)) / kSms;
-      const double bytes = static_cast<double>(d->n * pixels * d->c) * static_cast<double>(xb + yb);
-      // with few blocks on an SM, one's loads, arithmetic and stores leave the
-      // memory idle in turn (measured: one block per SM reaches half of it)
-      const double overlap = per_sm == 1 ? 2.0 : per_sm == 2 ? 1.4 : per_sm == 3 ? 1.15 : 1.0;
-      const double ns = latency + std::max(latency * static_cast<double>(waves - 1),
-                                           waste * overlap * bytes / (6500.0 * busy));
-      if (ns < best_ns) {
-        best_ns = ns;
-        best.cluster = true;
-        best.range_groups = static_cast<int>(g);
-        best.ranges = static_cast<int>(ranges);
-        best.blocks = blocks;
-        best.smem = smem;
-      }
+    return ceil_div(ceil_div(pixels, blocks), rows) * kGnThreads * item_bytes(d->x_type, v) +
+           (v + 1) * kGnThreads * 4 + (20 + 8 * blocks) * g + 32;
+  };
+  auto fits = [&](int64_t g, int blocks) {
+    const int64_t share = ceil_div(pixels, blocks);
+    return smem_for(g, blocks) <= kSmemPerSm / 2 - 1024 && share * g * cg <= 32768 &&
+           (blocks == 1 || share * (blocks - 1) < pixels);
+  };
+  auto accept = [&](int64_t g, int blocks) {
+    p.cluster = true;
+    p.range_groups = static_cast<int>(g);
+    p.ranges = static_cast<int>(d->groups / g);
+    p.blocks = blocks;
+    p.smem = smem_for(g, blocks);
+  };
+  for (int64_t segment = 64; v > 1 && segment >= 32 && !p.cluster; segment /= 2) {
+    int64_t g = 1;
+    while (g < d->groups && !(range_fits(d, g, v) && g * cg * xb >= segment)) ++g;
+    if (!range_fits(d, g, v)) break;
+    for (int blocks = 1; blocks <= 8 && !p.cluster; blocks *= 2) {
+      if (fits(g, blocks)) accept(g, blocks);
     }
   }
-  // two kernels: a second launch, x read again from L2 (about twice as fast)
-  const double two_ns = 9000.0 + static_cast<double>(d->n * pixels * d->c_store) *
-                                     (1.5 * static_cast<double>(xb) + static_cast<double>(yb)) /
-                                     6500.0;
-  if (best.cluster && best_ns <= two_ns) return best;
-  best.cluster = false;
-  // ranges: whole pixels if the threads cover them and the image fits a wave,
-  // else the narrowest range of at least 256 bytes
-  const int64_t image = pixels * d->c_store * xb;
-  best.range_groups = static_cast<int>(d->groups);
-  const bool whole = ceil_div(d->c, v) <= kGnThreads && image <= kWaveBytes;
-  if (!whole) {
-    best.range_groups = 0;
+  // small images: at least 16 KB a block
+  for (int64_t g = p.range_groups + 1;
+       p.cluster && p.blocks == 1 && g <= d->groups && p.range_groups * cg * pixels * xb < 16384 &&
+       g * cg <= kGnThreads * v;
+       ++g) {
+    if (range_fits(d, g, v) && fits(g, 1)) accept(g, 1);
+  }
+  if (p.cluster) return p;
+  // ranges: whole pixels if the threads cover them, else the narrowest range of
+  // at least 256 bytes
+  p.range_groups = static_cast<int>(d->groups);
+  if (ceil_div(d->c, v) > kGnThreads) {
+    p.range_groups = 0;
     for (int64_t g = 1; g <= d->groups; ++g) {
       if (!range_fits(d, g, v)) continue;
       // several groups only within the threads' columns
-      if (best.range_groups > 0 && ceil_div(g * cg, v) > kGnThreads) break;
-      best.range_groups = static_cast<int>(g);
+      if (p.range_groups > 0 && ceil_div(g * cg, v) > kGnThreads) break;
+      p.range_groups = static_cast<int>(g);
       if (g * cg * xb >= 256) break;
     }
   }
-  const int64_t channels = best.range_groups * cg;
-  best.ranges = static_cast<int>(d->groups / best.range_groups);
+  const int64_t channels = p.range_groups * cg;
+  p.ranges = static_cast<int>(d->groups / p.range_groups);
   const int64_t rows = std::max<int64_t>(1, kGnThreads / ceil_div(channels, v));
-  if (image <= kWaveBytes) {
-    best.wave_images = std::min(d->n, std::max<int64_t>(1, kWaveBytes / image));
-    best.wave_ranges = best.ranges;
-  } else {
-    best.wave_images = 1;
-    best.wave_ranges = static_cast<int>(
-        std::min<int64_t>(best.ranges, std::max<int64_t>(1, kWaveBytes * best.ranges / image)));
+  const int64_t units = d->n * p.ranges;
+  int64_t blocks = std::min(ceil_div(pixels * channels * xb, 32768), int64_t{256});
+  blocks = std::max<int64_t>(1, std::min(blocks, ceil_div(pixels, kGnBatch * rows)));
+  if (blocks > kGnCluster) {  // whole clusters, and every block has pixels
+    blocks -= blocks % kGnCluster;
+    while (blocks > kGnCluster && ceil_div(pixels, blocks) * (blocks - 1) >= pixels) {
+      blocks -= kGnCluster;
+    }
+    p.joined = kGnCluster;
   }
-  const int64_t units = best.wave_images * best.wave_ranges;
-  best.blocks = static_cast<int>(
-      std::max<int64_t>(1, std::min(2 * kSms / units, ceil_div(pixels, kGnBatch * rows))));
-  best.apply_blocks = static_cast<int>(
-      std::max<int64_t>(1, std::min(2 * kSms / units, ceil_div(pixels, 4 * rows))));
-  best.smem = (v + 1) * kGnThreads * 4 + 4 * best.range_groups;
-  best.workspace = units * best.blocks * best.range_groups * static_cast<int64_t>(sizeof(float2));
-  return best;
+  p.blocks = static_cast<int>(blocks);
+  p.apply_blocks = static_cast<int>(std::max<int64_t>(
+      1, std::min(std::max(4 * kSms / units, ceil_div(pixels * channels * (xb + yb), 262144)),
+                  ceil_div(pixels, 4 * rows))));
+  p.smem = (v + 1) * kGnThreads * 4 + 12 * p.range_groups + 8;
+  p.workspace =
+      units * (p.blocks / p.joined) * p.range_groups * static_cast<int64_t>(sizeof(float2));
+  return p;
 }
 
 // Vectors of 16 bytes of x where pixels, pointers and ranges allow it.
@@ -181,28 +174,23 @@ int vector_width(const ie_group_norm_desc* d) {
 }
 
 template <class Kernel>
-int allow_smem(Kernel kernel, int64_t smem, bool wide_cluster) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       static_cast<int>(smem));
-  if (e == cudaSuccess && wide_cluster) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  }
+int allow_smem(Kernel kernel, int64_t smem) {
+  const cudaError_t e = cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   return e == cudaSuccess ? IE_OK : fail(IE_RUNTIME, "group_norm: %s", cudaGetErrorString(e));
 }
 
-template <int XT, int YT, int V, int ACT>
-int launch_cluster(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
-  auto kernel = group_norm_cluster_kernel<XT, YT, V, ACT>;
-  const int rc = allow_smem(kernel, p.smem, p.blocks > 8);
-  if (rc != IE_OK) return rc;
+template <class Kernel>
+int launch_clusters(Kernel kernel, int64_t blocks, int cluster, int64_t smem, cudaStream_t s,
+                    const GroupNormArgs& a) {
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(images * p.ranges * p.blocks));
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(kGnThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(p.smem);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = s;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = static_cast<unsigned>(p.blocks);
+  attr.val.clusterDim.x = static_cast<unsigned>(cluster);
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
@@ -215,28 +203,26 @@ int launch_cluster(const GroupNormArgs& a, const Plan& p, int64_t images, cudaSt
 }
 
 template <int XT, int YT, int V, int ACT>
-int launch_two(GroupNormArgs a, const Plan& p, int64_t images, cudaStream_t s) {
+int launch_cluster(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
+  auto kernel = group_norm_cluster_kernel<XT, YT, V, ACT>;
+  const int rc = allow_smem(kernel, p.smem);
+  if (rc != IE_OK) return rc;
+  return launch_clusters(kernel, images * p.ranges * p.blocks, p.blocks, p.smem, s, a);
+}
+
+template <int XT, int YT, int V, int ACT>
+int launch_two(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
   auto stats = group_norm_stats_kernel<XT, V>;
   auto apply = group_norm_apply_kernel<XT, YT, V, ACT>;
   const int64_t apply_smem = 8 * p.range_groups;
-  int rc = allow_smem(stats, p.smem, false);
-  if (rc == IE_OK) rc = allow_smem(apply, apply_smem, false);
-  for (int64_t i = 0; rc == IE_OK && i < images; i += p.wave_images) {
-    a.first_image = i;
-    const int64_t wave = std::min(p.wave_images, images - i);
-    for (int r = 0; rc == IE_OK && r < p.ranges; r += p.wave_ranges) {
-      a.first_range = r;
-      a.launch_ranges = std::min(p.wave_ranges, p.ranges - r);
-      const int64_t units = wave * a.launch_ranges;
-      stats<<<static_cast<unsigned>(units * p.blocks), kGnThreads, p.smem, s>>>(a);
-      rc = check_launch("group_norm statistics");
-      if (rc != IE_OK) break;
-      apply<<<static_cast<unsigned>(units * p.apply_blocks), kGnThreads, apply_smem, s>>>(
-          a, p.apply_blocks);
-      rc = check_launch("group_norm");
-    }
-  }
-  return rc;
+  int rc = allow_smem(stats, p.smem);
+  if (rc == IE_OK) rc = allow_smem(apply, apply_smem);
+  const int64_t units = images * p.ranges;
+  if (rc == IE_OK) rc = launch_clusters(stats, units * p.blocks, p.joined, p.smem, s, a);
+  if (rc != IE_OK) return rc;
+  apply<<<static_cast<unsigned>(units * p.apply_blocks), kGnThreads, apply_smem, s>>>(
+      a, p.apply_blocks);
+  return check_launch("group_norm");
 }
 
 template <int XT, int YT, int ACT>
@@ -323,6 +309,8 @@ int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const
   a.ranges = p.ranges;
   a.blocks = p.blocks;
   a.share = static_cast<int>(ceil_div(a.pixels, p.blocks));
+  a.parts = p.blocks / p.joined;
+  a.part_share = a.share * p.joined;
   for (int last = 0; last < 2; ++last) {
     const int64_t channels = int64_t{p.range_groups} * a.group_channels;
     const int64_t stored = last ? desc->c_store - (p.ranges - 1) * channels : channels;
