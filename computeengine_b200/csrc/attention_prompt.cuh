@@ -9,13 +9,16 @@
 // The rows of a tile are 128 positions of one head, or, for few positions, all
 // positions of several heads that read the same kv head.
 //
-// Each tile has two S buffers, so the threads of a row always find the next S:
-// from P in TMEM to the next S there pass the MMAs and 400 cycles of latency,
-// which took a third of the time when a tile had one S of 128 keys.  The price
-// is that S of 64 keys costs 49 cycles per 16 elements of the head where half
-// of one of 128 keys costs 32 (Q is read from shared memory for each), so a
-// head of 128 runs at most at 79% of the tensor core's rate.  The exponentials
-// take 16 a cycle and SM; part of them is a polynomial on the FMA pipes.
+// From P in TMEM to the next S there pass the MMAs and 400 cycles of latency.
+// Tiles with heads of 128 have two S buffers, so the threads of a row always
+// find the next S; with one S of 128 keys they waited a third of the time.  The
+// price is that S of 64 keys costs 49 cycles per 16 elements of the head where
+// half of one of 128 keys costs 32 (Q is read from shared memory for each), so a
+// head of 128 runs at most at 79% of the tensor core's rate.  With heads of 64
+// there is room for two blocks per SM instead.  Then the exponentials are what
+// takes longest (16 a cycle and SM); a polynomial on the FMA pipes for a quarter
+// of them changed nothing (113 to 121 us against 113 to 118 us for 4096 tokens,
+// 16 heads of 64).
 // Warps 0-3 and 4-7 hold the rows of the tiles, warps 8 and 9 issue their MMAs
 // (one thread for both tiles spent 2200 cycles a step on the waits between
 // them), warp 10 the TMA loads of Q, K and V, warp 11 clears the rows of V
@@ -32,7 +35,6 @@ constexpr unsigned kErrAttnQ = 0x201, kErrAttnKv = 0x202, kErrAttnEmpty = 0x203,
 
 constexpr int kPromptThreads = 384;
 constexpr int kStep = 64;      // keys per step
-constexpr int kPolyEvery = 4;  // one pair of exponentials in so many is a polynomial
 
 struct PromptArgs : AttentionArgs {
   int tiles;           // blocks per (head unit, batch row), documents: upper bound in all
@@ -52,8 +54,14 @@ struct PromptPlan {
   static constexpr int kCols = DP / 64;               // 128-byte wide column blocks of a tile
   static constexpr int kQ = kCols * 128 * 128;        // bytes of 128 rows of Q
   static constexpr int kKv = kCols * kStep * 128;     // bytes of a step's K or V
-  static constexpr int kSlot = 2 * kKv;               // V of a step, K of the step two ahead
-  static constexpr int kStages = DP == 128 ? 5 : 8;
+  // Heads of 128: two S buffers per tile, one block per SM.  Heads of 64: one S
+  // buffer, so that two blocks share the SM's tensor memory (and its registers):
+  // four tiles hide each other's latencies.
+  static constexpr int kBuffers = DP == 128 ? 2 : 1;
+  static constexpr int kBlocks = DP == 128 ? 1 : 2;   // per SM
+  static constexpr int kColumns = DP == 128 ? 512 : 256;  // of tensor memory
+  static constexpr int kSlot = 2 * kKv;               // V of a step, K of one ahead
+  static constexpr int kStages = DP == 128 ? 5 : 4;
   static constexpr int kSmem = 2 * kQ + kStages * kSlot + 1024 + 512;
 };
 
@@ -134,31 +142,6 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   return y;
 }
 
-// 2^x for two values x <= 8 without the special function unit: x = n + f with
-// n the nearest integer (adding 1.5 * 2^23 leaves it in the low bits) and f in
-// [-1/2, 1/2], 2^f by its minimax polynomial of degree 4 with 2^0 = 1 exactly
-// (relative error below 3e-6; the weights are rounded to 2^-9 or 2^-12), n
-// added to the exponent.  Below -127 the result is exactly 0.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-  float a, b;
-  unpair(x, &a, &b);
-  x = pair_of(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
-  const uint64_t magic = pair_of(12582912.0f, 12582912.0f);
-  const uint64_t shifted = add2(x, magic);
-  const uint64_t n = add2(shifted, pair_of(-12582912.0f, -12582912.0f));
-  const uint64_t f = fma2(n, pair_of(-1.0f, -1.0f), x);
-  uint64_t p = fma2(f, pair_of(0.009582852944731712f, 0.009582852944731712f),
-                    pair_of(0.055906426161527634f, 0.055906426161527634f));
-  p = fma2(p, f, pair_of(0.24024099111557007f, 0.24024099111557007f));
-  p = fma2(p, f, pair_of(0.6931241750717163f, 0.6931241750717163f));
-  p = fma2(p, f, pair_of(1.0f, 1.0f));
-  float pa, pb, sa, sb;
-  unpair(p, &pa, &pb);
-  unpair(shifted, &sa, &sb);
-  return pair_of(__uint_as_float(__float_as_uint(pa) + (__float_as_uint(sa) << 23)),
-                 __uint_as_float(__float_as_uint(pb) + (__float_as_uint(sb) << 23)));
-}
-
 // tanh(u) / u for |u| <= kTanhLimit as a polynomial in u^2 (minimax of tanh u
 // with slope 1 at 0, absolute error below 2.7e-7).
 constexpr float kTanhLimit = 0.75f;
@@ -171,12 +154,12 @@ __device__ __forceinline__ uint64_t tanh_ratio(uint64_t uu) {
 }
 
 template <int DP, int T, bool CAP, bool BIAS>
-__global__ void __launch_bounds__(kPromptThreads, 1)
+__global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     attention_prompt_kernel(const PromptArgs a, const __grid_constant__ CUtensorMap map_q,
                             const __grid_constant__ CUtensorMap map_k,
                             const __grid_constant__ CUtensorMap map_v) {
   using P = PromptPlan<DP>;
-  constexpr int kStages = P::kStages;
+  constexpr int kStages = P::kStages, kBuffers = P::kBuffers;
   extern __shared__ uint8_t smem_raw[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -238,12 +221,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const bool last_short =
       length % kStep != 0 && begin + steps == (length + kStep - 1) / kStep;
   // A slot of the ring holds what a tile's MMAs wait for together: K of the
-  // first two steps, then V of a step and K of the step two ahead.
+  // first kBuffers steps, then V of a step and K of the step kBuffers ahead.
   const int slots = steps > 0 ? steps + 1 : 0;
   auto load_slot = [&](int i, int slot) {
     // a barrier of its own lets warp 11 wait for the last load from the start
     uint64_t* full = last_short && i == slots - 1 ? short_full : &kv_full[slot];
-    const int first = i == 0 ? 0 : i - 1, second = i + 1;  // steps of the two halves
+    const int first = i == 0 ? 0 : i - 1;  // steps of the two halves
+    const int second = i == 0 && kBuffers == 1 ? steps : i + kBuffers - 1;
     mbar_arrive_expect_tx(full, second < steps ? 2 * P::kKv : P::kKv);
     uint8_t* to = ring + slot * P::kSlot;
     for (int c = 0; c < P::kCols; ++c) {
@@ -256,7 +240,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   };
   if (warp == 8) {
-    tmem_alloc(tmem_slot, 512);
+    tmem_alloc(tmem_slot, P::kColumns);
     tmem_relinquish();
   } else if (warp == 10) {
     // barriers 0 .. 13 + 2 kStages in their order above, one per lane
@@ -289,11 +273,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // TMEM columns: S buffer b of tile t (and P over it) at 128 t + 64 b, O at
-  // 256 + DP t
+  // TMEM columns: S buffer b of tile t (and P over it) at 64 (kBuffers t + b),
+  // O of tile t behind them
+  constexpr int kO = 2 * kBuffers * kStep;
 
   if (warp >= 8) {
-    setmaxnreg_dec<120>();
+    setmaxnreg_dec<P::kBlocks == 1 ? 120 : 48>();
     if (warp == 10 && elect_one()) {
       // ------------------------------------------------ TMA loads
       int issued = min(slots, kStages), slot = 0;
@@ -317,7 +302,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const uint64_t q_desc = make_smem_desc(smem_u32(q_tile + t * P::kQ), 16, 1024, 2);
       const uint64_t k_desc = make_smem_desc(smem_u32(ring), 16, 1024, 2);
       const uint64_t v_desc = make_smem_desc(smem_u32(ring), kStep * 128, 1024, 2);
-      const uint32_t s_tmem = tmem + 128 * t, o_tmem = tmem + 256 + DP * t;
+      const uint32_t s_tmem = tmem + kBuffers * kStep * t, o_tmem = tmem + kO + DP * t;
       int slot = 0;
       uint32_t phase = 0;
       auto advance = [&] {
@@ -334,7 +319,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       // Unrolled: an MMA takes 33 to 65 cycles, a loop around it up to 86.
       auto scores = [&](int s, uint32_t k_offset) {  // S of step s = Q K^T
         const uint64_t kd = k_desc + (k_offset >> 4);
-        const uint32_t d = s_tmem + 64 * (s & 1);
+        const uint32_t d = s_tmem + kStep * (s % kBuffers);
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k) {
           if (k < ksteps) {
@@ -347,7 +332,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       if (ok && steps > 0) {
         ok = mbar_wait(&kv_full[0], 0, abort_flag, kErrAttnKv, a.wait_limit_ns);
         if (ok) {
-          for (int s = 0; s < 2; ++s) {
+          for (int s = 0; s < kBuffers; ++s) {
             if (s < n) scores(s, s * P::kKv);
             if (n > 0) tc_commit(&s_full[2 * t + s]);
           }
@@ -360,21 +345,21 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
                  ? mbar_wait(fixed, 0, abort_flag, kErrAttnFix, a.wait_limit_ns)
                  : mbar_wait(&kv_full[slot], phase, abort_flag, kErrAttnKv, a.wait_limit_ns);
         if (ok && s < n) {
-          ok = mbar_wait(&p_full[2 * t + (s & 1)], (s >> 1) & 1, abort_flag, kErrAttnP,
+          ok = mbar_wait(&p_full[2 * t + s % kBuffers], (s / kBuffers) & 1, abort_flag, kErrAttnP,
                          a.wait_limit_ns);
         }
         if (!ok) break;
         if (s < n) {
           tc_fence_after();
           const uint64_t vd = v_desc + ((slot * P::kSlot) >> 4);
-          const uint32_t p = s_tmem + 64 * (s & 1);
+          const uint32_t p = s_tmem + kStep * (s % kBuffers);
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k) {
             mma_f16_ta(o_tmem, p + 8 * k, vd + ((k * 2048) >> 4), idesc_o, s > 0 || k > 0);
           }
-          if (s + 2 < n) scores(s + 2, slot * P::kSlot + P::kKv);
-          // S of step s + 2 is there, or (behind the last) just O += P V of step s
-          tc_commit(&s_full[2 * t + (s & 1)]);
+          if (s + kBuffers < n) scores(s + kBuffers, slot * P::kSlot + P::kKv);
+          // S of that step is there, or (behind the last) just O += P V of step s
+          tc_commit(&s_full[2 * t + s % kBuffers]);
         }
         release(slot, s < n);
         advance();
@@ -398,12 +383,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     }
   } else {
     // ------------------------------------------------ rows
-    setmaxnreg_inc<192>();
+    setmaxnreg_inc<P::kBlocks == 1 ? 192 : 96>();
     const int t = warp >> 2;
     const int r = threadIdx.x & 127;
     const int row = row_t[t] + r % a.tile_rows, h = head_t[t] + r / a.tile_rows;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-    const uint32_t s_at = tmem + 128 * t + lanes, o_at = tmem + 256 + DP * t + lanes;
+    const uint32_t s_at = tmem + kBuffers * kStep * t + lanes, o_at = tmem + kO + DP * t + lanes;
     const bool valid = some_t[t] && r < a.tile_rows * a.tile_heads && row < seq.q1;
     const int seen = valid ? seq.seen(row, a.causal) : 0;
     // what every row of this tile sees, and the first row's place
@@ -435,13 +420,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     const int n = steps_t[t];
 #pragma unroll 1
     for (int s = 0; s < n; ++s) {
-      if (!wait_ready(&s_full[2 * t + (s & 1)], (s >> 1) & 1, abort_flag, kErrAttnS,
+      if (!wait_ready(&s_full[2 * t + s % kBuffers], (s / kBuffers) & 1, abort_flag, kErrAttnS,
                       a.wait_limit_ns)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      const uint32_t s_now = s_at + 64 * (s & 1);
+      const uint32_t s_now = s_at + kStep * (s % kBuffers);
       const int key0 = (begin + s) * kStep;
       float x[kStep];
       {
@@ -519,9 +504,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       }
       if (s > 0 && __any_sync(0xFFFFFFFFu, moved)) {
         l *= factor;
-        // the next step's S comes after O += P V of the step before this one
-        if (!wait_ready(&s_full[2 * t + ((s + 1) & 1)], ((s + 1) >> 1) & 1, abort_flag, kErrAttnO,
-                        a.wait_limit_ns)) {
+        // O += P V of the step before this one comes before S of this step (one
+        // buffer) or of the next
+        if (kBuffers == 2 && !wait_ready(&s_full[2 * t + ((s + 1) & 1)], ((s + 1) >> 1) & 1,
+                                         abort_flag, kErrAttnO, a.wait_limit_ns)) {
           ok = false;
           break;
         }
@@ -544,31 +530,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       for (int e = 0; e < 32; ++e) {
         uint64_t y = pair_of(x[2 * e], x[2 * e + 1]);
         y = kScaled ? add2(y, base2) : fma2(y, to2, base2);
-        if (e % kPolyEvery == kPolyEvery - 1) {
-          y = exp2_pair(y);
-        } else {
-          float y0, y1;
-          unpair(y, &y0, &y1);
-          y = pair_of(ex2(y0), ex2(y1));
-        }
-        sum[e & 1] = add2(sum[e & 1], y);
         float p0, p1;
         unpair(y, &p0, &p1);
+        p0 = ex2(p0);
+        p1 = ex2(p1);
+        sum[e & 1] = add2(sum[e & 1], pair_of(p0, p1));
         p[e] = pack_pair<T>(p0, p1);
       }
       tmem_st_32x32b_x32(s_now, p);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[2 * t + (s & 1)]);
+      if (lane == 0) mbar_arrive(&p_full[2 * t + s % kBuffers]);
       float s0, s1;
       unpair(add2(sum[0], sum[1]), &s0, &s1);
       l += s0 + s1;
     }
     if (n > 0 && ok) {
       // what follows the last step's O += P V
-      ok = wait_ready(&s_full[2 * t + ((n + 1) & 1)], ((n + 1) >> 1) & 1, abort_flag, kErrAttnO,
-                      a.wait_limit_ns);
+      const int behind = n + kBuffers - 1;
+      ok = wait_ready(&s_full[2 * t + behind % kBuffers], (behind / kBuffers) & 1, abort_flag,
+                      kErrAttnO, a.wait_limit_ns);
     }
     tc_fence_after();
     if (ok) {
@@ -689,7 +671,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   }
   if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, P::kColumns);
   }
 }
 
