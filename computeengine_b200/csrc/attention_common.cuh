@@ -67,6 +67,13 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// 1 / x for 1 <= x, 0 for infinity.
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
@@ -123,6 +130,7 @@ __global__ void __launch_bounds__(128) attention_join_kernel(const AttentionArgs
   const int i = static_cast<int>(at % a.q_len);
   const int h = static_cast<int>(at / a.q_len % a.q_heads);
   const int64_t b = at / a.q_len / a.q_heads;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // until the shares are written
   float top = -INFINITY;
   for (int s = threadIdx.x; s < splits; s += 128) {
     weight[s] = part_lse[s * rows + at];

@@ -18,7 +18,7 @@
 namespace ie_cuda {
 
 constexpr int kStepThreads = 128;
-constexpr int kStepStages = 3;
+constexpr int kStepStages = 2;  // three blocks per SM; 3 stages and two blocks: 2% slower
 constexpr int kStepKeys = 16;
 
 struct StepArgs : AttentionArgs {
@@ -125,11 +125,24 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
   const bool my_data = my_chunk * 8 < a.head_dim;
   const uint16_t* k_next = k + (my_data ? my_chunk * 8 : 0) + (first + my_row) * a.k_stride[1];
   const uint16_t* v_next = v + (my_data ? my_chunk * 8 : 0) + (first + my_row) * a.v_stride[1];
+  const int64_t k_rows = kRows * a.k_stride[1], v_rows = kRows * a.v_stride[1];
+  const bool whole = a.head_dim == DP;  // every chunk of a row holds data
   int key_next = first;
   auto fetch = [&](int stage) {
     const uint32_t at = ring_at + stage * P::kStage;
-    if constexpr (VEC) {
+    if (VEC && whole && key_next + kStepKeys <= to) {
+      const uint16_t* kp = k_next;
+      const uint16_t* vp = v_next;
 #pragma unroll
+      for (int i = 0; i < kCopies; ++i, kp += k_rows, vp += v_rows) {
+        const uint32_t s = at + step_at<DP>(my_row + i * kRows, my_chunk);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s), "l"(kp) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s + kStepKeys * P::kRow),
+                     "l"(vp)
+                     : "memory");
+      }
+    } else if constexpr (VEC) {
+#pragma unroll 1
       for (int i = 0; i < kCopies; ++i) {
         const int r = my_row + i * kRows;
         const bool in = key_next + r < to && my_data;
@@ -143,8 +156,6 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
                      "l"(vp), "r"(bytes)
                      : "memory");
       }
-      k_next += kStride * a.k_stride[1];
-      v_next += kStride * a.v_stride[1];
     } else {
       uint8_t* p = ring + stage * P::kStage;
       for (int e = lane; e < kStepKeys * DP; e += 32) {
@@ -158,6 +169,8 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
       __syncwarp();
     }
     key_next += kStride;
+    k_next += kStride * a.k_stride[1];
+    v_next += kStride * a.v_stride[1];
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
 #pragma unroll
@@ -251,7 +264,7 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
         for (int half = 0; half < 2; ++half) {
           float x = s[n][2 * half + i];
           if (cap) {
-            x = cap_out - __fdividef(2.0f * cap_out, 1.0f + ex2(x * cap_in));
+            x = fmaf(-2.0f * cap_out, reciprocal(1.0f + ex2(x * cap_in)), cap_out);
           } else {
             x *= scale;
           }
