@@ -497,7 +497,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
       // The maximum in use moves only when it grew by more than 2^8: until then
       // the weights stay below 256, which both 16-bit types hold as well as 1.
       float factor = 1.0f;
-      const bool moved = !((top - m) * to_log2 <= 8.0f) && top != -INFINITY;
+      // (Rows that do not exist hold anything and must not ask for it.)
+      const bool moved = valid && !((top - m) * to_log2 <= 8.0f) && top != -INFINITY;
       if (moved) {
         factor = m == -INFINITY ? 1.0f : ex2((m - top) * to_log2);
         m = top;

@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const G
   // more columns than threads: the range is one group
   for (int at = col; row < rows && row < count && at < all; at += cols) {
     const int c = r.c0 + at * V;
-    constexpr int K = XT == IE_DT_BF16X2 ? 1 : 2;  // batches in flight
+    constexpr int K = XT == IE_DT_BF16X2 ? 2 : 4;  // batches in flight
     const int64_t step = static_cast<int64_t>(rows) * channel_at<XT>(1, a.c_store, 0);
     int64_t from_x = channel_at<XT>(p0 + row, a.c_store, c);
     int left = (count - row + rows - 1) / rows;  // pixels of this thread
@@ -562,6 +562,8 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const G
       run.add(item_pairs<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store)));
     }
   }
+  // the second kernel may be launched; it waits for this one's end
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // the block's mean of each group, then each channel's squares about it
   const int group_channels = all > cols ? cols * V : r.group_channels;
   Pairs<V> sum = run.mean;
@@ -636,6 +638,7 @@ __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 :
   const int range = static_cast<int>(unit - image * a.ranges);
   const Range r(a, range);
   const int lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // until the statistics are written
   for (int g = threadIdx.x >> 5; g < a.range_groups; g += kGnThreads / 32) {
     const float2* p = a.partial + (static_cast<int64_t>(unit) * a.range_groups + g) * a.parts;
     // up to 64 parts stay in registers between the mean and the squares

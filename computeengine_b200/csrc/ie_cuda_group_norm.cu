@@ -220,8 +220,21 @@ int launch_two(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream
   const int64_t units = images * p.ranges;
   if (rc == IE_OK) rc = launch_clusters(stats, units * p.blocks, p.joined, p.smem, s, a);
   if (rc != IE_OK) return rc;
-  apply<<<static_cast<unsigned>(units * p.apply_blocks), kGnThreads, apply_smem, s>>>(
-      a, p.apply_blocks);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * p.apply_blocks));
+  cfg.blockDim = dim3(kGnThreads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(apply_smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};  // its launch overlaps the end of the statistics kernel
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, apply, a, p.apply_blocks);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(IE_RUNTIME, "group_norm: %s", cudaGetErrorString(e));
+  }
   return check_launch("group_norm");
 }
 

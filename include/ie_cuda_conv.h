@@ -564,8 +564,10 @@ typedef struct ie_attention_desc {
  *   slopes       [q_heads] fp32
  * A query that sees no key gets o = 0 and lse = -inf.  Rows of o and lse that
  * belong to no document are left as they were.  Keys and values behind a
- * sequence's length may hold anything.  Values outside the ranges above are
- * clamped to them. */
+ * sequence's length, and other sequences', may hold anything.  A NaN or
+ * infinite value of v inside a sequence may also reach queries of that sequence
+ * that causal hides it from (a masked weight is 0, and 0 * NaN is NaN).
+ * Values outside the ranges above are clamped to them. */
 typedef struct ie_attention_mask {
   int32_t causal;
   int32_t documents;
@@ -578,8 +580,12 @@ typedef struct ie_attention_mask {
 
 /* mask may be NULL (every key visible).  lse: fp32 [batch, q_heads, q_len] or
  * NULL.  workspace must hold ie_cuda_attention_workspace_bytes(desc, mask)
- * bytes (256-byte aligned, 0 for prompts, then it may be NULL); its contents need not be
- * kept, calls that overlap on the GPU need one each. */
+ * bytes (256-byte aligned; 0 where the rows alone fill the GPU, then it may be
+ * NULL): few queries over many keys are computed in shares, whose number
+ * depends on the batch, and joined.  Its contents need not be kept; calls that
+ * overlap on the GPU need one each.
+ * Full speed: q, k and v 16-byte aligned, head_dim a multiple of 8, strides
+ * multiples of 8 and not 0; other tensors take a slower kernel. */
 size_t ie_cuda_attention_workspace_bytes(const ie_attention_desc* desc,
                                          const ie_attention_mask* mask);
 int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* mask, const void* q,
