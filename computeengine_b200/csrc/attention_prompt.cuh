@@ -269,6 +269,17 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
       }
     }
   }
+  if (a.packed && warp < 8) {
+    // rows of Q that no head fills: zeros, or what another block left there could
+    // be NaN, for which a row would look for a new maximum at every step
+    const int rows = a.tile_rows * a.tile_heads;
+    for (int i = rows * 8 + static_cast<int>(threadIdx.x); i < 128 * 8; i += 256) {
+      for (int c = 0; c < 2 * P::kCols; ++c) {
+        *reinterpret_cast<uint4*>(q_tile + c * 16384 + i * 16) = make_uint4(0, 0, 0, 0);
+      }
+    }
+    fence_proxy_async_smem();
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -497,8 +508,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
       // The maximum in use moves only when it grew by more than 2^8: until then
       // the weights stay below 256, which both 16-bit types hold as well as 1.
       float factor = 1.0f;
-      // (Rows that do not exist hold anything and must not ask for it.)
-      const bool moved = valid && !((top - m) * to_log2 <= 8.0f) && top != -INFINITY;
+      const bool moved = !((top - m) * to_log2 <= 8.0f) && top != -INFINITY;
       if (moved) {
         factor = m == -INFINITY ? 1.0f : ex2((m - top) * to_log2);
         m = top;
