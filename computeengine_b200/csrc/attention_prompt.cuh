@@ -20,9 +20,11 @@
 // of them changed nothing (113 to 121 us against 113 to 118 us for 4096 tokens,
 // 16 heads of 64).
 // Warps 0-3 and 4-7 hold the rows of the tiles, warps 8 and 9 issue their MMAs
-// (one thread for both tiles spent 2200 cycles a step on the waits between
-// them), warp 10 the TMA loads of Q, K and V, warp 11 clears the rows of V
+// (one thread for both tiles took about 2200 cycles a step, 1200 of them between
+// its waits and the MMAs), warp 10 the TMA loads of Q, K and V, warp 11 clears the rows of V
 // behind the sequence's end (0 * NaN would reach O).
+// 4096 tokens, 16 heads of 128, no mask: 126 us, 1090 TFLOP/s; of 64: 126 us,
+// 543 TFLOP/s.
 #pragma once
 
 #include "attention_common.cuh"
@@ -67,8 +69,8 @@ struct PromptPlan {
 
 // True in one thread of the (converged) warp.  The compiler then knows that
 // one thread runs what follows: with `lane == 0` it walks the warp's active
-// threads around every MMA, which took 86 cycles an MMA instead of the 64 that
-// the tensor core needs for it.
+// threads around every MMA, which took 81 to 87 cycles an MMA instead of the 65 that
+// it takes then (128 x 128 x 16).
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes = 0;
   asm volatile(

