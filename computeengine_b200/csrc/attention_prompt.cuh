@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     // scores up to here go through the polynomial
     const float cap_limit = CAP ? kTanhLimit / fabsf(cap_arg) : 0.0f;
     const float slope = BIAS && valid && a.slopes != nullptr ? a.slopes[h] * kLog2e : 0.0f;
-    const float place = static_cast<float>(valid ? seq.place(row) : 0);
+    const int place = valid ? seq.place(row) : 0;
     // x is the score in units of log2 e (plain: before the scale)
     constexpr bool kScaled = CAP || BIAS;
     const float to_log2 = kScaled ? 1.0f : scale;
@@ -475,7 +475,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
         }
       }
       if constexpr (BIAS) {
-        const float from = place - static_cast<float>(key0);
+        // subtracted as integers: fp32 does not hold every place behind 2^24
+        const float from = static_cast<float>(place - key0);
         const float factor = CAP ? 1.0f : scale;
         if (all_past >= key0 + kStep - 1) {  // no key lies ahead of its row
           const uint64_t f2 = pair_of(factor, factor), s2 = pair_of(slope, slope);

@@ -207,8 +207,8 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
   const float cap_in = cap ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
   const float cap_out = a.softcap * kLog2e;
   const bool bias = a.slopes != nullptr;
-  float slope[NT][2], place[NT][2];
-  int seen[NT][2];
+  float slope[NT][2];
+  int place[NT][2], seen[NT][2];
   float o[NT][DP / 16][4], top[NT][2], sum[NT][2];
 #pragma unroll
   for (int n = 0; n < NT; ++n) {
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
       const int pos = row0 + r % a.tile_rows;
       const bool valid = r < rows && pos < seq.q1;
       seen[n][i] = valid ? min(to, seq.seen(pos, a.causal)) : 0;
-      place[n][i] = valid ? static_cast<float>(seq.place(pos)) : 0.0f;
+      place[n][i] = valid ? seq.place(pos) : 0;
       slope[n][i] = valid && bias ? a.slopes[h0 + r / a.tile_rows] * kLog2e : 0.0f;
       top[n][i] = -INFINITY;
       sum[n][i] = 0.0f;
@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
             x *= scale;
           }
           const int j = j0 + 8 * half;
-          if (bias) x -= slope[n][i] * fabsf(place[n][i] - static_cast<float>(j));
+          // subtracted as integers: fp32 does not hold every place behind 2^24
+          if (bias) x -= slope[n][i] * fabsf(static_cast<float>(place[n][i] - j));
           s[n][2 * half + i] = j < seen[n][i] ? x : -INFINITY;
         }
         t[i] = max_nan(top[n][i], max_nan(s[n][i], s[n][2 + i]));

@@ -377,3 +377,64 @@ def test_operator():
         o = [None]
         st = op.forward(bad, o)
         assert not st and st.code == code and o == [None], bad
+
+
+@pytest.mark.parametrize("q_len", [1, 17])
+def test_bias_of_near_keys_behind_2_24(q_len):
+    """The distance bias of keys next to their query, at places that fp32 does
+    not hold: the last 2048 keys stand for all of them, as a key further away has
+    at most e^(60 - 2047) of the weight of the nearest, which is zero.
+
+    Tolerance of lse: distances below 2048 are exact and the products and
+    exponentials of single scores are off by steps of scores below 2^7 for what
+    weighs anything, 2^-16; scores of the running maximum alike."""
+    import torch
+    from computeengine_b200 import _lib as L
+    n, d, tail = (1 << 24) + 1029, 8, 2048
+    g = torch.Generator(device="cuda").manual_seed(5)
+    k = torch.randn(1, n, 1, d, generator=g, device="cuda").bfloat16()
+    q = torch.randn(1, q_len, 1, d, generator=g, device="cuda").bfloat16()
+    slopes = torch.tensor([1.0], device="cuda")
+    o = torch.empty_like(q)
+    lse = torch.empty(1, 1, q_len, device="cuda")
+    desc = attention_desc(L, q, k, k, o, d ** -0.5)
+    run_attention(L, desc, attention_mask(L, slopes=slopes), q, k, k, o, lse)
+    near = k[:, n - tail:].double()[0, :, 0]
+    s = desc.scale * q.double()[0, :, 0] @ near.T
+    p = torch.arange(q_len, device="cuda") + tail - q_len
+    s = s - (p[:, None] - torch.arange(tail, device="cuda")[None]).abs().double()
+    want = torch.softmax(s, 1) @ near
+    assert (lse[0, 0].double() - torch.logsumexp(s, 1)).abs().max() < 2.0 ** -14
+    size = torch.softmax(s, 1) @ near.abs()
+    tol = HALF_STEP[torch.bfloat16] * (want.abs() + size) + 2.0 ** -12 * size
+    assert ((o[0, :, 0].double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_offsets_past_32_bits(q_len):
+    """A batch row, and a token, more than 2^32 bytes and 2^31 elements away."""
+    import torch
+    from computeengine_b200 import _lib as L
+    d, n, far = 64, 300, (1 << 31) + 4096
+    store = torch.empty(far + 2 * n * d, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(7)
+    near = torch.randn(2, n, 1, d, generator=g, device="cuda").bfloat16()
+    k = store.as_strided((2, n, 1, d), (far, d, d, 1))
+    k.copy_(near)
+    q = torch.randn(2, q_len, 1, d, generator=g, device="cuda").bfloat16()
+    out = []
+    for kk in (k, near):
+        o = torch.empty_like(q)
+        m = attention_mask(L, causal=1)
+        run_attention(L, attention_desc(L, q, kk, kk, o, 0.125), m, q, kk, kk, o)
+        out.append(o)
+    assert torch.equal(*out)
+    stride = (1 << 23) + 64
+    k = store.as_strided((1, 257, 1, d), (stride, stride, d, 1))
+    k.copy_(near[:1, :257])
+    q, out = q[:1], []
+    for kk in (k, near[:1, :257]):
+        o = torch.empty_like(q)
+        run_attention(L, attention_desc(L, q, kk, kk, o, 0.125), None, q, kk, kk, o)
+        out.append(o)
+    assert torch.equal(*out)
