@@ -48,6 +48,13 @@ constexpr int kGnCluster = 4;  // blocks of the statistics kernel joined before 
 // Kinds of activation: a clamp to [low, high] (none, ReLU, ReLU6), SiLU, GELU.
 enum { kActClamp = 0, kActSilu = 1, kActGelu = 2 };
 
+// 1 / x for 1 <= x, 0 from 2^126 on.
+__device__ __forceinline__ float reciprocal(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 template <int ACT, int V>
 __device__ __forceinline__ void activate(float (&v)[V], float low, float high) {
   if constexpr (ACT == kActClamp) {
@@ -60,23 +67,31 @@ __device__ __forceinline__ void activate(float (&v)[V], float low, float high) {
     // v / (1 + 2^(-v log2 e)) on the special function unit, within a few steps
     // of fp32.  It takes 16 results a cycle and SM, which exponential and
     // reciprocal for each value would make the bound; so two values share the
-    // reciprocal of their denominators' product (held below overflow: from
-    // 2^60 on v / 2^60 is below every type's last place).
+    // reciprocal of their denominators' product, where that has a normal one.
+    // Where it has not, each takes its own: a NaN stays in its channel, and far
+    // below zero v / infinity is 0.
+    constexpr float kNormal = 0x1p126f;
     float d[V];
+    bool shared = true;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-      float x = v[e] * -1.4426950408889634f;
-      asm("min.NaN.f32 %0, %1, %2;" : "=f"(x) : "f"(x), "f"(60.0f));
-      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(x));
+      float x;
+      asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(v[e] * -1.4426950408889634f));
       d[e] = 1.0f + x;
+      if (e % 2 == 1) shared = shared && d[e - 1] * d[e] <= kNormal;
     }
+    if (V % 2 == 1) shared = shared && d[V - 1] <= kNormal;
+    if (shared) {
 #pragma unroll
-    for (int e = 0; e < V; e += 2) {
-      const float other = e + 1 < V ? d[e + 1] : 1.0f;
-      float r;
-      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d[e] * other));
-      v[e] *= r * other;
-      if (e + 1 < V) v[e + 1] *= r * d[e];
+      for (int e = 0; e < V; e += 2) {
+        const float other = e + 1 < V ? d[e + 1] : 1.0f;
+        const float r = reciprocal(d[e] * other);
+        v[e] *= r * other;
+        if (e + 1 < V) v[e + 1] *= r * d[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] *= reciprocal(d[e]);
     }
   } else {
 #pragma unroll
@@ -382,8 +397,8 @@ __device__ __forceinline__ void channel_affine(const GroupNormArgs& a, int c, in
   add_pairs->set(add);
 }
 
-// Normalizes, activates and stores one item; channels past c become zero
-// (mul and add are zero there, but x may hold anything).
+// Normalizes, activates and stores one item; channels past c are zero before
+// the activation already (mul and add are zero there, but x may hold anything).
 template <int YT, int V, int ACT>
 __device__ __forceinline__ void finish_item(const GroupNormArgs& a, const Pairs<V>& x,
                                             const Pairs<V>& mul, const Pairs<V>& add, uint8_t* y,
@@ -395,11 +410,11 @@ __device__ __forceinline__ void finish_item(const GroupNormArgs& a, const Pairs<
     f[2 * i] = r.x;
     if (2 * i + 1 < V) f[2 * i + 1] = r.y;
   }
-  activate<ACT, V>(f, a.low, a.high);
   if (valid < V) {
 #pragma unroll
     for (int e = 0; e < V; ++e) f[e] = e < valid ? f[e] : 0.0f;
   }
+  activate<ACT, V>(f, a.low, a.high);
   store_item<YT, V>(y, 0, a.c_store, f);
 }
 
