@@ -74,6 +74,33 @@ __device__ __forceinline__ float reciprocal(float x) {
   return y;
 }
 
+// ---- cap * tanh(s / cap), in units of log2 e.  With u = s / cap:
+//   |u| <= kTanhLimit   s * (tanh(u) / u), the ratio a polynomial in u^2 (minimax
+//                       of tanh u with slope 1 at 0, absolute error below 2.7e-7)
+//   beyond              cap * (1 - 2 / (1 + exp(2 u)))
+// Either is off by a few 2^-22 of the result, whatever the cap: the second form
+// alone is off by that of the cap, 0.1 for scores of 1 under a cap of 10^6.
+// Up to kSmallCap the second form's error, 2^-17 then, is far below that of the
+// 16-bit weights, and the prompt kernel takes it for all scores of a warp when one is
+// beyond kTanhLimit: 284 us against 303 us with both forms (4096 tokens, 16 heads
+// of 128, a cap of 2 and nearly all scores beyond it).
+constexpr float kTanhLimit = 0.75f;
+constexpr float kSmallCap = 64.0f;
+constexpr float kTanh1 = -0.33328044414520264f, kTanh2 = 0.13253363966941833f,
+                kTanh3 = -0.04986608773469925f, kTanh4 = 0.012750583700835705f;
+
+// u per unit of q.k.  Held below overflow: a cap that small leaves no score.
+__device__ __forceinline__ float cap_argument(const AttentionArgs& a) {
+  return fminf(fmaxf(a.scale / a.softcap, -1e30f), 1e30f);
+}
+
+__device__ __forceinline__ float tanh_ratio(float uu) {
+  float p = fmaf(uu, kTanh4, kTanh3);
+  p = fmaf(p, uu, kTanh2);
+  p = fmaf(p, uu, kTanh1);
+  return fmaf(p, uu, 1.0f);
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));

@@ -144,14 +144,10 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   return y;
 }
 
-// tanh(u) / u for |u| <= kTanhLimit as a polynomial in u^2 (minimax of tanh u
-// with slope 1 at 0, absolute error below 2.7e-7).
-constexpr float kTanhLimit = 0.75f;
-__device__ __forceinline__ uint64_t tanh_ratio(uint64_t uu) {
-  uint64_t p = fma2(uu, pair_of(0.012750583700835705f, 0.012750583700835705f),
-                    pair_of(-0.04986608773469925f, -0.04986608773469925f));
-  p = fma2(p, uu, pair_of(0.13253363966941833f, 0.13253363966941833f));
-  p = fma2(p, uu, pair_of(-0.33328044414520264f, -0.33328044414520264f));
+__device__ __forceinline__ uint64_t tanh_ratio2(uint64_t uu) {
+  uint64_t p = fma2(uu, pair_of(kTanh4, kTanh4), pair_of(kTanh3, kTanh3));
+  p = fma2(p, uu, pair_of(kTanh2, kTanh2));
+  p = fma2(p, uu, pair_of(kTanh1, kTanh1));
   return fma2(p, uu, pair_of(1.0f, 1.0f));
 }
 
@@ -409,7 +405,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     const int all_past = some_t[t] ? seq.place(row_t[t]) : 0;
     constexpr float kLog2e = 1.4426950408889634f;
     const float scale = a.scale * kLog2e;
-    const float cap_arg = CAP ? a.scale / a.softcap : 0.0f;
+    const float cap_arg = CAP ? cap_argument(a) : 0.0f;
     const float cap_out = CAP ? a.softcap * kLog2e : 0.0f;
     // scores up to here go through the polynomial
     const float cap_limit = CAP ? kTanhLimit / fabsf(cap_arg) : 0.0f;
@@ -418,14 +414,13 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     // x is the score in units of log2 e (plain: before the scale)
     constexpr bool kScaled = CAP || BIAS;
     const float to_log2 = kScaled ? 1.0f : scale;
-    // cap * tanh(s / cap) = cap * (1 - 2 / (1 + exp(2 s / cap)))
     auto capped = [&](float s) {
       const float u = ex2(s * (2.0f * kLog2e * cap_arg));
       return cap_out - __fdividef(2.0f * cap_out, 1.0f + u);
     };
     auto capped_pair = [&](uint64_t s) {
       const uint64_t u = mul2(s, pair_of(cap_arg, cap_arg));
-      return mul2(mul2(u, pair_of(cap_out, cap_out)), tanh_ratio(mul2(u, u)));
+      return mul2(mul2(s, pair_of(scale, scale)), tanh_ratio2(mul2(u, u)));
     };
 
     float m = -INFINITY, l = 0.0f;
@@ -461,7 +456,6 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
             lo[c] = min3(lo[c], x[e + 2 * c], x[e + 2 * c + 1]);
           }
         }
-        // NaN takes the exact way
         const bool small = max_nan(hi[0], hi[1]) <= cap_limit &&
                            min3(lo[0], lo[1], lo[1]) >= -cap_limit;
         if (__all_sync(0xFFFFFFFFu, small)) {
@@ -469,9 +463,19 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
           for (int e = 0; e < kStep; e += 2) {
             unpair(capped_pair(pair_of(x[e], x[e + 1])), &x[e], &x[e + 1]);
           }
-        } else {
+        } else if (a.softcap <= kSmallCap) {
 #pragma unroll
           for (int e = 0; e < kStep; ++e) x[e] = capped(x[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kStep; e += 2) {
+            float t[2];
+            unpair(capped_pair(pair_of(x[e], x[e + 1])), &t[0], &t[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              x[e + k] = fabsf(x[e + k]) <= cap_limit ? t[k] : capped(x[e + k]);
+            }
+          }
         }
       }
       if constexpr (BIAS) {

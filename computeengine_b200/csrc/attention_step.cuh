@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
   constexpr float kLog2e = 1.4426950408889634f;
   const float scale = a.scale * kLog2e;
   const bool cap = a.softcap > 0.0f;
-  const float cap_in = cap ? 2.0f * kLog2e * a.scale / a.softcap : 0.0f;
+  const float cap_arg = cap ? cap_argument(a) : 0.0f;
   const float cap_out = a.softcap * kLog2e;
   const bool bias = a.slopes != nullptr;
   float slope[NT][2];
@@ -259,17 +259,33 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
     const int j0 = key + lane / 4;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+      if (cap) {
+        float u[4];
+        bool small = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          u[e] = s[n][e] * cap_arg;
+          small = small && fabsf(u[e]) <= kTanhLimit;
+          s[n][e] *= scale * tanh_ratio(u[e] * u[e]);
+        }
+        if (__any_sync(0xFFFFFFFFu, !small)) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float far = fmaf(-2.0f * cap_out, reciprocal(1.0f + ex2(u[e] * (2.0f * kLog2e))),
+                                   cap_out);
+            s[n][e] = fabsf(u[e]) <= kTanhLimit ? s[n][e] : far;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] *= scale;
+      }
       float t[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           float x = s[n][2 * half + i];
-          if (cap) {
-            x = fmaf(-2.0f * cap_out, reciprocal(1.0f + ex2(x * cap_in)), cap_out);
-          } else {
-            x *= scale;
-          }
           const int j = j0 + 8 * half;
           // subtracted as integers: fp32 does not hold every place behind 2^24
           if (bias) x -= slope[n][i] * fabsf(static_cast<float>(place[n][i] - j));
