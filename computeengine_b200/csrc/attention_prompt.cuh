@@ -21,8 +21,9 @@
 // 16 heads of 64).
 // Warps 0-3 and 4-7 hold the rows of the tiles, warps 8 and 9 issue their MMAs
 // (one thread for both tiles took about 2200 cycles a step, 1200 of them between
-// its waits and the MMAs), warp 10 the TMA loads of Q, K and V, warp 11 clears the rows of V
-// behind the sequence's end (0 * NaN would reach O).
+// its waits and the MMAs), warp 10 the TMA loads of Q, K and V; it also
+// clears the rows of V behind the sequence's end (0 * NaN would reach O).  Warp 11
+// is idle: it completes the warpgroup that gives its registers away.
 // 4096 tokens, 16 heads of 128, no mask: 126 us, 1090 TFLOP/s; of 64: 126 us,
 // 543 TFLOP/s.
 #pragma once
@@ -207,12 +208,11 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
   uint64_t* q_full = bars;                 // [2]
   uint64_t* s_full = bars + 2;             // [2][buffers]
   uint64_t* p_full = bars + 6;             // [2][buffers]
-  uint64_t* short_full = bars + 10;        // the last V, when it is cut short
-  uint64_t* fixed = bars + 11;             // and its rows behind the end are cleared
-  uint64_t* drain = bars + 12;             // [2]
-  uint64_t* kv_full = bars + 14;           // [kStages]
-  uint64_t* kv_empty = bars + 14 + kStages;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14 + 2 * kStages);
+  uint64_t* fixed = bars + 10;             // the last V's rows behind the end are cleared
+  uint64_t* drain = bars + 11;             // [2]
+  uint64_t* kv_full = bars + 13;           // [kStages]
+  uint64_t* kv_empty = bars + 13 + kStages;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13 + 2 * kStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* loads_issued = const_cast<int*>(abort_flag) + 1;
 
@@ -222,8 +222,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
   // first kBuffers steps, then V of a step and K of the step kBuffers ahead.
   const int slots = steps > 0 ? steps + 1 : 0;
   auto load_slot = [&](int i, int slot) {
-    // a barrier of its own lets warp 11 wait for the last load from the start
-    uint64_t* full = last_short && i == slots - 1 ? short_full : &kv_full[slot];
+    uint64_t* full = &kv_full[slot];
     const int first = i == 0 ? 0 : i - 1;  // steps of the two halves
     const int second = i == 0 && kBuffers == 1 ? steps : i + kBuffers - 1;
     mbar_arrive_expect_tx(full, second < steps ? 2 * P::kKv : P::kKv);
@@ -241,11 +240,11 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     tmem_alloc(tmem_slot, P::kColumns);
     tmem_relinquish();
   } else if (warp == 10) {
-    // barriers 0 .. 13 + 2 kStages in their order above, one per lane
-    for (int i = lane; i < 14 + 2 * kStages; i += 32) {
+    // barriers 0 .. 12 + 2 kStages in their order above, one per lane
+    for (int i = lane; i < 13 + 2 * kStages; i += 32) {
       mbar_init(&bars[i], i >= 6 && i < 10 ? 4           // p_full: a lane of each warp
-                          : i == 11        ? 32          // fixed
-                          : i >= 14 + kStages ? 2        // kv_empty: both MMA warps
+                          : i == 10        ? 32          // fixed
+                          : i >= 13 + kStages ? 2        // kv_empty: both MMA warps
                                               : 1);
     }
     if (lane == 0) {
@@ -288,20 +287,39 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
 
   if (warp >= 8) {
     setmaxnreg_dec<P::kBlocks == 1 ? 120 : 48>();
-    if (warp == 10 && elect_one()) {
+    if (warp == 10) {
       // ------------------------------------------------ TMA loads
-      int issued = min(slots, kStages), slot = 0;
-      uint32_t phase = 0;
-      for (int i = kStages; i < slots; ++i) {
-        if (!mbar_wait(&kv_empty[slot], phase, abort_flag, kErrAttnEmpty, a.wait_limit_ns)) break;
-        load_slot(i, slot);
-        issued = i + 1;
-        if (++slot == kStages) {
-          slot = 0;
-          phase ^= 1u;
+      if (elect_one()) {
+        int issued = min(slots, kStages), slot = 0;
+        uint32_t phase = 0;
+        for (int i = kStages; i < slots; ++i) {
+          if (!mbar_wait(&kv_empty[slot], phase, abort_flag, kErrAttnEmpty, a.wait_limit_ns)) break;
+          load_slot(i, slot);
+          issued = i + 1;
+          if (++slot == kStages) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+        *loads_issued = issued;
+      }
+      __syncwarp();
+      // Rows of the last V behind the end, when all loads are issued: a wait from
+      // the start would have the whole block's time for its limit.
+      if (last_short && steps > 0) {
+        const int last = (slots - 1) % kStages;
+        if (mbar_wait_warp(&kv_full[last], ((slots - 1) / kStages) & 1, abort_flag, kErrAttnKv,
+                           a.wait_limit_ns)) {
+          uint8_t* v = ring + last * P::kSlot;
+          const int from = length % kStep, pieces = (kStep - from) * 8;
+          for (int e = lane; e < pieces * P::kCols; e += 32) {
+            *reinterpret_cast<uint4*>(v + e / pieces * (kStep * 128) + from * 128 +
+                                      e % pieces * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          mbar_arrive(fixed);
         }
       }
-      *loads_issued = issued;
     } else if (warp < 10 && elect_one()) {
       // ------------------------------------------------ MMAs of tile t
       const int t = warp - 8, n = steps_t[t];
@@ -377,18 +395,6 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
       tc_commit(&drain[t]);
       int dummy_abort = 0;
       mbar_wait(&drain[t], 0, &dummy_abort, kErrAttnO, a.wait_limit_ns);
-    } else if (warp == 11 && last_short && steps > 0) {
-      // ------------------------------------------------ rows of V behind the end
-      if (mbar_wait_warp(short_full, 0, abort_flag, kErrAttnKv, a.wait_limit_ns)) {
-        uint8_t* v = ring + (slots - 1) % kStages * P::kSlot;  // the last load
-        const int from = length % kStep, pieces = (kStep - from) * 8;
-        for (int e = lane; e < pieces * P::kCols; e += 32) {
-          *reinterpret_cast<uint4*>(v + e / pieces * (kStep * 128) + from * 128 +
-                                    e % pieces * 16) = make_uint4(0, 0, 0, 0);
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(fixed);
-      }
     }
   } else {
     // ------------------------------------------------ rows
@@ -682,9 +688,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     }
     const int issued = *loads_issued;
     for (int i = max(0, issued - kStages); i < issued; ++i) {
-      const bool cut = last_short && i == slots - 1;
-      mbar_wait(cut ? short_full : &kv_full[i % kStages], cut ? 0 : (i / kStages) & 1,
-                &dummy_abort, kErrAttnKv, a.wait_limit_ns);
+      mbar_wait(&kv_full[i % kStages], (i / kStages) & 1, &dummy_abort, kErrAttnKv,
+                a.wait_limit_ns);
     }
   }
   if (warp == 8) {
