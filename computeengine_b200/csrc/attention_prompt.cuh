@@ -38,6 +38,11 @@ constexpr unsigned kErrAttnQ = 0x201, kErrAttnKv = 0x202, kErrAttnEmpty = 0x203,
 
 constexpr int kPromptThreads = 384;
 constexpr int kStep = 64;      // keys per step
+// The tensor core cuts off what lies below its fp32 sum's last place.  For keys
+// of equal weight that was 0.6% of o after 2^20 of them: so after this many steps
+// (2^15 keys, 0.02%) O is put away, added to what was put away before (in fp32,
+// rounded to nearest), and begins anew.
+constexpr int kFold = 512;
 
 struct PromptArgs : AttentionArgs {
   int tiles;           // blocks per (head unit, batch row), documents: upper bound in all
@@ -46,8 +51,9 @@ struct PromptArgs : AttentionArgs {
   int tile_rows;       // positions of a tile: 128, packed: q_len
   int tile_heads;      // heads of a tile: 1, packed: tile_rows * tile_heads <= 128
   int splits;          // shares of each sequence's keys
-  float* part_o;       // splits > 1: fp32 [splits][batch][q_heads][q_len][head_dim]
-  float* part_lse;     //             fp32 [splits][batch][q_heads][q_len]
+  // splits > 1, or more than kFold steps: fp32 [splits][batch][q_heads][q_len][head_dim]
+  float* part_o;
+  float* part_lse;     // splits > 1: fp32 [splits][batch][q_heads][q_len]
   int o_vec;           // rows of o can be written in 16-byte pieces
   uint64_t wait_limit_ns;
 };
@@ -382,7 +388,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
           const uint32_t p = s_tmem + kStep * (s % kBuffers);
 #pragma unroll
           for (int k = 0; k < kStep / 16; ++k) {
-            mma_f16_ta(o_tmem, p + 8 * k, vd + ((k * 2048) >> 4), idesc_o, s > 0 || k > 0);
+            mma_f16_ta(o_tmem, p + 8 * k, vd + ((k * 2048) >> 4), idesc_o,
+                       s % kFold > 0 || k > 0);
           }
           if (s + kBuffers < n) scores(s + kBuffers, slot * P::kSlot + P::kKv);
           // S of that step is there, or (behind the last) just O += P V of step s
@@ -432,143 +439,188 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     const int n = steps_t[t];
+    // the row among all rows, and among the shares' rows
+    auto lse_at = [&] {
+      return (static_cast<int64_t>(seq.batch) * a.q_heads + h) * a.q_len + row;
+    };
+    auto part_at = [&] {
+      return blockIdx.y * (static_cast<int64_t>(a.batch) * a.q_heads * a.q_len) + lse_at();
+    };
+    float m_kept = -INFINITY;  // the maximum in use when O was put away
+    auto kept_factor = [&] { return m_kept == m ? 1.0f : ex2((m_kept - m) * to_log2); };
 #pragma unroll 1
-    for (int s = 0; s < n; ++s) {
-      if (!wait_ready(&s_full[2 * t + s % kBuffers], (s / kBuffers) & 1, abort_flag, kErrAttnS,
-                      a.wait_limit_ns)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const uint32_t s_now = s_at + kStep * (s % kBuffers);
-      const int key0 = (begin + s) * kStep;
-      float x[kStep];
-      {
-        uint32_t sr[2][32];
-        tmem_ld_32x32b_x32(s_now, sr[0]);
-        tmem_ld_32x32b_x32(s_now + 32, sr[1]);
-        tmem_ld_wait(sr[0]);
-        tmem_ld_wait(sr[1]);
-#pragma unroll
-        for (int e = 0; e < kStep; ++e) x[e] = __uint_as_float(sr[e / 32][e % 32]);
-      }
-      if constexpr (CAP) {
-        float hi[2] = {x[0], x[0]}, lo[2] = {x[0], x[0]};
-#pragma unroll
-        for (int e = 0; e < kStep; e += 4) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            hi[c] = max3(hi[c], x[e + 2 * c], x[e + 2 * c + 1]);
-            lo[c] = min3(lo[c], x[e + 2 * c], x[e + 2 * c + 1]);
-          }
-        }
-        const bool small = max_nan(hi[0], hi[1]) <= cap_limit &&
-                           min3(lo[0], lo[1], lo[1]) >= -cap_limit;
-        if (__all_sync(0xFFFFFFFFu, small)) {
-#pragma unroll
-          for (int e = 0; e < kStep; e += 2) {
-            unpair(capped_pair(pair_of(x[e], x[e + 1])), &x[e], &x[e + 1]);
-          }
-        } else if (a.softcap <= kSmallCap) {
-#pragma unroll
-          for (int e = 0; e < kStep; ++e) x[e] = capped(x[e]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kStep; e += 2) {
-            float t[2];
-            unpair(capped_pair(pair_of(x[e], x[e + 1])), &t[0], &t[1]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              x[e + k] = fabsf(x[e + k]) <= cap_limit ? t[k] : capped(x[e + k]);
-            }
-          }
-        }
-      }
-      if constexpr (BIAS) {
-        // subtracted as integers: fp32 does not hold every place behind 2^24
-        const float from = static_cast<float>(place - key0);
-        const float factor = CAP ? 1.0f : scale;
-        if (all_past >= key0 + kStep - 1) {  // no key lies ahead of its row
-          const uint64_t f2 = pair_of(factor, factor), s2 = pair_of(slope, slope);
-          const uint64_t c2 = pair_of(-slope * from, -slope * from);
-#pragma unroll
-          for (int e = 0; e < kStep; e += 2) {
-            const uint64_t c =
-                fma2(s2, pair_of(static_cast<float>(e), static_cast<float>(e + 1)), c2);
-            const uint64_t y = CAP ? add2(pair_of(x[e], x[e + 1]), c)
-                                   : fma2(pair_of(x[e], x[e + 1]), f2, c);
-            unpair(y, &x[e], &x[e + 1]);
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < kStep; ++e) {
-            x[e] = x[e] * factor - slope * fabsf(from - static_cast<float>(e));
-          }
-        }
-      }
-      if (key0 + kStep > all_see) {
-        const int vis = seen - key0;
-#pragma unroll
-        for (int e = 0; e < kStep; ++e) x[e] = e < vis ? x[e] : -INFINITY;
-      }
-      float hi[4] = {m, m, m, m};
-#pragma unroll
-      for (int e = 0; e < kStep; e += 8) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) hi[c] = max3(hi[c], x[e + 2 * c], x[e + 2 * c + 1]);
-      }
-      const float top = max_nan(max3(hi[0], hi[1], hi[2]), hi[3]);
-      // The maximum in use moves only when it grew by more than 2^8: until then
-      // the weights stay below 256, which both 16-bit types hold as well as 1.
-      float factor = 1.0f;
-      const bool moved = !((top - m) * to_log2 <= 8.0f) && top != -INFINITY;
-      if (moved) {
-        factor = m == -INFINITY ? 1.0f : ex2((m - top) * to_log2);
-        m = top;
-      }
-      if (s > 0 && __any_sync(0xFFFFFFFFu, moved)) {
-        l *= factor;
-        // O += P V of the step before this one comes before S of this step (one
-        // buffer) or of the next
-        if (kBuffers == 2 && !wait_ready(&s_full[2 * t + ((s + 1) & 1)], ((s + 1) >> 1) & 1,
-                                         abort_flag, kErrAttnO, a.wait_limit_ns)) {
+    for (int s = 0; ok && s < n;) {
+      if (s > 0) {
+        // O += P V of the step before comes before S of this step (one buffer) or of the next
+        const int then = s + kBuffers - 1;
+        if (!wait_ready(&s_full[2 * t + then % kBuffers], (then / kBuffers) & 1, abort_flag,
+                        kErrAttnO, a.wait_limit_ns)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        const float factor = kept_factor();
+        float4* to = reinterpret_cast<float4*>(a.part_o + part_at() * a.head_dim);
 #pragma unroll 1
-        for (int c = 0; c < DP / 16; ++c) {
-          uint32_t o[16];
-          tmem_ld_32x32b_x16(o_at + 16 * c, o);
+        for (int c = 0; c < a.head_dim; c += 32, to += 8) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_ld_32x32b_x32(o_at + c, o);
           tmem_ld_wait(o);
+          if (valid) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-          tmem_st_32x32b_x16(o_at + 16 * c, o);
+            for (int i = 0; i < 8; ++i) {
+              if (c + 4 * i >= a.head_dim) break;
+              const float4 old = s == kFold ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : to[i];
+              to[i] = make_float4(fmaf(old.x, factor, __uint_as_float(o[4 * i])),
+                                  fmaf(old.y, factor, __uint_as_float(o[4 * i + 1])),
+                                  fmaf(old.z, factor, __uint_as_float(o[4 * i + 2])),
+                                  fmaf(old.w, factor, __uint_as_float(o[4 * i + 3])));
+            }
+          }
         }
+        __syncwarp();
+        m_kept = m;
       }
-      const float base = m == -INFINITY ? 0.0f : m * to_log2;
-      const uint64_t to2 = pair_of(to_log2, to_log2), base2 = pair_of(-base, -base);
-      uint64_t sum[2] = {0, 0};
-      uint32_t p[32];
+      const int stop = min(n, s + kFold);
+#pragma unroll 1
+      for (; s < stop; ++s) {
+        if (!wait_ready(&s_full[2 * t + s % kBuffers], (s / kBuffers) & 1, abort_flag, kErrAttnS,
+                        a.wait_limit_ns)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t s_now = s_at + kStep * (s % kBuffers);
+        const int key0 = (begin + s) * kStep;
+        float x[kStep];
+        {
+          uint32_t sr[2][32];
+          tmem_ld_32x32b_x32(s_now, sr[0]);
+          tmem_ld_32x32b_x32(s_now + 32, sr[1]);
+          tmem_ld_wait(sr[0]);
+          tmem_ld_wait(sr[1]);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        uint64_t y = pair_of(x[2 * e], x[2 * e + 1]);
-        y = kScaled ? add2(y, base2) : fma2(y, to2, base2);
-        float p0, p1;
-        unpair(y, &p0, &p1);
-        p0 = ex2(p0);
-        p1 = ex2(p1);
-        sum[e & 1] = add2(sum[e & 1], pair_of(p0, p1));
-        p[e] = pack_pair<T>(p0, p1);
+          for (int e = 0; e < kStep; ++e) x[e] = __uint_as_float(sr[e / 32][e % 32]);
+        }
+        if constexpr (CAP) {
+          float hi[2] = {x[0], x[0]}, lo[2] = {x[0], x[0]};
+#pragma unroll
+          for (int e = 0; e < kStep; e += 4) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              hi[c] = max3(hi[c], x[e + 2 * c], x[e + 2 * c + 1]);
+              lo[c] = min3(lo[c], x[e + 2 * c], x[e + 2 * c + 1]);
+            }
+          }
+          const bool small = max_nan(hi[0], hi[1]) <= cap_limit &&
+                             min3(lo[0], lo[1], lo[1]) >= -cap_limit;
+          if (__all_sync(0xFFFFFFFFu, small)) {
+#pragma unroll
+            for (int e = 0; e < kStep; e += 2) {
+              unpair(capped_pair(pair_of(x[e], x[e + 1])), &x[e], &x[e + 1]);
+            }
+          } else if (a.softcap <= kSmallCap) {
+#pragma unroll
+            for (int e = 0; e < kStep; ++e) x[e] = capped(x[e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < kStep; e += 2) {
+              float t[2];
+              unpair(capped_pair(pair_of(x[e], x[e + 1])), &t[0], &t[1]);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                x[e + k] = fabsf(x[e + k]) <= cap_limit ? t[k] : capped(x[e + k]);
+              }
+            }
+          }
+        }
+        if constexpr (BIAS) {
+          // subtracted as integers: fp32 does not hold every place behind 2^24
+          const float from = static_cast<float>(place - key0);
+          const float factor = CAP ? 1.0f : scale;
+          if (all_past >= key0 + kStep - 1) {  // no key lies ahead of its row
+            const uint64_t f2 = pair_of(factor, factor), s2 = pair_of(slope, slope);
+            const uint64_t c2 = pair_of(-slope * from, -slope * from);
+#pragma unroll
+            for (int e = 0; e < kStep; e += 2) {
+              const uint64_t c =
+                  fma2(s2, pair_of(static_cast<float>(e), static_cast<float>(e + 1)), c2);
+              const uint64_t y = CAP ? add2(pair_of(x[e], x[e + 1]), c)
+                                     : fma2(pair_of(x[e], x[e + 1]), f2, c);
+              unpair(y, &x[e], &x[e + 1]);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < kStep; ++e) {
+              x[e] = x[e] * factor - slope * fabsf(from - static_cast<float>(e));
+            }
+          }
+        }
+        if (key0 + kStep > all_see) {
+          const int vis = seen - key0;
+#pragma unroll
+          for (int e = 0; e < kStep; ++e) x[e] = e < vis ? x[e] : -INFINITY;
+        }
+        float hi[4] = {m, m, m, m};
+#pragma unroll
+        for (int e = 0; e < kStep; e += 8) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) hi[c] = max3(hi[c], x[e + 2 * c], x[e + 2 * c + 1]);
+        }
+        const float top = max_nan(max3(hi[0], hi[1], hi[2]), hi[3]);
+        // The maximum in use moves only when it grew by more than 2^8: until then
+        // the weights stay below 256, which both 16-bit types hold as well as 1.
+        float factor = 1.0f;
+        const bool moved = !((top - m) * to_log2 <= 8.0f) && top != -INFINITY;
+        if (moved) {
+          factor = m == -INFINITY ? 1.0f : ex2((m - top) * to_log2);
+          m = top;
+        }
+        if (s > 0 && __any_sync(0xFFFFFFFFu, moved)) {
+          l *= factor;
+          // O += P V of the step before this one comes before S of this step (one
+          // buffer) or of the next
+          if (kBuffers == 2 && !wait_ready(&s_full[2 * t + ((s + 1) & 1)], ((s + 1) >> 1) & 1,
+                                           abort_flag, kErrAttnO, a.wait_limit_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < DP / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(o_at + 16 * c, o);
+            tmem_ld_wait(o);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+            tmem_st_32x32b_x16(o_at + 16 * c, o);
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m * to_log2;
+        const uint64_t to2 = pair_of(to_log2, to_log2), base2 = pair_of(-base, -base);
+        uint64_t sum[2] = {0, 0};
+        uint32_t p[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+          uint64_t y = pair_of(x[2 * e], x[2 * e + 1]);
+          y = kScaled ? add2(y, base2) : fma2(y, to2, base2);
+          float p0, p1;
+          unpair(y, &p0, &p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          sum[e & 1] = add2(sum[e & 1], pair_of(p0, p1));
+          p[e] = pack_pair<T>(p0, p1);
+        }
+        tmem_st_32x32b_x32(s_now, p);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + s % kBuffers]);
+        float s0, s1;
+        unpair(add2(sum[0], sum[1]), &s0, &s1);
+        l += s0 + s1;
       }
-      tmem_st_32x32b_x32(s_now, p);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[2 * t + s % kBuffers]);
-      float s0, s1;
-      unpair(add2(sum[0], sum[1]), &s0, &s1);
-      l += s0 + s1;
     }
     if (n > 0 && ok) {
       // what follows the last step's O += P V
@@ -580,21 +632,19 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     if (ok) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const bool none = l == 0.0f;
-      const int64_t at = (static_cast<int64_t>(seq.batch) * a.q_heads + h) * a.q_len + row;
       const float lse = none ? -INFINITY : (m * to_log2 + log2f(l)) * 0.6931471805599453f;
-      const int64_t part_rows = static_cast<int64_t>(a.batch) * a.q_heads * a.q_len;
       if (valid) {
         if (a.splits > 1) {
-          a.part_lse[blockIdx.y * part_rows + at] = lse;
+          a.part_lse[part_at()] = lse;
         } else if (a.lse != nullptr) {
-          a.lse[at] = lse;
+          a.lse[lse_at()] = lse;
         }
       }
       const int64_t oo = static_cast<int64_t>(seq.batch) * a.o_stride[0] +
                          static_cast<int64_t>(row) * a.o_stride[1] +
                          static_cast<int64_t>(h) * a.o_stride[2];
-      const float* part = a.splits > 1 ? a.part_o + (blockIdx.y * part_rows + at) * a.head_dim
-                                       : nullptr;
+      float* part = a.part_o + part_at() * a.head_dim;  // splits > 1, or n > kFold
+      const float kept = n > kFold ? kept_factor() : 0.0f;
       // 32 columns at a time through the warp's share of the tile's Q (its MMAs
       // are done): a row's pieces are written side by side by neighbouring
       // threads, not by the one thread that holds the row.
@@ -625,10 +675,24 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
           tmem_ld_32x32b_x32(o_at + 32 * c, acc);
           tmem_ld_wait(acc);
         }
+        const int left = a.head_dim - 32 * c;  // a multiple of 8
+        if (n > kFold && valid) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            if (e < left) {
+              const float4 old = *reinterpret_cast<const float4*>(part + 32 * c + e);
+              const float o[4] = {old.x, old.y, old.z, old.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                acc[e + i] = __float_as_uint(fmaf(o[i], kept, __uint_as_float(acc[e + i])));
+              }
+            }
+          }
+        }
+        __syncwarp();
         float y[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) y[e] = none ? 0.0f : __uint_as_float(acc[e]) * inv;
-        const int left = a.head_dim - 32 * c;  // a multiple of 8
         if (a.splits > 1) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {

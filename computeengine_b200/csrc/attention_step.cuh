@@ -330,7 +330,13 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
       uint32_t m[4];
       ldmatrix4<true>(m, v_at + step_at<DP>(v_row, 2 * d + v_half));
 #pragma unroll
-      for (int n = 0; n < NT; ++n) mma_16816<T>(o[n][d], m, p[n][0], p[n][1]);
+      for (int n = 0; n < NT; ++n) {
+        // added here: the tensor core would cut off what lies below o's last place
+        float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        mma_16816<T>(y, m, p[n][0], p[n][1]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][d][e] += y[e];
+      }
     }
   }
   asm volatile("cp.async.wait_all;" ::: "memory");

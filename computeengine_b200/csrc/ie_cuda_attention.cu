@@ -199,6 +199,14 @@ PromptTiles prompt_tiles(const ie_attention_desc* d, const ie_attention_mask* m)
   return p;
 }
 
+// The prompt kernel's workspace: the shares' partial results, or, where a block may
+// take more than kFold steps, room for each row's O.
+size_t prompt_bytes(const ie_attention_desc* d, const PromptTiles& t) {
+  if (t.splits > 1) return share_bytes(d, t.splits);
+  if (d->kv_len <= kFold * kStep) return 0;
+  return static_cast<size_t>(d->batch * d->q_heads * d->q_len * d->head_dim * 4);
+}
+
 template <int DP, int T, bool CAP, bool BIAS>
 int launch_prompt(const PromptArgs& a, const CUtensorMap* maps, dim3 grid, cudaStream_t s) {
   auto kernel = attention_prompt_kernel<DP, T, CAP, BIAS>;
@@ -328,7 +336,7 @@ int run_prompt(const ie_attention_desc* d, const ie_attention_mask* m, const Att
   a.tiles = static_cast<int>(t.tiles);
   a.splits = t.splits;
   const int64_t rows = d->batch * d->q_heads * d->q_len * a.splits;
-  a.part_o = a.splits > 1 ? workspace : nullptr;
+  a.part_o = workspace;
   a.part_lse = a.splits > 1 ? workspace + round_up(rows * d->head_dim, 64) : nullptr;
   a.o_vec = reinterpret_cast<uintptr_t>(a.o) % 16 == 0 && a.o_lo % 8 == 0;
   for (int i = 0; i < 3; ++i) a.o_vec = a.o_vec && a.o_stride[i] % 8 == 0;
@@ -366,8 +374,8 @@ size_t ie_cuda_attention_workspace_bytes(const ie_attention_desc* desc,
                                          const ie_attention_mask* mask) {
   if (check_attention(desc, mask) != IE_OK) return 0;
   // few rows always run on the step kernel; many rows that TMA cannot read are not split
-  return share_bytes(desc, few_rows(desc, mask) ? step_tiles(desc, mask).splits
-                                                : prompt_tiles(desc, mask).splits);
+  return few_rows(desc, mask) ? share_bytes(desc, step_tiles(desc, mask).splits)
+                              : prompt_bytes(desc, prompt_tiles(desc, mask));
 }
 
 int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* mask, const void* q,
@@ -386,7 +394,7 @@ int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* ma
                                           desc->batch, desc->q_stride);
   const size_t need =
       few ? share_bytes(desc, step_tiles(desc, mask).splits)
-          : tma ? share_bytes(desc, prompt_tiles(desc, mask).splits) : size_t{0};
+          : tma ? prompt_bytes(desc, prompt_tiles(desc, mask)) : size_t{0};
   if (need > 0 && (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 256 != 0 ||
                    workspace_bytes < need)) {
     return fail(IE_INVALID_ARGUMENT, "Attention needs %zu bytes of 256-byte aligned workspace",

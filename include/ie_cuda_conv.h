@@ -580,9 +580,10 @@ typedef struct ie_attention_mask {
 
 /* mask may be NULL (every key visible).  lse: fp32 [batch, q_heads, q_len] or
  * NULL.  workspace must hold ie_cuda_attention_workspace_bytes(desc, mask)
- * bytes (256-byte aligned; 0 where the rows alone fill the GPU, then it may be
- * NULL): few queries over many keys are computed in shares, whose number
- * depends on the batch, and joined.  Its contents need not be kept; calls that
+ * bytes (256-byte aligned; 0 where the rows alone fill the GPU and kv_len is at
+ * most 32768, then it may be NULL): few queries over many keys are computed in
+ * shares, whose number depends on the batch, and joined; sums over more keys than
+ * that are put away in between.  Its contents need not be kept; calls that
  * overlap on the GPU need one each.
  * Full speed: q, k and v 16-byte aligned, head_dim a multiple of 8, strides
  * multiples of 8 and not 0; other tensors take a slower kernel. */

@@ -1,0 +1,81 @@
+"""Attention over so many keys of nearly equal weight that a sum of them is large
+next to each.
+
+The weights are equal and exact (q is 0), v is not negative: o is the mean of v,
+off by one rounding to its type and by what the sums lose.  A tensor core cuts
+off what lies below its fp32 sum's last place: of n products of about 1 at most
+n * 2^-24 of each, so 2^-9 for the 2^15 keys that go through one such sum, and
+half of that on average.  Everything else is rounded to nearest."""
+import pytest
+
+from tests.token_ops import HALF_STEP, attention_desc, attention_mask, run_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def run(q, k, v, document):
+    import math
+    import torch
+    from computeengine_b200 import _lib as L
+    o = torch.full_like(q, float("nan"))
+    lse = torch.full((q.shape[0], q.shape[2], q.shape[1]), float("nan"), device="cuda")
+    m = attention_mask(L)
+    if document:  # the keys of a document are not shared out
+        at = [torch.tensor([0, n], dtype=torch.int32, device="cuda")
+              for n in (q.shape[1], k.shape[1])]
+        m = attention_mask(L, documents=1, q_offsets=at[0], kv_offsets=at[1])
+    run_attention(L, attention_desc(L, q, k, v, o, 1.0), m, q, k, v, o, lse)
+    assert L.take_device_error() == 0
+    want = v.double().mean(dim=1, keepdim=True).repeat_interleave(q.shape[2] // v.shape[2], 2)
+    err = ((o.double() - want).abs() / want).max()
+    assert err <= HALF_STEP[q.dtype] + 2.0 ** -10, float(err)
+    assert (lse - math.log(k.shape[1])).abs().max() <= 2.0 ** -12
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("keys", [(1 << 15) + 1, 1 << 18, (1 << 20) + 77, 1 << 23])
+@pytest.mark.parametrize("sq, hq, hk, document", [(1, 1, 1, False), (1, 1, 1, True),
+                                                  (3, 8, 2, False), (40, 4, 2, False),
+                                                  (300, 2, 1, True)])
+def test_equal_weights(sq, hq, hk, document, keys, dtype):
+    """Single tokens with and without shares, packed rows with shares, whole tiles."""
+    import torch
+    dt = getattr(torch, dtype)
+    for d in (8, 72) if keys < 1 << 20 else (8,):
+        g = torch.Generator(device="cuda").manual_seed(keys)
+        v = (torch.rand(1, keys, hk, d, generator=g, device="cuda") + 0.5).to(dt)
+        run(torch.zeros(1, sq, hq, d, dtype=dt, device="cuda"), torch.zeros_like(v), v, document)
+
+
+@pytest.mark.parametrize("document", [False, True])
+def test_equal_weights_of_rows_that_tma_cannot_read(document):
+    import torch
+    v = torch.rand(1, 1 << 20, 1, 9, device="cuda")[..., 1:].add(0.5).to(torch.float16)
+    v = torch.cat([v[..., :1], v], -1)[..., 1:]  # rows of 18 bytes
+    q = torch.zeros(1, 5, 1, 8, dtype=torch.float16, device="cuda")
+    run(q, torch.zeros_like(v), v, document)
+
+
+@pytest.mark.parametrize("sq, document", [(1, False), (40, False), (300, True)])
+def test_growing_scores_over_many_keys(sq, document):
+    """The maximum moves all the time, between and at the points where the sums
+    are put away; a causal border and a cap besides.  Against 64 bits."""
+    import torch
+    from computeengine_b200 import _lib as L
+    from tests.token_ops import attention_64, check_attention
+    n = 70001
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.rand(1, sq, 2, 64, generator=g, device="cuda").bfloat16()
+    k = torch.rand(1, n, 1, 64, generator=g, device="cuda")
+    k = (k * torch.linspace(0, 1, n, device="cuda")[None, :, None, None]).bfloat16()
+    v = torch.randn(1, n, 1, 64, generator=g, device="cuda").bfloat16()
+    o, lse = torch.empty_like(q), torch.empty(1, 2, sq, device="cuda")
+    at = [torch.tensor([0, x], dtype=torch.int32, device="cuda") for x in (sq, n)]
+    kw = dict(causal=1)
+    if document:
+        kw.update(q_offsets=at[0], kv_offsets=at[1])
+    m = attention_mask(L, documents=int(document), **kw)
+    for cap in (0.0, 30.0):
+        run_attention(L, attention_desc(L, q, k, v, o, 2.0, cap), m, q, k, v, o, lse)
+        assert not o.isnan().any()
+        check_attention(o, lse, attention_64(q, k, v, 2.0, cap, **kw), q.dtype)
