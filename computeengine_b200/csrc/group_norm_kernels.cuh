@@ -2,21 +2,22 @@
 //
 // A thread owns V neighbouring channels (one 16-byte load of x) and strides
 // over the pixels, so everything it does is per channel and a group may begin
-// and end anywhere in a vector.  Statistics: each batch of pixels gives its
-// exact mean and sum of squared differences per channel, joined with what the
-// thread has by the pairwise update of Chan, Golub and LeVeque (1979); threads,
-// then blocks are joined the same way in a fixed order.  A mean far from zero
-// therefore costs no precision and results do not depend on timing.
+// and end anywhere in a vector.  Statistics: a thread takes each channel's mean, and
+// the squares about it, from differences to a pixel or to the mean so far; threads,
+// then blocks are joined by the differences of their means to one value of the group
+// (its first channel at the image's first pixel) and the squares about their mean
+// (Chan, Golub and LeVeque 1979), all in fp32 and in a fixed order.  The mean, kept as
+// two numbers, is subtracted before the scale.  So errors follow the spread, however
+// far the mean is from zero, and results do not depend on timing.
 //
 // group_norm_cluster_kernel: a channel range of an image is held in the shared
 // memory of one block or a cluster of up to 8, so x is read once.
 // group_norm_stats_kernel, group_norm_apply_kernel: for images that do not fit.
-// 32 x 56 x 56 x 256 fp32 (held): 59 us, 3.5 TB/s of x and y; 512 x 512 x 128
-// bf16 (read twice): 50 us, 2.7 TB/s of x and y, 4.0 TB/s with the second read.
+// 32 x 56 x 56 x 256 fp32 (held): 56 us, 3.7 TB/s of x and y; 512 x 512 x 128
+// bf16 (read twice): 53 us, 2.5 TB/s of x and y, 3.8 TB/s with the second read.
 #pragma once
 
 #include <cooperative_groups.h>
-
 
 #include "element_types.cuh"
 
@@ -37,12 +38,11 @@ struct GroupNormArgs {
   int share;            // pixels of a block
   int parts, part_share;  // two-kernel path: clusters of blocks, and their pixels
   int cols[2], rows[2]; // threads over a range's vectors and pixels: inner, last range
-  float2* partial;      // two-kernel path: mean and sum of squared differences,
-                        // [image][range][range_groups][part]
+  float4* partial;      // two-kernel path: [image][range][range_groups][part]
 };
 
 constexpr int kGnThreads = 256;
-constexpr int kGnBatch = 4;  // pixels per exact mean
+constexpr int kGnBatch = 4;    // a thread's pixels, at least, in a statistics block
 constexpr int kGnCluster = 4;  // blocks of the statistics kernel joined before memory
 
 // Kinds of activation: a clamp to [low, high] (none, ReLU, ReLU6), SiLU, GELU.
@@ -171,12 +171,26 @@ struct Pairs {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) p[i] = add2(p[i], o.p[i]);
   }
-  __device__ __forceinline__ void add_squares(const Pairs& o, const Pairs& minus) {
+  __device__ __forceinline__ Pairs plus(const Pairs& o) const {
+    Pairs r;
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const uint64_t d = add2(o.p[i], minus.p[i]);
-      p[i] = fma2(d, d, p[i]);
-    }
+    for (int i = 0; i < kCount; ++i) r.p[i] = add2(p[i], o.p[i]);
+    return r;
+  }
+  __device__ __forceinline__ Pairs times(float f) const {
+    Pairs r;
+    const uint64_t f2 = pair_of(f, f);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) r.p[i] = mul2(p[i], f2);
+    return r;
+  }
+  __device__ __forceinline__ void add_product(const Pairs& a, const Pairs& b) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) p[i] = fma2(a.p[i], b.p[i], p[i]);
+  }
+  __device__ __forceinline__ void add_squares(const Pairs& d) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) p[i] = fma2(d.p[i], d.p[i], p[i]);
   }
 };
 
@@ -226,57 +240,52 @@ __device__ __forceinline__ void store_item(void* y, int64_t at, int c_store, con
   }
 }
 
-// Running statistics of V channels over the pixels a thread has seen.
+// Running statistics of V channels over the pixels a thread has seen: the mean is
+// pivot + rest, and pivot moves with it, so that sums of a batch's differences to it
+// and of their squares lose no more than the squares of the means' differences.
 template <int V>
 struct Running {
-  Pairs<V> mean, m2;
+  Pairs<V> pivot, rest, m2;
   int n = 0;
 
   __device__ __forceinline__ Running() {
-    mean.zero();
+    pivot.zero();
+    rest.zero();
     m2.zero();
   }
-  // Joins k > 0 pixels of the given mean and squares about it.
-  __device__ __forceinline__ void join(int k, const Pairs<V>& batch, const Pairs<V>& squares) {
-    if (n == 0) {
-      mean = batch;
-      m2 = squares;
-    } else {
-      const float share = static_cast<float>(k) / static_cast<float>(n + k);
-      const float weight = static_cast<float>(n) * share;
-      const uint64_t share2 = pair_of(share, share), weight2 = pair_of(weight, weight);
-      const uint64_t minus1 = pair_of(-1.0f, -1.0f);
+  // The next K pixels, the k-th of them at(k).
+  template <int K, class At>
+  __device__ __forceinline__ void add(const At& at) {
+    if (n == 0) pivot = at(0);
+    const Pairs<V> minus = pivot.times(-1.0f);
+    Pairs<V> sum;
+    sum.zero();
 #pragma unroll
-      for (int i = 0; i < Pairs<V>::kCount; ++i) {
-        const uint64_t d = fma2(mean.p[i], minus1, batch.p[i]);
-        mean.p[i] = fma2(d, share2, mean.p[i]);
-        m2.p[i] = add2(m2.p[i], fma2(mul2(d, d), weight2, squares.p[i]));
-      }
+    for (int k = 0; k < K; ++k) {
+      const Pairs<V> d = at(k).plus(minus);
+      sum.add(d);
+      m2.add_squares(d);
     }
-    n += k;
-  }
-  // A whole batch in registers.
-  __device__ __forceinline__ void add(const Pairs<V> (&f)[kGnBatch]) {
-    Pairs<V> s = f[0], q, minus;
-#pragma unroll
-    for (int i = 1; i < kGnBatch; ++i) s.add(f[i]);
-    const uint64_t inv = pair_of(1.0f / kGnBatch, 1.0f / kGnBatch);
-    const uint64_t minus_inv = pair_of(-1.0f / kGnBatch, -1.0f / kGnBatch);
+    const float share = static_cast<float>(K) / static_cast<float>(n + K);
+    const float weight = static_cast<float>(n) * share;
+    const uint64_t share2 = pair_of(share, share), weight2 = pair_of(weight, weight);
+    const uint64_t inv = pair_of(1.0f / K, 1.0f / K), minus1 = pair_of(-1.0f, -1.0f);
 #pragma unroll
     for (int i = 0; i < Pairs<V>::kCount; ++i) {
-      minus.p[i] = mul2(s.p[i], minus_inv);
-      s.p[i] = mul2(s.p[i], inv);
+      const uint64_t mean = mul2(sum.p[i], inv);  // of the batch, as difference to pivot
+      const uint64_t d = fma2(rest.p[i], minus1, mean);
+      const uint64_t squares = fma2(mul2(sum.p[i], minus1), mean, m2.p[i]);
+      m2.p[i] = fma2(mul2(d, d), weight2, squares);
+      const uint64_t moved = fma2(d, share2, rest.p[i]);
+      const uint64_t to = add2(pivot.p[i], moved);
+      rest.p[i] = add2(fma2(to, minus1, pivot.p[i]), moved);
+      pivot.p[i] = to;
     }
-    q.zero();
-#pragma unroll
-    for (int i = 0; i < kGnBatch; ++i) q.add_squares(f[i], minus);
-    join(kGnBatch, s, q);
+    n += K;
   }
-  // One pixel.
-  __device__ __forceinline__ void add(const Pairs<V>& f) {
-    Pairs<V> q;
-    q.zero();
-    join(1, f, q);
+  // The mean as difference to `base`.
+  __device__ __forceinline__ Pairs<V> mean(const Pairs<V>& base) const {
+    return pivot.plus(base.times(-1.0f)).plus(rest);
   }
 };
 
@@ -285,80 +294,200 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// Sums each thread's V channels into the groups of the block's channel range:
-// out[g], in an order that is always the same.  Thread t holds the channels
-// (t % cols) * V .. of the range, rows = threads per column.  First slices of
-// the rows of each channel are summed by all threads, then a warp sums a
-// group.  scratch holds (V + 1) * threads floats.  (A single group wider than
-// the threads' columns: group_channels is what the columns hold.)
+// A group's statistics: mean + rest is its mean (below the last join, `mean` is the
+// value that differences are taken to), squares the sum of squares about it.
+struct Stat {
+  float mean, rest, squares;
+};
+
+// The same with `mean` the mean rounded, and 1 / sigma in the place of the squares.
+__device__ __forceinline__ Stat finished(const Stat& s, float size, float eps) {
+  const float mean = s.mean + s.rest;
+  const float back = mean - s.mean;  // what of rest went into mean; the rest is exact
+  const float squares = s.squares < 0.0f ? 0.0f : s.squares;  // a rounding below; NaN stays
+  return {mean, (s.mean - (mean - back)) + (s.rest - back), 1.0f / sqrtf(squares / size + eps)};
+}
+
+// Block-wide joins of what each thread holds of V channels: thread t has the
+// channels (t % cols) * V .. of the range, rows = threads per column, whose `count`
+// pixels are dealt to the rows in turn.  First slices of the rows of each channel are
+// joined by all threads, then a warp joins a group.  scratch holds (V + 2) * threads
+// floats, 16-byte aligned.  Everything that needs a division is made before the data.
 template <int V>
-__device__ __forceinline__ void group_sums(const Pairs<V>& v, int cols, int rows,
-                                           int group_channels, int groups, float* scratch,
-                                           float* out) {
-  const int width = cols * V, t = threadIdx.x, lane = t & 31;
-  if (t < cols * rows) {  // [rows][width]
+struct Columns {
+  int cols, rows, width, count;
+  int all;             // columns of the range; more than cols: it is a single group
+  int group_channels;  // of the columns held (all > cols: all of them)
+  int groups;
+  bool wide;           // threads own channels, not slices of them
+  int slices, slice, channel;  // of rows; this thread's
+  int shift;           // lanes over a group's channels; the others over slices
+  int each, extra;     // pixels of row k: each + (k < extra)
+  float inv_size, inv_slices, inv_pixels;  // of a group, and of this thread's slice
+
+  __device__ __forceinline__ Columns(int cols, int rows, int all, int count, int group_channels,
+                                     int groups, float size)
+      : cols(cols), rows(rows), width(cols * V), count(count), all(all),
+        group_channels(group_channels), groups(groups), inv_size(1.0f / size) {
+    const int t = threadIdx.x;
+    wide = width >= kGnThreads;
+    slices = wide ? 1 : kGnThreads / width;
+    slice = wide ? 0 : t / width;
+    channel = t - slice * width;
+    shift = 0;
+    while ((1 << shift) < group_channels && shift < 5) ++shift;
+    each = count / rows;
+    extra = count - each * rows;
+    inv_slices = 1.0f / static_cast<float>(slices);
+    const float p = pixels(slice);
+    inv_pixels = p > 0.0f ? 1.0f / p : 0.0f;
+  }
+  // ceil(v / slices) of -slices < v <= 256
+  __device__ __forceinline__ float per_slice(int v) const {
+    return ceilf((static_cast<float>(v) - 0.5f) * inv_slices);
+  }
+  __device__ __forceinline__ float pixels(int k) const {  // of slice k
+    return static_cast<float>(each) * per_slice(rows - k) + fmaxf(per_slice(extra - k), 0.0f);
+  }
+};
+
+template <int V>
+__device__ __forceinline__ void put_channels(const Pairs<V>& v, const Columns<V>& c,
+                                             float* scratch) {
+  const int t = threadIdx.x;
+  if (t >= c.cols * c.rows) return;  // [rows][width]
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const float2 lo = floats_of(v.p[e / 2]), hi = floats_of(v.p[e / 2 + 1]);
+      *reinterpret_cast<float4*>(scratch + t * V + e) = make_float4(lo.x, lo.y, hi.x, hi.y);
+    }
+  } else {
 #pragma unroll
     for (int e = 0; e < V; ++e) scratch[t * V + e] = v[e];
   }
+}
+
+// Joins each thread's means (0 where it has no pixel) and squares into stat[g].rest and
+// stat[g].squares.
+template <int V>
+__device__ __forceinline__ void join_threads(const Pairs<V>& mean, const Pairs<V>& squares,
+                                             const Columns<V>& c, float* scratch, Stat* stat) {
+  const int t = threadIdx.x, lane = t & 31;
+  put_channels<V>(mean, c, scratch);
   __syncthreads();
-  float* partial = scratch;  // [slices][width]
-  int slices = 1;
-  if (width >= kGnThreads) {  // a channel's sum replaces its first row
-    for (int ch = t; ch < width; ch += kGnThreads) {
-      float s = scratch[ch];
-      for (int k = 1; k < rows; ++k) s += scratch[k * width + ch];
-      scratch[ch] = s;
+  // The slice's rows of a channel, about the first of them: the squares about it are
+  // at most as many times those about their mean as there are rows, below 2 V.
+  auto join_rows = [&](int ch) {
+    const float first = scratch[c.slice * c.width + ch];
+    float s = 0.0f, q = 0.0f;
+#pragma unroll 4
+    for (int k = c.slice; k < c.rows; k += c.slices) {
+      const float w = static_cast<float>(c.each + (k < c.extra ? 1 : 0));
+      const float d = scratch[k * c.width + ch] - first, wd = w * d;
+      s += wd;
+      q = fmaf(wd, d, q);
+    }
+    const float m = s * c.inv_pixels;
+    return make_float2(first + m, q - s * m);
+  };
+  auto sum_rows = [&](int ch) {
+    float s = 0.0f;
+#pragma unroll 4
+    for (int k = c.slice; k < c.rows; k += c.slices) s += scratch[k * c.width + ch];
+    return s;
+  };
+  float* part_mean = scratch;  // [slices][width], and the squares
+  float* part_squares = scratch + c.width;
+  if (c.wide) {  // over a channel's first two rows
+    for (int ch = t; ch < c.width; ch += kGnThreads) {
+      const float2 r = join_rows(ch);
+      part_mean[ch] = r.x;
+      if (c.rows > 1) part_squares[ch] = r.y;
     }
   } else {
-    partial = scratch + V * kGnThreads;
-    slices = kGnThreads / width;
-    const int slice = t / width, ch = t - slice * width;
-    if (slice < slices) {
-      float s = 0.0f;
-#pragma unroll 4
-      for (int k = slice; k < rows; k += slices) s += scratch[k * width + ch];
-      partial[t] = s;
+    part_mean = scratch + V * kGnThreads;
+    part_squares = part_mean + kGnThreads;
+    float2 r = make_float2(0.0f, 0.0f);
+    if (c.slice < c.slices) r = join_rows(c.channel);
+    __syncthreads();
+    put_channels<V>(squares, c, scratch);
+    __syncthreads();
+    if (c.slice < c.slices) {
+      part_mean[t] = r.x;
+      part_squares[t] = r.y + sum_rows(c.channel);
     }
   }
   __syncthreads();
-  // lanes over the group's channels, and over slices when they are few
-  int lanes = 1, shift = 0;
-  while (lanes < group_channels && lanes < 32) {
-    lanes <<= 1;
-    ++shift;
-  }
-  for (int g = t >> 5; g < groups; g += kGnThreads / 32) {
-    float s = 0.0f;
-    for (int k = lane >> shift; k < slices; k += 32 >> shift) {
-      const float* row = partial + k * width + g * group_channels;
-      for (int ch = lane & (lanes - 1); ch < group_channels; ch += lanes) s += row[ch];
+  const int shift = c.shift, lanes = 1 << shift, ch0 = lane & (lanes - 1);
+  // pixels of a slice (all > cols: of a thread's columns)
+  auto weight = [&](int k, int ch) {
+    if (c.all <= c.cols) return c.pixels(k);
+    return static_cast<float>(c.count * ((c.all - ch / V + c.cols - 1) / c.cols));
+  };
+  for (int g = t >> 5; g < c.groups; g += kGnThreads / 32) {
+    const float first = part_mean[g * c.group_channels];
+    float s = 0.0f, q = 0.0f;
+    for (int k = lane >> shift; k < c.slices; k += 32 >> shift) {
+      const int row = k * c.width + g * c.group_channels;
+      float w = weight(k, 0);
+      for (int ch = ch0; ch < c.group_channels; ch += lanes) {
+        if (c.all > c.cols) w = weight(k, ch);
+        s = fmaf(w, part_mean[row + ch] - first, s);
+        if (!c.wide || c.rows > 1) q += part_squares[row + ch];
+      }
     }
+    const float m = warp_sum(s) * c.inv_size;
+    for (int k = lane >> shift; k < c.slices; k += 32 >> shift) {
+      const int row = k * c.width + g * c.group_channels;
+      float w = weight(k, 0);
+      for (int ch = ch0; ch < c.group_channels; ch += lanes) {
+        if (c.all > c.cols) w = weight(k, ch);
+        const float d = (part_mean[row + ch] - first) - m;
+        q = fmaf(w * d, d, q);
+      }
+    }
+    q = warp_sum(q);
+    if (lane == 0) {
+      stat[g].rest = first + m;
+      stat[g].squares = q;
+    }
+  }
+  __syncthreads();
+  if (!c.wide) return;
+  put_channels<V>(squares, c, scratch);
+  __syncthreads();
+  for (int ch = t; ch < c.width; ch += kGnThreads) scratch[ch] = sum_rows(ch);
+  __syncthreads();
+  for (int g = t >> 5; g < c.groups; g += kGnThreads / 32) {
+    float s = 0.0f;
+    for (int ch = lane; ch < c.group_channels; ch += 32) s += scratch[g * c.group_channels + ch];
     s = warp_sum(s);
-    if (lane == 0) out[g] = s;
+    if (lane == 0) stat[g].squares += s;
   }
   __syncthreads();
 }
 
-// Joins the statistics of `blocks` pixel blocks, block k's at at(k), into the
-// mean and 1 / sigma of a group.
+// Joins the statistics of `blocks` blocks of `share` pixels, all about one value:
+// first the means, then the squares about their mean.
 template <class At>
-__device__ __forceinline__ float2 join_blocks(const GroupNormArgs& a, int group_channels,
-                                              const At& at) {
+__device__ __forceinline__ Stat join_blocks(int blocks, int share, int pixels, int group_channels,
+                                            const At& at) {
+  auto pixels_of = [&](int k) {
+    return static_cast<float>(min(pixels, (k + 1) * share) - k * share);
+  };
   float s = 0.0f, q = 0.0f;
-  for (int k = 0; k < a.blocks; ++k) {
-    const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
-    if (w > 0) s += static_cast<float>(w) * at(k).x;
+  for (int k = 0; k < blocks; ++k) {
+    if (pixels_of(k) > 0.0f) s = fmaf(pixels_of(k), at(k).rest, s);
   }
-  const float mu = a.blocks == 1 ? at(0).x : s / static_cast<float>(a.pixels);
-  for (int k = 0; k < a.blocks; ++k) {
-    const int w = min(a.pixels, (k + 1) * a.share) - k * a.share;
-    if (w <= 0) continue;
-    const float2 o = at(k);
-    const float d = o.x - mu;
-    q += o.y + static_cast<float>(w) * static_cast<float>(group_channels) * d * d;
+  const float mean = s / static_cast<float>(pixels);
+  for (int k = 0; k < blocks; ++k) {
+    if (pixels_of(k) > 0.0f) {
+      const float d = at(k).rest - mean;
+      q += at(k).squares + pixels_of(k) * static_cast<float>(group_channels) * d * d;
+    }
   }
-  const float size = static_cast<float>(a.pixels) * static_cast<float>(group_channels);
-  return make_float2(mu, 1.0f / sqrtf(q / size + a.eps));
+  return {at(0).mean, mean, q};
 }
 
 // Geometry shared by the kernels: the block's channel range.
@@ -374,39 +503,73 @@ struct Range {
   }
 };
 
-// mul and add of the V channels from c: gamma / sigma, and beta less the mean's
-// share of it.  stat: mean and 1 / sigma of the range's groups; the thread's
-// first channel is `inner` channels into group `first`.
+// The value of a group that its statistics are about.
+template <int XT>
+__device__ __forceinline__ float group_base(const GroupNormArgs& a, const Range& r, int64_t image,
+                                            int g) {
+  const int64_t at = channel_at<XT>(image * a.pixels, a.c_store, r.c0 + g * r.group_channels);
+  float v = load_element<XT>(a.x, at);
+  if constexpr (XT == IE_DT_BF16X2) v += load_element<XT>(a.x, at + a.c_store);
+  return v;
+}
+
+// Of the groups of V channels, the first `inner` channels into group g; 0 for padding.
+template <int V>
+__device__ __forceinline__ Pairs<V> group_bases(const Stat* stat, int groups, int group_channels,
+                                                int g, int inner) {
+  float base[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) {
+    base[e] = g < groups ? stat[g].mean : 0.0f;
+    if (++inner == group_channels) {
+      inner = 0;
+      ++g;
+    }
+  }
+  Pairs<V> p;
+  p.set(base);
+  return p;
+}
+
+// Of the V channels from c: the mean to subtract, gamma / sigma, and beta less the
+// share of what the mean lacks.  stat: the range's groups; the thread's first channel
+// is `inner` channels into group `first`.
+template <int V>
+struct Affine {
+  Pairs<V> minus, mul, add;
+};
+
 template <int V>
 __device__ __forceinline__ void channel_affine(const GroupNormArgs& a, int c, int first, int inner,
-                                               const float2* stat, Pairs<V>* mul_pairs,
-                                               Pairs<V>* add_pairs) {
-  float mul[V], add[V];
+                                               const Stat* stat, Affine<V>* affine) {
+  float minus[V], mul[V], add[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) {
     const bool in = c + e < a.c;
-    const float2 st = in ? stat[first] : make_float2(0.0f, 0.0f);
-    mul[e] = in && a.gamma != nullptr ? st.y * a.gamma[c + e] : st.y;
-    add[e] = fmaf(-st.x, mul[e], in && a.beta != nullptr ? a.beta[c + e] : 0.0f);
+    const Stat st = in ? stat[first] : Stat{0.0f, 0.0f, 0.0f};
+    minus[e] = -st.mean;
+    mul[e] = in && a.gamma != nullptr ? st.squares * a.gamma[c + e] : st.squares;
+    add[e] = fmaf(-st.rest, mul[e], in && a.beta != nullptr ? a.beta[c + e] : 0.0f);
     if (++inner == a.group_channels) {
       inner = 0;
       ++first;
     }
   }
-  mul_pairs->set(mul);
-  add_pairs->set(add);
+  affine->minus.set(minus);
+  affine->mul.set(mul);
+  affine->add.set(add);
 }
 
 // Normalizes, activates and stores one item; channels past c are zero before
 // the activation already (mul and add are zero there, but x may hold anything).
 template <int YT, int V, int ACT>
 __device__ __forceinline__ void finish_item(const GroupNormArgs& a, const Pairs<V>& x,
-                                            const Pairs<V>& mul, const Pairs<V>& add, uint8_t* y,
-                                            int valid) {
+                                            const Affine<V>& affine, uint8_t* y, int valid) {
   float f[V];
 #pragma unroll
   for (int i = 0; i < Pairs<V>::kCount; ++i) {
-    const float2 r = floats_of(fma2(x.p[i], mul.p[i], add.p[i]));
+    const float2 r = floats_of(
+        fma2(add2(x.p[i], affine.minus.p[i]), affine.mul.p[i], affine.add.p[i]));
     f[2 * i] = r.x;
     if (2 * i + 1 < V) f[2 * i + 1] = r.y;
   }
@@ -427,12 +590,11 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
   constexpr int kItem = Item<XT, V>::kBytes * (XT == IE_DT_BF16X2 ? 2 : 1);
   static_assert(Item<XT, V>::kBytes == 16, "16-byte copies");
   extern __shared__ __align__(16) uint8_t smem[];
-  float2* own = reinterpret_cast<float2*>(smem);    // [range_groups] of this block
-  float2* stat = own + a.range_groups;              // [range_groups] mean, 1 / sigma
-  float2* others = stat + a.range_groups;           // [blocks][range_groups]
-  float* sums = reinterpret_cast<float*>(others + a.blocks * a.range_groups);  // [range_groups]
-  float* scratch = sums + a.range_groups;
-  uint8_t* items = reinterpret_cast<uint8_t*>(scratch + (V + 1) * kGnThreads);
+  float* scratch = reinterpret_cast<float*>(smem);
+  Stat* own = reinterpret_cast<Stat*>(scratch + (V + 2) * kGnThreads);  // of this block
+  Stat* stat = own + a.range_groups;                                    // of the image
+  Stat* others = stat + a.range_groups;                                 // [blocks][range_groups]
+  uint8_t* items = reinterpret_cast<uint8_t*>(others + a.blocks * a.range_groups);
   items += (16 - reinterpret_cast<uintptr_t>(items) % 16) % 16;
 
   cg::cluster_group cluster = cg::this_cluster();
@@ -467,6 +629,12 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
   }
   // the thread's place among the groups, while the copies are under way
   const int first = col * V / r.group_channels, inner = col * V - first * r.group_channels;
+  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) {
+    own[g].mean = group_base<XT>(a, r, image, g);
+  }
+  const Columns<V> columns(r.cols, r.rows, r.cols, count, r.group_channels, a.range_groups,
+                           static_cast<float>(count) * static_cast<float>(r.group_channels));
+  const float inv_n = n > 0 ? 1.0f / static_cast<float>(n) : 0.0f;
   asm volatile("cp.async.wait_all;" ::: "memory");
 
   auto item = [&](int i) {
@@ -475,34 +643,27 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
     if constexpr (XT == IE_DT_BF16X2) it.lo = load_bytes<16>(mine + i * kStep + kGnThreads * 16);
     return item_pairs<XT, V>(it);
   };
-  // the block's mean of each group, then the squares about it
-  Pairs<V> v;
-  v.zero();
+  // the thread's differences to its first pixel, and their squares (of at most 28
+  // pixels, by the shared memory: at most 28 times the squares about their mean)
+  __syncthreads();  // the groups' values
+  Pairs<V> mean, squares;
+  mean.zero();
+  squares.zero();
+  if (n > 0) {
+    const Pairs<V> first_pixel = item(0), minus = first_pixel.times(-1.0f);
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) v.add(item(i));
-  group_sums<V>(v, r.cols, r.rows, r.group_channels, a.range_groups, scratch, sums);
-  const float inv = 1.0f / (static_cast<float>(count) * static_cast<float>(r.group_channels));
-  {
-    float minus[V];
-    int g = first, in_group = inner;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {  // padding channels: the group's that would follow
-      minus[e] = -sums[min(g, a.range_groups - 1)] * inv;
-      if (++in_group == r.group_channels) {
-        in_group = 0;
-        ++g;
-      }
+    for (int i = 1; i < n; ++i) {
+      const Pairs<V> d = item(i).plus(minus);
+      mean.add(d);
+      squares.add_squares(d);
     }
-    Pairs<V> minus_pairs;
-    minus_pairs.set(minus);
-    v.zero();
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) v.add_squares(item(i), minus_pairs);
+    const Pairs<V> sum = mean;
+    mean = sum.times(inv_n);
+    squares.add_product(sum, mean.times(-1.0f));
+    const Pairs<V> base = group_bases<V>(own, a.range_groups, r.group_channels, first, inner);
+    mean.add(first_pixel.plus(base.times(-1.0f)));
   }
-  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) own[g].x = sums[g] * inv;
-  __syncthreads();
-  group_sums<V>(v, r.cols, r.rows, r.group_channels, a.range_groups, scratch, sums);
-  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) own[g].y = sums[g];
+  join_threads<V>(mean, squares, columns, scratch, own);
 
   // the blocks' statistics, in rank order
   if (a.blocks > 1) {
@@ -516,20 +677,24 @@ __global__ void __launch_bounds__(kGnThreads, 4) group_norm_cluster_kernel(const
   }
   __syncthreads();
   for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) {
-    stat[g] = join_blocks(a, r.group_channels, [&](int k) {
-      return a.blocks > 1 ? others[k * a.range_groups + g] : own[g];
-    });
+    Stat all = own[g];
+    if (a.blocks > 1) {
+      all = join_blocks(a.blocks, a.share, a.pixels, r.group_channels,
+                        [&](int k) { return others[k * a.range_groups + g]; });
+    }
+    stat[g] = finished(all, static_cast<float>(a.pixels) * static_cast<float>(r.group_channels),
+                       a.eps);
   }
   __syncthreads();
-  Pairs<V> g, b;
-  if (n > 0) channel_affine<V>(a, c, first, inner, stat, &g, &b);
+  Affine<V> affine;
+  if (n > 0) channel_affine<V>(a, c, first, inner, stat, &affine);
   uint8_t* y = static_cast<uint8_t*>(a.y) +
                channel_at<YT>(p0 + row, a.c_store, c) * element_bytes(YT);
   const int64_t y_step = static_cast<int64_t>(r.rows) * channel_at<YT>(1, a.c_store, 0) *
                          element_bytes(YT);
 #pragma unroll(ACT == kActGelu ? 1 : 2)
   for (int i = 0; i < n; ++i, y += y_step) {
-    finish_item<YT, V, ACT>(a, item(i), g, b, y, a.c - c);
+    finish_item<YT, V, ACT>(a, item(i), affine, y, a.c - c);
   }
   if (a.blocks > 1) cluster.barrier_wait();
 }
@@ -539,9 +704,8 @@ template <int XT, int V>
 __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const GroupNormArgs a) {
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint8_t smem[];
-  float2* own = reinterpret_cast<float2*>(smem);  // [range_groups] of this block
-  float* sums = reinterpret_cast<float*>(own + a.range_groups);  // [range_groups]
-  float* scratch = sums + a.range_groups;
+  float* scratch = reinterpret_cast<float*>(smem);
+  Stat* own = reinterpret_cast<Stat*>(scratch + (V + 2) * kGnThreads);  // of this block
   const uint32_t unit = blockIdx.x / static_cast<uint32_t>(a.blocks);
   const int block = static_cast<int>(blockIdx.x - unit * a.blocks);
   const int64_t image = unit / static_cast<uint32_t>(a.ranges);
@@ -553,6 +717,9 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const G
   const int from = block * a.share;
   const int count = max(0, min(a.pixels, from + a.share) - from);
   const int64_t p0 = image * a.pixels + from;
+  // the groups' values are on their way while the pixels are read
+  const float own_base =
+      threadIdx.x < a.range_groups ? group_base<XT>(a, r, image, threadIdx.x) : 0.0f;
   Running<V> run;
   // more columns than threads: the range is one group
   for (int at = col; row < rows && row < count && at < all; at += cols) {
@@ -567,75 +734,52 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const G
       for (int e = 0; e < K * kGnBatch; ++e, from_x += step) {
         it[e] = load_item<XT, V>(a.x, from_x, a.c_store);
       }
-#pragma unroll
-      for (int k = 0; k < K; ++k) {
-        Pairs<V> f[kGnBatch];
-#pragma unroll
-        for (int e = 0; e < kGnBatch; ++e) f[e] = item_pairs<XT, V>(it[k * kGnBatch + e]);
-        run.add(f);
-      }
+      run.template add<K * kGnBatch>([&](int e) { return item_pairs<XT, V>(it[e]); });
     }
     for (; left > 0; --left, from_x += step) {
-      run.add(item_pairs<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store)));
+      const Pairs<V> f = item_pairs<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store));
+      run.template add<1>([&](int) { return f; });
     }
   }
   // the second kernel may be launched; it waits for this one's end
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // the block's mean of each group, then each channel's squares about it
-  const int group_channels = all > cols ? cols * V : r.group_channels;
-  Pairs<V> sum = run.mean;
-  const uint64_t seen = pair_of(static_cast<float>(run.n), static_cast<float>(run.n));
-#pragma unroll
-  for (int i = 0; i < Pairs<V>::kCount; ++i) sum.p[i] = mul2(sum.p[i], seen);
-  group_sums<V>(sum, cols, rows, group_channels, a.range_groups, scratch, sums);
-  const float inv = 1.0f / (static_cast<float>(count) * static_cast<float>(r.group_channels));
-  int g = col * V / group_channels, inner = col * V - g * group_channels;
-  float v[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const float d = run.mean[e] - sums[min(g, a.range_groups - 1)] * inv;
-    v[e] = run.n > 0 ? fmaf(d * d, static_cast<float>(run.n), run.m2[e]) : 0.0f;
-    if (++inner == group_channels) {
-      inner = 0;
-      ++g;
-    }
+  const Columns<V> columns(cols, rows, all, count, all > cols ? cols * V : r.group_channels,
+                           a.range_groups,
+                           static_cast<float>(count) * static_cast<float>(r.group_channels));
+  for (int g = threadIdx.x; g < a.range_groups; g += kGnThreads) {
+    own[g].mean = g < kGnThreads ? own_base : group_base<XT>(a, r, image, g);
   }
-  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) own[i].x = sums[i] * inv;
   __syncthreads();
-  sum.set(v);
-  group_sums<V>(sum, cols, rows, group_channels, a.range_groups, scratch, sums);
-  for (int i = threadIdx.x; i < a.range_groups; i += kGnThreads) own[i].y = sums[i];
+  Pairs<V> base;
+  {
+    const int first = all > cols ? 0 : col * V / r.group_channels;
+    base = group_bases<V>(own, a.range_groups, r.group_channels, first,
+                          col * V - first * r.group_channels);
+  }
+  Pairs<V> mean = run.mean(base);
+  if (run.n == 0) mean.zero();
+  join_threads<V>(mean, run.m2, columns, scratch, own);
   // A cluster's blocks are joined here, so that the second kernel's blocks,
   // which each join them all, find few parts: [unit][group][part].
   cg::cluster_group cluster = cg::this_cluster();
-  const int size = static_cast<int>(cluster.num_blocks());
+  const int size_of_cluster = static_cast<int>(cluster.num_blocks());
   cluster.sync();
-  const int part = block / size, first_pixel = part * a.part_share;
-  const int pixels = min(a.pixels, first_pixel + a.part_share) - first_pixel;
+  const int part = block / size_of_cluster;
+  const int pixels = min(a.pixels, (part + 1) * a.part_share) - part * a.part_share;
   for (int i = static_cast<int>(cluster.block_rank()) * kGnThreads + threadIdx.x;
-       i < a.range_groups; i += kGnThreads * size) {
-    float s = 0.0f, q = 0.0f;
-    float2 o[kGnCluster];
+       i < a.range_groups; i += kGnThreads * size_of_cluster) {
+    Stat o[kGnCluster];
 #pragma unroll
     for (int k = 0; k < kGnCluster; ++k) {
-      o[k] = k < size ? *cluster.map_shared_rank(own + i, k) : make_float2(0.0f, 0.0f);
+      o[k] = *cluster.map_shared_rank(own + i, min(k, size_of_cluster - 1));
     }
-#pragma unroll
-    for (int k = 0; k < kGnCluster; ++k) {
-      const int w = min(pixels, (k + 1) * a.share) - k * a.share;
-      if (k < size && w > 0) s += static_cast<float>(w) * o[k].x;
-    }
-    const float mu = s / static_cast<float>(pixels);
-#pragma unroll
-    for (int k = 0; k < kGnCluster; ++k) {
-      const int w = min(pixels, (k + 1) * a.share) - k * a.share;
-      const float d = o[k].x - mu;
-      if (k < size && w > 0) {
-        q += o[k].y + static_cast<float>(w) * static_cast<float>(r.group_channels) * d * d;
-      }
+    Stat part_stat = o[0];
+    if (size_of_cluster > 1) {  // kGnCluster
+      part_stat = join_blocks(kGnCluster, a.share, pixels, r.group_channels,
+                              [&](int k) { return o[k]; });
     }
     a.partial[(static_cast<int64_t>(unit) * a.range_groups + i) * a.parts + part] =
-        make_float2(mu, q);
+        make_float4(part_stat.mean, part_stat.rest, part_stat.squares, 0.0f);
   }
   cluster.sync();  // no block leaves while another reads its statistics
 }
@@ -645,10 +789,9 @@ __global__ void __launch_bounds__(kGnThreads, 2) group_norm_stats_kernel(const G
 // kernel's blocks, all on the GPU at once, read the ends last, so L2 holds them.
 template <int XT, int YT, int V, int ACT>
 __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 : 4)
-    group_norm_apply_kernel(const GroupNormArgs a,
-                                                                      int apply_blocks) {
+    group_norm_apply_kernel(const GroupNormArgs a, int apply_blocks) {
   extern __shared__ __align__(16) uint8_t smem[];
-  float2* stat = reinterpret_cast<float2*>(smem);
+  Stat* stat = reinterpret_cast<Stat*>(smem);
   const uint32_t unit = blockIdx.x / static_cast<uint32_t>(apply_blocks);
   const int block = static_cast<int>(blockIdx.x - unit * apply_blocks);
   const int64_t image = unit / static_cast<uint32_t>(a.ranges);
@@ -657,28 +800,35 @@ __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 :
   const int lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // until the statistics are written
   for (int g = threadIdx.x >> 5; g < a.range_groups; g += kGnThreads / 32) {
-    const float2* p = a.partial + (static_cast<int64_t>(unit) * a.range_groups + g) * a.parts;
-    // up to 64 parts stay in registers between the mean and the squares
-    const float2 mine[2] = {lane < a.parts ? p[lane] : make_float2(0.0f, 0.0f),
-                            lane + 32 < a.parts ? p[lane + 32] : make_float2(0.0f, 0.0f)};
+    const float4* p = a.partial + (static_cast<int64_t>(unit) * a.range_groups + g) * a.parts;
+    // up to 64 parts stay in registers between the means and the squares
+    const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const float4 mine[2] = {lane < a.parts ? p[lane] : none,
+                            lane + 32 < a.parts ? p[lane + 32] : none};
+    auto part = [&](int k, int i) {
+      const float4 v = i == 0 ? mine[0] : i == 1 ? mine[1] : p[k];
+      return Stat{v.x, v.y, v.z};
+    };
     auto pixels_of = [&](int k) {
       return static_cast<float>(max(0, min(a.pixels, (k + 1) * a.part_share) - k * a.part_share));
     };
     float s = 0.0f, q = 0.0f;
     for (int k = lane, i = 0; k < a.parts; k += 32, ++i) {
-      if (pixels_of(k) > 0.0f) s += pixels_of(k) * (i == 0 ? mine[0] : i == 1 ? mine[1] : p[k]).x;
+      if (pixels_of(k) > 0.0f) s = fmaf(pixels_of(k), part(k, i).rest, s);
     }
-    const float mu = warp_sum(s) / static_cast<float>(a.pixels);
+    const float mean = warp_sum(s) / static_cast<float>(a.pixels);
     for (int k = lane, i = 0; k < a.parts; k += 32, ++i) {
-      const float2 o = i == 0 ? mine[0] : i == 1 ? mine[1] : p[k];
-      const float d = o.x - mu;
+      const Stat o = part(k, i);
+      const float d = o.rest - mean;
       if (pixels_of(k) > 0.0f) {
-        q += o.y + pixels_of(k) * static_cast<float>(r.group_channels) * d * d;
+        q += o.squares + pixels_of(k) * static_cast<float>(r.group_channels) * d * d;
       }
     }
     q = warp_sum(q);
-    const float size = static_cast<float>(a.pixels) * static_cast<float>(r.group_channels);
-    if (lane == 0) stat[g] = make_float2(mu, 1.0f / sqrtf(q / size + a.eps));
+    if (lane == 0) {  // lane 0 holds a part
+      const float size = static_cast<float>(a.pixels) * static_cast<float>(r.group_channels);
+      stat[g] = finished({mine[0].x, mean, q}, size, a.eps);
+    }
   }
   __syncthreads();
   const int share = (a.pixels + apply_blocks - 1) / apply_blocks;
@@ -692,8 +842,8 @@ __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 :
     if (row >= rows || row >= count) continue;
     const int c = r.c0 + col * V;
     const int first = col * V / r.group_channels;
-    Pairs<V> mul, add;
-    channel_affine<V>(a, c, first, col * V - first * r.group_channels, stat, &mul, &add);
+    Affine<V> affine;
+    channel_affine<V>(a, c, first, col * V - first * r.group_channels, stat, &affine);
     constexpr int K = ACT == kActGelu || XT == IE_DT_BF16X2 ? 2 : 4;
     const int64_t x_step = -static_cast<int64_t>(rows) * channel_at<XT>(1, a.c_store, 0);
     const int64_t y_step = -static_cast<int64_t>(rows) * channel_at<YT>(1, a.c_store, 0) *
@@ -710,12 +860,12 @@ __global__ void __launch_bounds__(kGnThreads, V == 8 && XT == IE_DT_BF16X2 ? 2 :
       }
 #pragma unroll
       for (int e = 0; e < K; ++e, y += y_step) {
-        finish_item<YT, V, ACT>(a, item_pairs<XT, V>(it[e]), mul, add, y, a.c - c);
+        finish_item<YT, V, ACT>(a, item_pairs<XT, V>(it[e]), affine, y, a.c - c);
       }
     }
     for (; left > 0; --left, from_x += x_step, y += y_step) {
-      finish_item<YT, V, ACT>(a, item_pairs<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store)), mul,
-                              add, y, a.c - c);
+      finish_item<YT, V, ACT>(a, item_pairs<XT, V>(load_item<XT, V>(a.x, from_x, a.c_store)),
+                              affine, y, a.c - c);
     }
   }
 }

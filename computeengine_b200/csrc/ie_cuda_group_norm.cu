@@ -54,6 +54,8 @@ int64_t item_bytes(int x_type, int v) {
   return int64_t{v} * element_bytes(x_type) * (x_type == IE_DT_BF16X2 ? 2 : 1);
 }
 
+int64_t scratch_bytes(int v) { return int64_t{v + 2} * kGnThreads * 4; }
+
 struct Plan {
   int v = 1;
   bool cluster = false;
@@ -93,7 +95,7 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
     if (cols > kGnThreads) return int64_t{1} << 40;
     const int64_t rows = kGnThreads / cols;
     return ceil_div(ceil_div(pixels, blocks), rows) * kGnThreads * item_bytes(d->x_type, v) +
-           (v + 1) * kGnThreads * 4 + (20 + 8 * blocks) * g + 32;
+           scratch_bytes(v) + static_cast<int64_t>(sizeof(Stat)) * (2 + blocks) * g + 16;
   };
   auto fits = [&](int64_t g, int blocks) {
     const int64_t share = ceil_div(pixels, blocks);
@@ -153,9 +155,9 @@ Plan plan_for(const ie_group_norm_desc* d, int v) {
   p.apply_blocks = static_cast<int>(std::max<int64_t>(
       1, std::min(std::max(4 * kSms / units, ceil_div(pixels * channels * (xb + yb), 262144)),
                   ceil_div(pixels, 4 * rows))));
-  p.smem = (v + 1) * kGnThreads * 4 + 12 * p.range_groups + 8;
+  p.smem = scratch_bytes(v) + static_cast<int64_t>(sizeof(Stat)) * p.range_groups;
   p.workspace =
-      units * (p.blocks / p.joined) * p.range_groups * static_cast<int64_t>(sizeof(float2));
+      units * (p.blocks / p.joined) * p.range_groups * static_cast<int64_t>(sizeof(float4));
   return p;
 }
 
@@ -214,7 +216,7 @@ template <int XT, int YT, int V, int ACT>
 int launch_two(const GroupNormArgs& a, const Plan& p, int64_t images, cudaStream_t s) {
   auto stats = group_norm_stats_kernel<XT, V>;
   auto apply = group_norm_apply_kernel<XT, YT, V, ACT>;
-  const int64_t apply_smem = 8 * p.range_groups;
+  const int64_t apply_smem = static_cast<int64_t>(sizeof(Stat)) * p.range_groups;
   int rc = allow_smem(stats, p.smem);
   if (rc == IE_OK) rc = allow_smem(apply, apply_smem);
   const int64_t units = images * p.ranges;
@@ -330,7 +332,7 @@ int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const
     a.cols[last] = static_cast<int>(ceil_div(stored, p.v));
     a.rows[last] = std::max(1, kGnThreads / a.cols[last]);
   }
-  a.partial = static_cast<float2*>(workspace);
+  a.partial = static_cast<float4*>(workspace);
   return launch(desc->x_type, desc->y_type, desc->act, a, p, desc->n, as_stream(stream));
 }
 
