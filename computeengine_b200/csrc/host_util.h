@@ -43,6 +43,12 @@ inline int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+// A pointer (or NULL) to elements of `bytes` bytes; the GPU faults on others.
+inline int check_aligned(const void* p, size_t bytes, const char* what) {
+  if (reinterpret_cast<uintptr_t>(p) % bytes == 0) return IE_OK;
+  return fail(IE_INVALID_ARGUMENT, "%s must be %zu-byte aligned", what, bytes);
+}
+
 inline int check_launch(const char* what) {
   ++g_launches;
   g_packed_weights_stream.store(0, std::memory_order_relaxed);

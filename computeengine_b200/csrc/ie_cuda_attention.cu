@@ -381,11 +381,23 @@ size_t ie_cuda_attention_workspace_bytes(const ie_attention_desc* desc,
 int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* mask, const void* q,
                       const void* k, const void* v, void* o, float* lse, void* workspace,
                       size_t workspace_bytes, void* stream) {
-  const int rc = check_attention(desc, mask);
+  int rc = check_attention(desc, mask);
   if (rc != IE_OK) return rc;
   if (q == nullptr || k == nullptr || v == nullptr || o == nullptr) {
     return fail(IE_INVALID_ARGUMENT, "null tensor or buffer");
   }
+  for (const void* p : {q, k, v, static_cast<const void*>(o)}) {
+    if (rc == IE_OK) rc = check_aligned(p, 2, "Attention q, k, v and o");
+  }
+  if (rc == IE_OK) rc = check_aligned(lse, 4, "Attention lse");
+  if (mask != nullptr) {
+    const void* given[] = {mask->kv_lens, mask->prefix_lens, mask->q_offsets, mask->kv_offsets,
+                           mask->slopes};
+    for (const void* p : given) {
+      if (rc == IE_OK) rc = check_aligned(p, 4, "Attention lengths, offsets and slopes");
+    }
+  }
+  if (rc != IE_OK) return rc;
   const bool few = few_rows(desc, mask);
   const bool kv_tma =
       tma_readable(k, desc->head_dim, desc->kv_len, desc->kv_heads, desc->batch, desc->k_stride) &&

@@ -291,9 +291,14 @@ size_t ie_cuda_group_norm_workspace_bytes(const ie_group_norm_desc* desc) {
 int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const float* gamma,
                             const float* beta, void* y, void* workspace, size_t workspace_bytes,
                             void* stream) {
-  const int rc = check_group_norm(desc);
+  int rc = check_group_norm(desc);
   if (rc != IE_OK) return rc;
   if (x == nullptr || y == nullptr) return fail(IE_INVALID_ARGUMENT, "null tensor or buffer");
+  rc = check_aligned(x, element_bytes(desc->x_type), "GroupNorm x");
+  if (rc == IE_OK) rc = check_aligned(y, element_bytes(desc->y_type), "GroupNorm y");
+  if (rc == IE_OK) rc = check_aligned(gamma, 4, "GroupNorm gamma");
+  if (rc == IE_OK) rc = check_aligned(beta, 4, "GroupNorm beta");
+  if (rc != IE_OK) return rc;
   if (x == y && desc->x_type != desc->y_type) {
     return fail(IE_INVALID_ARGUMENT, "GroupNorm in place needs equal element types");
   }

@@ -136,7 +136,7 @@ int ie_rotary_plan_init(const ie_rotary_desc* desc, ie_rotary_plan* plan) {
 int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const void* x,
                    const void* positions, void* y, void* stream) {
   int pairs = 0;
-  const int rc = check_head_layout(desc, &pairs);
+  int rc = check_head_layout(desc, &pairs);
   if (rc != IE_OK) return rc;
   if (plan == nullptr || x == nullptr || y == nullptr || positions == nullptr) {
     return fail(IE_INVALID_ARGUMENT, "null tensor or buffer");
@@ -161,6 +161,10 @@ int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const
   if (desc->pos_bits != 32 && desc->pos_bits != 64) {
     return fail(IE_INVALID_ARGUMENT, "positions have 32 or 64 bits");
   }
+  rc = check_aligned(x, element_bytes(desc->x_type), "Rotary x");
+  if (rc == IE_OK) rc = check_aligned(y, element_bytes(desc->y_type), "Rotary y");
+  if (rc == IE_OK) rc = check_aligned(positions, desc->pos_bits / 8, "Rotary positions");
+  if (rc != IE_OK) return rc;
   if (desc->x_token_stride < 0 || desc->x_head_stride < 0 || desc->y_token_stride < 0 ||
       desc->y_head_stride < 0 || desc->pos_axis_stride < 0) {
     return fail(IE_INVALID_ARGUMENT, "strides must not be negative");

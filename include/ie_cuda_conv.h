@@ -441,7 +441,8 @@ int ie_cuda_gemm_f32(int64_t m, int64_t n, int64_t k, int32_t trans_a, int32_t t
  * these read, and their BF16X2 outputs are the split input
  * ie_cuda_conv2d_bf16x3 reads.  Calls are asynchronous on the stream, keep
  * nothing between calls and can be captured; tensors live on the current
- * device.  Inputs may not overlap outputs unless an entry says so. */
+ * device, at addresses aligned to their elements (others are refused).  Inputs may
+ * not overlap outputs unless an entry says so. */
 
 /* Element types.  IE_DT_BF16X2 is the split form of IE_Y_BF16X2_NHWC: bf16
  * [hi plane | lo plane] per pixel, standing for hi + lo. */
@@ -586,7 +587,8 @@ typedef struct ie_attention_mask {
  * that are put away in between.  Its contents need not be kept; calls that
  * overlap on the GPU need one each.
  * Full speed: q, k and v 16-byte aligned, head_dim a multiple of 8, strides
- * multiples of 8 and not 0; other tensors take a slower kernel. */
+ * multiples of 8 and not 0; others, aligned to their elements, take a slower
+ * kernel. */
 size_t ie_cuda_attention_workspace_bytes(const ie_attention_desc* desc,
                                          const ie_attention_mask* mask);
 int ie_cuda_attention(const ie_attention_desc* desc, const ie_attention_mask* mask, const void* q,
