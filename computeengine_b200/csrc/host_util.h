@@ -49,6 +49,26 @@ inline int check_aligned(const void* p, size_t bytes, const char* what) {
   return fail(IE_INVALID_ARGUMENT, "%s must be %zu-byte aligned", what, bytes);
 }
 
+// Whether rows of `width` elements at the given strides may share an element: no
+// unless each stride, in ascending order, spans all that lies below it.
+template <int N>
+bool rows_overlap(const int64_t (&extent)[N], const int64_t (&stride)[N], int64_t width) {
+  bool taken[N] = {};
+  int64_t span = width;
+  for (int i = 0; i < N; ++i) {
+    int next = -1;
+    for (int k = 0; k < N; ++k) {
+      if (!taken[k] && extent[k] > 1 && (next < 0 || stride[k] < stride[next])) next = k;
+    }
+    if (next < 0) break;
+    taken[next] = true;
+    if (stride[next] < span) return true;
+    if (extent[next] - 1 > (INT64_MAX - span) / stride[next]) return true;  // no such address
+    span += stride[next] * (extent[next] - 1);
+  }
+  return false;
+}
+
 inline int check_launch(const char* what) {
   ++g_launches;
   g_packed_weights_stream.store(0, std::memory_order_relaxed);

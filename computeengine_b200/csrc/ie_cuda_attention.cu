@@ -41,16 +41,18 @@ int check_attention(const ie_attention_desc* d, const ie_attention_mask* m) {
     return fail(IE_INVALID_ARGUMENT, "Attention scale and softcap must be finite, softcap not "
                                      "negative");
   }
-  const int64_t extent[3] = {d->batch, d->q_len, d->q_heads};
   for (int i = 0; i < 3; ++i) {
     if (d->q_stride[i] < 0 || d->k_stride[i] < 0 || d->v_stride[i] < 0 || d->o_stride[i] < 0) {
       return fail(IE_INVALID_ARGUMENT, "strides must not be negative");
     }
-    if (extent[i] > 1 && d->o_stride[i] < d->head_dim) {
-      return fail(IE_INVALID_ARGUMENT, "the rows of o overlap");
-    }
   }
-  if (d->o_type == IE_DT_BF16X2 && (d->o_stride[1] % 2 != 0 || d->o_stride[1] < 2 * d->head_dim)) {
+  const bool split = d->o_type == IE_DT_BF16X2;
+  if (rows_overlap({d->batch, d->q_len, d->q_heads, split ? 2 : 1},
+                   {d->o_stride[0], d->o_stride[1], d->o_stride[2], d->o_stride[1] / 2},
+                   d->head_dim)) {
+    return fail(IE_INVALID_ARGUMENT, "the rows of o overlap");
+  }
+  if (split && d->o_stride[1] % 2 != 0) {
     return fail(IE_INVALID_ARGUMENT, "split output: the token stride holds both planes");
   }
   if (m != nullptr) {

@@ -169,8 +169,8 @@ int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const
       desc->y_head_stride < 0 || desc->pos_axis_stride < 0) {
     return fail(IE_INVALID_ARGUMENT, "strides must not be negative");
   }
-  if ((desc->tokens > 1 && desc->y_token_stride < desc->head_dim) ||
-      (desc->heads > 1 && desc->y_head_stride < desc->head_dim)) {
+  if (rows_overlap({desc->tokens, int64_t{desc->heads}},
+                   {desc->y_token_stride, desc->y_head_stride}, desc->head_dim)) {
     return fail(IE_INVALID_ARGUMENT, "the tokens or heads of y overlap");
   }
   const bool in_place = x == y;
