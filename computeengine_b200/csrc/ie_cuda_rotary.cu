@@ -33,7 +33,6 @@ int check_head_layout(const ie_rotary_desc* d, int* pairs) {
   if (d->freq != IE_ROTARY_FREQ_SHARED && d->freq != IE_ROTARY_FREQ_PER_AXIS) {
     return fail(IE_INVALID_ARGUMENT, "bad rotary frequencies");
   }
-
   if (!(d->theta > 0.0) || std::isinf(d->theta)) {
     return fail(IE_INVALID_ARGUMENT, "Rotary theta must be positive and finite");
   }
@@ -115,11 +114,12 @@ int ie_rotary_plan_init(const ie_rotary_desc* desc, ie_rotary_plan* plan) {
       const long double e = desc->freq == IE_ROTARY_FREQ_SHARED
                                 ? static_cast<long double>(i) / pairs
                                 : static_cast<long double>(j) / desc->section[a];
-      long double t = std::pow(static_cast<long double>(desc->theta), -e) / kTwoPi;
-      t -= std::floor(t);  // whole turns per position change nothing
-      long double fixed = std::round(t * 0x1p64L);
-      if (fixed >= 0x1p64L) fixed = 0.0L;
-      plan->turns[i] = static_cast<uint64_t>(fixed);
+      const long double t = std::pow(static_cast<long double>(desc->theta), -e) / kTwoPi;
+      if (!(t < 1.0L)) {  // above, long double has no 2^-64 turns left
+        return fail(IE_UNSUPPORTED, "Rotary frequencies are below one turn per position");
+      }
+      const long double fixed = std::round(t * 0x1p64L);
+      plan->turns[i] = fixed < 0x1p64L ? static_cast<uint64_t>(fixed) : 0;  // a whole turn
       plan->axis[i] = static_cast<uint8_t>(a);
     }
     plan->section[a] = desc->section[a];

@@ -495,7 +495,9 @@ int ie_cuda_group_norm_nhwc(const ie_group_norm_desc* desc, const void* x, const
  *                            of pairs of the axes before a
  * Angles are taken modulo one turn in fixed point (frequencies rounded to
  * 2^-64 turns), so far positions lose nothing: at position 2^32 an angle is
- * still within 2^-32 turns before its sine and cosine are taken in fp32. */
+ * still within 2^-32 turns before its sine and cosine are taken in fp32.
+ * Frequencies of a turn per position and more (theta below 0.16 or so) are
+ * refused: IE_UNSUPPORTED. */
 enum { IE_ROTARY_PAIRS = 0, IE_ROTARY_HALVES = 1, IE_ROTARY_AXIS_HALVES = 2 };
 enum { IE_ROTARY_FREQ_SHARED = 0, IE_ROTARY_FREQ_PER_AXIS = 1 };
 
