@@ -402,14 +402,34 @@ _DTYPES = {torch.float32: _lib.IE_DT_F32, torch.bfloat16: _lib.IE_DT_BF16,
 
 def _number(attrs, key, default):
     v = attrs.get(key, default)
-    if isinstance(v, bool) or not isinstance(v, (int, float)) or not math.isfinite(v):
+    ok = not isinstance(v, bool) and isinstance(v, (int, float))
+    try:
+        ok = ok and math.isfinite(v)
+    except OverflowError:  # an int beyond every float
+        ok = False
+    if not ok:
         return default, Status.error(Code.InvalidArgument, f"attribute '{key}' must be a finite number")
     return float(v), OK
 
 
+def _number_f32(attrs, key, default):
+    """A number that the descriptors hold in fp32: neither infinite nor zero there."""
+    v, st = _number(attrs, key, default)
+    held = _lib.C.c_float(v).value
+    if st and (not math.isfinite(held) or (held == 0.0) != (v == 0.0)):
+        st = Status.error(Code.InvalidArgument, f"attribute '{key}' is out of range: {v}")
+    return v, st
+
+
+def _int32(v, key) -> Status:
+    if -(1 << 31) <= v < 1 << 31:
+        return OK
+    return Status.error(Code.InvalidArgument, f"attribute '{key}' is out of range: {v}")
+
+
 def _choice(attrs, key, table, default):
     v = attrs.get(key, default)
-    if v not in table:
+    if not any(v is k or v == k for k in table):
         return None, Status.error(Code.InvalidArgument, f"unsupported {key}: {v}")
     return table[v], OK
 
@@ -449,10 +469,10 @@ class GroupNormOp(Op):
 
     def configure(self, attrs: dict) -> Status:
         g = attrs.get("groups")
-        if isinstance(g, bool) or not isinstance(g, int) or g <= 0:
+        if isinstance(g, bool) or not isinstance(g, int) or not 0 < g < 1 << 63:
             return Status.error(Code.InvalidArgument, "attribute 'groups' must be a positive int")
         self.groups = g
-        self.eps, st = _number(attrs, "epsilon", 1e-5)
+        self.eps, st = _number_f32(attrs, "epsilon", 1e-5)
         if st and self.eps < 0:
             st = Status.error(Code.InvalidArgument, "epsilon must not be negative")
         if not st:
@@ -522,6 +542,10 @@ class RotaryOp(Op):
             return st
         if not section or len(section) > 4:
             return Status.error(Code.InvalidArgument, "attribute 'section' must hold 1 to 4 ints")
+        for s in section:
+            st = _int32(s, "section")
+            if not st:
+                return st
         self.section = section
         self.layout, st = _choice(attrs, "layout", self.LAYOUTS, "HALVES")
         if not st:
@@ -535,6 +559,9 @@ class RotaryOp(Op):
         r = attrs.get("rot_heads")
         if r is not None and (isinstance(r, bool) or not isinstance(r, int)):
             return Status.error(Code.InvalidArgument, "attribute 'rot_heads' must be an int")
+        st = _int32(r or 0, "rot_heads")
+        if not st:
+            return st
         self.rot_heads, self.inverse = r, bool(attrs.get("inverse", False))
         self.dtype, st = _choice(attrs, "dtype", {None: None, **{d: d for d in _DTYPES}}, None)
         self._plans = {}
@@ -605,10 +632,10 @@ class AttentionOp(Op):
     def configure(self, attrs: dict) -> Status:
         self.scale = None
         if attrs.get("scale") is not None:
-            self.scale, st = _number(attrs, "scale", 1.0)
+            self.scale, st = _number_f32(attrs, "scale", 1.0)
             if not st:
                 return st
-        self.softcap, st = _number(attrs, "softcap", 0.0)
+        self.softcap, st = _number_f32(attrs, "softcap", 0.0)
         if st and self.softcap < 0:
             st = Status.error(Code.InvalidArgument, "softcap must not be negative")
         if not st:
