@@ -67,13 +67,6 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// 1 / x for 1 <= x, 0 for infinity.
-__device__ __forceinline__ float reciprocal(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // ---- cap * tanh(s / cap), in units of log2 e.  With u = s / cap:
 //   |u| <= kTanhLimit   s * (tanh(u) / u), the ratio a polynomial in u^2 (minimax
 //                       of tanh u with slope 1 at 0, absolute error below 2.7e-7)

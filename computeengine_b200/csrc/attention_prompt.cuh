@@ -116,29 +116,10 @@ __device__ __forceinline__ bool wait_ready(uint64_t* bar, uint32_t parity, volat
   return mbar_wait_warp(bar, parity, abort_flag, site, limit_ns);
 }
 
-// ---- two fp32 values at once (one instruction each on sm_100)
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ void unpair(uint64_t v, float* a, float* b) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(*a), "=f"(*b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
+  const float2 f = floats_of(v);
+  *a = f.x;
+  *b = f.y;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;

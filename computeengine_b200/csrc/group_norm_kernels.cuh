@@ -48,13 +48,6 @@ constexpr int kGnCluster = 4;  // blocks of the statistics kernel joined before 
 // Kinds of activation: a clamp to [low, high] (none, ReLU, ReLU6), SiLU, GELU.
 enum { kActClamp = 0, kActSilu = 1, kActGelu = 2 };
 
-// 1 / x for 1 <= x, 0 from 2^126 on.
-__device__ __forceinline__ float reciprocal(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 template <int ACT, int V>
 __device__ __forceinline__ void activate(float (&v)[V], float low, float high) {
   if constexpr (ACT == kActClamp) {
@@ -120,33 +113,6 @@ __device__ __forceinline__ Item<T, V> load_item(const void* x, int64_t at, int c
   i.v = load_bytes<Item<T, V>::kBytes>(p);
   if constexpr (T == IE_DT_BF16X2) i.lo = load_bytes<Item<T, V>::kBytes>(p + 2 * c_store);
   return i;
-}
-
-// Two fp32 values in one register pair, two operations per instruction (sm_100).
-__device__ __forceinline__ uint64_t pair_of(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 floats_of(uint64_t v) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-  return f;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
 }
 
 // V channels as pairs; V == 1: the second of the one pair is zero.

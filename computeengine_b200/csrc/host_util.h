@@ -219,6 +219,9 @@ inline int encode_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dty
 // Reads and clears the device error word of ie_cuda_attention.cu's kernels.
 int take_attention_error(unsigned int* code);
 
+// What the sizes of plans count with, so that they do not depend on the device.
+constexpr int64_t kSms = 148;
+
 inline int num_sms() {
   static int sms = [] {
     int dev = 0, v = 148;

@@ -122,8 +122,6 @@ bool tma_readable(const void* p, int64_t head_dim, int64_t len, int64_t heads, i
   return true;
 }
 
-constexpr int64_t kSms = 148;
-
 // Shares of each sequence's keys, their partial results in the workspace.
 size_t share_bytes(const ie_attention_desc* d, int splits) {
   if (splits <= 1) return 0;

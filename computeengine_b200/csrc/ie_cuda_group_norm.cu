@@ -48,7 +48,6 @@ int check_group_norm(const ie_group_norm_desc* d) {
 
 constexpr int64_t ceil_div(int64_t v, int64_t m) { return (v + m - 1) / m; }
 
-constexpr int64_t kSms = 148;
 constexpr int64_t kSmemPerSm = 227 * 1024;
 int64_t item_bytes(int x_type, int v) {
   return int64_t{v} * element_bytes(x_type) * (x_type == IE_DT_BF16X2 ? 2 : 1);

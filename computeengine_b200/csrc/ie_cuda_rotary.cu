@@ -211,7 +211,7 @@ int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const
   // Tokens per block: about eight units a thread, as long as that leaves four
   // blocks per SM; heads are shared out among blocks when there are fewer
   // tokens than SMs (one token per block then).
-  constexpr int64_t kSms = 148, kMaxItems = 1 << 15;
+  constexpr int64_t kMaxItems = 1 << 15;
   const int64_t units = std::max<int64_t>(1, int64_t{desc->rot_heads} * (pairs / w));
   int64_t block_tokens = std::min<int64_t>(8, std::max<int64_t>(1, 2048 / units));
   block_tokens = std::max<int64_t>(1, std::min(block_tokens, desc->tokens / (4 * kSms)));

@@ -48,6 +48,12 @@ __device__ __forceinline__ float2 rotary_angle(const RotaryArgs& a, int64_t t, i
   return make_float2(c, a.inverse ? -s : s);
 }
 
+// Place of one of a unit's 2 W table values (cosines, then sines).
+template <int W>
+__device__ __forceinline__ int table_at(int units, int unit, int value) {  // of 2 W values
+  return W == 1 ? 2 * unit + value : ((value >> 2) * units + unit) * 4 + (value & 3);
+}
+
 // One block takes a few tokens (and, when there are few of them, a share of
 // their heads): the cosines and sines of a token are taken once for all its
 // heads and kept in shared memory, then every thread rotates W pairs at a
@@ -62,11 +68,6 @@ __device__ __forceinline__ float2 rotary_angle(const RotaryArgs& a, int64_t t, i
 // W: pairs per unit; divides the layout's runs of pairs, the elements that are
 // not rotated and all strides, and the tensors are aligned to it.
 // CW: elements per unit of the heads that are only converted.
-template <int W>
-__device__ __forceinline__ int table_at(int units, int unit, int value) {  // of 2 W values
-  return W == 1 ? 2 * unit + value : ((value >> 2) * units + unit) * 4 + (value & 3);
-}
-
 template <int XT, int YT, int W, int CW>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryArgs a) {
   extern __shared__ __align__(16) float table[];  // [tokens of the block][2 pairs], unit offsets
