@@ -15,17 +15,18 @@
 // price is that S of 64 keys costs 49 cycles per 16 elements of the head where
 // half of one of 128 keys costs 32 (Q is read from shared memory for each), so a
 // head of 128 runs at most at 79% of the tensor core's rate.  With heads of 64
-// there is room for two blocks per SM instead.  Then the exponentials are what
-// takes longest (16 a cycle and SM); a polynomial on the FMA pipes for a quarter
-// of them changed nothing (113 to 121 us against 113 to 118 us for 4096 tokens,
-// 16 heads of 64).
+// there is room for two blocks per SM instead.  Then the exponentials are the
+// longest single part (16 a cycle and SM: 60 us of 113 to 126 us for 4096 tokens, 16
+// heads of 64); a polynomial on the FMA pipes for a quarter of them changed nothing.
 // Warps 0-3 and 4-7 hold the rows of the tiles, warps 8 and 9 issue their MMAs
 // (one thread for both tiles took about 2200 cycles a step, 1200 of them between
 // its waits and the MMAs), warp 10 the TMA loads of Q, K and V; it also
 // clears the rows of V behind the sequence's end (0 * NaN would reach O).  Warp 11
 // is idle: it completes the warpgroup that gives its registers away.
-// 4096 tokens, 16 heads of 128, no mask: 126 us, 1090 TFLOP/s; of 64: 126 us,
-// 543 TFLOP/s.
+// The weights are rounded to the 16-bit type, half a step of each, as the tensor
+// core takes them; their sum is that of the unrounded ones.
+// 4096 tokens, 16 heads of 128, no mask: 126 to 137 us, 1000 to 1090 TFLOP/s; of 64:
+// 113 to 126 us, 543 to 608 TFLOP/s.
 #pragma once
 
 #include "attention_common.cuh"

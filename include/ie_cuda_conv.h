@@ -546,7 +546,8 @@ int ie_cuda_rotary(const ie_rotary_desc* desc, const ie_rotary_plan* plan, const
  * to the query's sequence and, if causal, j <= p or j < prefix_lens. */
 typedef struct ie_attention_desc {
   int64_t batch, q_len, kv_len;
-  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* batch, token, head; elements */
+  int64_t q_stride[3], k_stride[3], v_stride[3], o_stride[3]; /* batch, token, head; elements;
+                                rows (and planes) of o may not overlap or interleave */
   int32_t q_heads, kv_heads; /* kv_heads divides q_heads */
   int32_t head_dim;          /* 1 .. 128, contiguous */
   int32_t type;              /* q, k, v: IE_DT_BF16 or IE_DT_F16 */
@@ -555,6 +556,9 @@ typedef struct ie_attention_desc {
   float scale;
   float softcap; /* 0: none */
 } ie_attention_desc;
+
+/* Scores, softmax and sums are fp32; the weights are rounded to the type of q, k and
+ * v, half a step of each, before they are multiplied with v. */
 
 /* Which keys a query sees; all pointers are device memory and may be NULL.
  *   kv_lens      [batch] keys of each sequence (0 .. kv_len), kv_len without it
