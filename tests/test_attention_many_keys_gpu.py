@@ -79,3 +79,53 @@ def test_growing_scores_over_many_keys(sq, document):
         run_attention(L, attention_desc(L, q, k, v, o, 2.0, cap), m, q, k, v, o, lse)
         assert not o.isnan().any()
         check_attention(o, lse, attention_64(q, k, v, 2.0, cap, **kw), q.dtype)
+
+
+@pytest.mark.parametrize("options", ["plain", "bias", "cap", "prefix", "cap bias"])
+@pytest.mark.parametrize("batch, sq, hq, hk, keys, dtype", [
+    (1, 130, 80, 1, 70001, "bfloat16"),    # blocks enough without shares
+    (3, 130, 30, 2, 66000, "float16"),     # the same over ragged lengths
+    (1, 130, 70, 1, 140000, "bfloat16"),   # two shares, each put away twice
+    (1, 40, 148, 2, 140000, "float16"),    # several heads in a tile
+])
+def test_long_keys_under_masks(batch, sq, hq, hk, keys, dtype, options):
+    """The first and last heads against 64 bits; the score's maximum moves along the
+    keys; a split output stands for the same values."""
+    import torch
+    from computeengine_b200 import _lib as L
+    from tests.token_ops import attention_64, check_attention, joined
+    g = torch.Generator(device="cuda").manual_seed(keys + sq)
+    dt, d = getattr(torch, dtype), 64
+    rand = lambda *shape: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    q, v = (rand(batch, sq, hq, d) * 2).to(dt), rand(batch, keys, hk, d).to(dt)
+    grow = torch.linspace(0.2, 1.5, keys, device="cuda")[None, :, None, None]
+    k = (rand(batch, keys, hk, d) * grow).to(dt)
+    slopes = 2.0 ** -(8.0 + 6.0 * torch.arange(1, hq + 1, device="cuda", dtype=torch.float32) / hq)
+    ints = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    kw = dict(causal=1)
+    if batch == 3:
+        kw.update(kv_lens=ints(keys, 40000, 100))
+    if "prefix" in options:
+        kw.update(prefix=ints(*[keys] * batch))
+    if "bias" in options:
+        kw.update(slopes=slopes)
+    cap = 40.0 if "cap" in options else 0.0
+    o, lse = torch.empty_like(q), torch.empty(batch, hq, sq, device="cuda")
+    m = attention_mask(L, **kw)
+    run_attention(L, attention_desc(L, q, k, v, o, d ** -0.5, cap), m, q, k, v, o, lse)
+    assert L.take_device_error() == 0
+    assert not o.isnan().any()
+    for h, c in ((0, 0), (hq - 1, hk - 1)):
+        part = dict(kw, slopes=slopes[h:h + 1]) if "bias" in options else kw
+        want = attention_64(q[:, :, h:h + 1], k[:, :, c:c + 1], v[:, :, c:c + 1], d ** -0.5, cap,
+                            **part)
+        check_attention(o[:, :, h:h + 1], lse[:, h:h + 1], want, dt)
+    if dt == torch.bfloat16:
+        two = torch.empty(batch, sq, 2 * hq * d, dtype=dt, device="cuda")
+        desc = attention_desc(L, q, k, v, o, d ** -0.5, cap, o_type=L.IE_DT_BF16X2)
+        for i, s in enumerate((sq * 2 * hq * d, 2 * hq * d, d)):
+            desc.o_stride[i] = s
+        run_attention(L, desc, m, q, k, v, two, None)
+        both = joined(two, hq * d, hq * d).reshape(o.shape)
+        # one rounding to bf16 apart, and the lo plane's own
+        assert ((both - o.double()).abs() <= (2.0 ** -8 + 2.0 ** -16) * both.abs() + 2.0 ** -126).all()
