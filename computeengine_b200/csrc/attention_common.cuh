@@ -94,6 +94,12 @@ __device__ __forceinline__ float tanh_ratio(float uu) {
   return fmaf(p, uu, 1.0f);
 }
 
+// Weights are 2^(score - maximum in use + this), at most 2^15: fp16 would otherwise
+// hold those below 2^-14 of the largest with fewer bits and none below 2^-25, which
+// many keys behind a heavy one add up to.  The factor cancels in o.
+template <int T>
+constexpr float kWeightShift = T == IE_DT_F16 ? 7.0f : 0.0f;
+
 __device__ __forceinline__ float max_nan(float a, float b) {
   float y;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));

@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
         }
         const float top = max_nan(max3(hi[0], hi[1], hi[2]), hi[3]);
         // The maximum in use moves only when it grew by more than 2^8: until then
-        // the weights stay below 256, which both 16-bit types hold as well as 1.
+        // the weights stay below 2^8 (fp16: 2^15), which the types hold as well as 1.
         float factor = 1.0f;
         const bool moved = !((top - m) * to_log2 <= 8.0f) && top != -INFINITY;
         if (moved) {
@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
             tmem_st_32x32b_x16(o_at + 16 * c, o);
           }
         }
-        const float base = m == -INFINITY ? 0.0f : m * to_log2;
+        const float base = m == -INFINITY ? 0.0f : m * to_log2 - kWeightShift<T>;
         const uint64_t to2 = pair_of(to_log2, to_log2), base2 = pair_of(-base, -base);
         uint64_t sum[2] = {0, 0};
         uint32_t p[32];
@@ -614,7 +614,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     if (ok) {
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const bool none = l == 0.0f;
-      const float lse = none ? -INFINITY : (m * to_log2 + log2f(l)) * 0.6931471805599453f;
+      const float lse =
+          none ? -INFINITY : (m * to_log2 + (log2f(l) - kWeightShift<T>)) * 0.6931471805599453f;
       if (valid) {
         if (a.splits > 1) {
           a.part_lse[part_at()] = lse;

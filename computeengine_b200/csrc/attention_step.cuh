@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
         moved[i] = !(t[i] - top[n][i] <= 8.0f) && t[i] != -INFINITY;
         factor[i] = moved[i] && top[n][i] != -INFINITY ? ex2(top[n][i] - t[i]) : 1.0f;
         if (moved[i]) top[n][i] = t[i];
-        base[i] = top[n][i] == -INFINITY ? 0.0f : top[n][i];
+        base[i] = top[n][i] == -INFINITY ? 0.0f : top[n][i] - kWeightShift<T>;
       }
       if (__any_sync(0xFFFFFFFFu, moved[0] || moved[1])) {
         sum[n][0] *= factor[0];
@@ -381,7 +381,8 @@ __global__ void __launch_bounds__(kStepThreads) attention_step_kernel(const Step
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t at = (int64_t{seq.batch} * a.q_heads + h) * a.q_len + pos;
-    const float lse = l == 0.0f ? -INFINITY : (base + log2f(l)) * 0.6931471805599453f;
+    const float lse =
+        l == 0.0f ? -INFINITY : (base + (log2f(l) - kWeightShift<T>)) * 0.6931471805599453f;
     const int64_t oo = seq.batch * a.o_stride[0] + pos * a.o_stride[1] + h * a.o_stride[2];
     if (lane == 0) {
       if (a.splits > 1) {
