@@ -211,26 +211,28 @@ __device__ __forceinline__ void store_item(void* y, int64_t at, int c_store, con
 // and of their squares lose no more than the squares of the means' differences.
 template <int V>
 struct Running {
-  Pairs<V> pivot, rest, m2;
+  Pairs<V> pivot, rest, m2, m2_rest;
   int n = 0;
 
   __device__ __forceinline__ Running() {
     pivot.zero();
     rest.zero();
     m2.zero();
+    m2_rest.zero();
   }
   // The next K pixels, the k-th of them at(k).
   template <int K, class At>
   __device__ __forceinline__ void add(const At& at) {
     if (n == 0) pivot = at(0);
     const Pairs<V> minus = pivot.times(-1.0f);
-    Pairs<V> sum;
+    Pairs<V> sum, squares;
     sum.zero();
+    squares.zero();
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       const Pairs<V> d = at(k).plus(minus);
       sum.add(d);
-      m2.add_squares(d);
+      squares.add_squares(d);
     }
     const float share = static_cast<float>(K) / static_cast<float>(n + K);
     const float weight = static_cast<float>(n) * share;
@@ -240,8 +242,12 @@ struct Running {
     for (int i = 0; i < Pairs<V>::kCount; ++i) {
       const uint64_t mean = mul2(sum.p[i], inv);  // of the batch, as difference to pivot
       const uint64_t d = fma2(rest.p[i], minus1, mean);
-      const uint64_t squares = fma2(mul2(sum.p[i], minus1), mean, m2.p[i]);
-      m2.p[i] = fma2(mul2(d, d), weight2, squares);
+      const uint64_t about_mean = fma2(mul2(sum.p[i], minus1), mean, squares.p[i]);
+      // what the running sum of squares cuts off each time goes into the next term
+      const uint64_t term = add2(fma2(mul2(d, d), weight2, about_mean), m2_rest.p[i]);
+      const uint64_t total = add2(m2.p[i], term);
+      m2_rest.p[i] = add2(fma2(total, minus1, m2.p[i]), term);
+      m2.p[i] = total;
       const uint64_t moved = fma2(d, share2, rest.p[i]);
       const uint64_t to = add2(pivot.p[i], moved);
       rest.p[i] = add2(fma2(to, minus1, pivot.p[i]), moved);
