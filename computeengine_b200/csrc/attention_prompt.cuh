@@ -42,7 +42,8 @@ constexpr int kStep = 64;      // keys per step
 // The tensor core cuts off what lies below its fp32 sum's last place.  For keys
 // of equal weight that was 0.6% of o after 2^20 of them: so after this many steps
 // (2^15 keys, 0.02%) O is put away, added to what was put away before (in fp32,
-// rounded to nearest), and begins anew.
+// rounded to nearest), and begins anew.  So does the weights' sum: additions of equal
+// weights to a long sum all round the same way.
 constexpr int kFold = 512;
 
 struct PromptArgs : AttentionArgs {
@@ -72,7 +73,11 @@ struct PromptPlan {
   static constexpr int kColumns = DP == 128 ? 512 : 256;  // of tensor memory
   static constexpr int kSlot = 2 * kKv;               // V of a step, K of one ahead
   static constexpr int kStages = DP == 128 ? 5 : 4;
-  static constexpr int kSmem = 2 * kQ + kStages * kSlot + 1024 + 512;
+  // barriers, and for heads of 64, whose threads have no register to spare, what a row
+  // keeps between the points where O is put away
+  static constexpr bool kKeptInSmem = DP == 64;
+  static constexpr int kSmem =
+      2 * kQ + kStages * kSlot + 1024 + 512 + (kKeptInSmem ? 256 * 8 : 0);
 };
 
 // True in one thread of the (converged) warp.  The compiler then knows that
@@ -428,8 +433,14 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     auto part_at = [&] {
       return blockIdx.y * (static_cast<int64_t>(a.batch) * a.q_heads * a.q_len) + lse_at();
     };
-    float m_kept = -INFINITY;  // the maximum in use when O was put away
-    auto kept_factor = [&] { return m_kept == m ? 1.0f : ex2((m_kept - m) * to_log2); };
+    // the maximum in use when O was put away, and the weights' sum then
+    float2 kept = make_float2(-INFINITY, 0.0f);
+    float2* const kept_at =
+        P::kKeptInSmem ? reinterpret_cast<float2*>(ring + kStages * P::kSlot + 512) + threadIdx.x
+                       : &kept;
+    auto kept_factor = [&](float m_kept) {
+      return m_kept == m ? 1.0f : ex2((m_kept - m) * to_log2);
+    };
 #pragma unroll 1
     for (int s = 0; ok && s < n;) {
       if (s > 0) {
@@ -441,7 +452,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
           break;
         }
         tc_fence_after();
-        const float factor = kept_factor();
+        const float2 before = s == kFold ? make_float2(m, 0.0f) : *kept_at;
+        const float factor = kept_factor(before.x);
         float4* to = reinterpret_cast<float4*>(a.part_o + part_at() * a.head_dim);
 #pragma unroll 1
         for (int c = 0; c < a.head_dim; c += 32, to += 8) {
@@ -462,7 +474,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
           }
         }
         __syncwarp();
-        m_kept = m;
+        *kept_at = make_float2(m, fmaf(before.y, factor, l));
+        l = 0.0f;
       }
       const int stop = min(n, s + kFold);
 #pragma unroll 1
@@ -612,6 +625,11 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
     }
     tc_fence_after();
     if (ok) {
+      float share_kept = 0.0f;  // what was put away counts by
+      if (n > kFold) {
+        share_kept = kept_factor(kept_at->x);
+        l = fmaf(kept_at->y, share_kept, l);
+      }
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const bool none = l == 0.0f;
       const float lse =
@@ -627,7 +645,6 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
                          static_cast<int64_t>(row) * a.o_stride[1] +
                          static_cast<int64_t>(h) * a.o_stride[2];
       float* part = a.part_o + part_at() * a.head_dim;  // splits > 1, or n > kFold
-      const float kept = n > kFold ? kept_factor() : 0.0f;
       // 32 columns at a time through the warp's share of the tile's Q (its MMAs
       // are done): a row's pieces are written side by side by neighbouring
       // threads, not by the one thread that holds the row.
@@ -667,7 +684,8 @@ __global__ void __launch_bounds__(kPromptThreads, PromptPlan<DP>::kBlocks)
               const float o[4] = {old.x, old.y, old.z, old.w};
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                acc[e + i] = __float_as_uint(fmaf(o[i], kept, __uint_as_float(acc[e + i])));
+                acc[e + i] =
+                    __float_as_uint(fmaf(o[i], share_kept, __uint_as_float(acc[e + i])));
               }
             }
           }

@@ -151,10 +151,11 @@ StepTiles step_tiles(const ie_attention_desc* d, const ie_attention_mask* m) {
     t.tiles = 1;
     // Two blocks for each SM; with ragged lengths three times as many, which
     // evens them out (4 or 10 times the SMs: within 5%, 16 times: 25% slower).
-    // Shares of at least 256 keys.
+    // Shares of at least 256 keys and, for the precision of their sums, 2^20 at most.
     const int64_t units = d->batch * d->kv_heads;
     const int64_t blocks = (m != nullptr && m->kv_lens != nullptr ? 6 : 2) * kSms;
-    const int64_t share = std::max<int64_t>(256, ceil_div(units * d->kv_len, blocks));
+    const int64_t share =
+        std::min<int64_t>(std::max<int64_t>(256, ceil_div(units * d->kv_len, blocks)), 1 << 20);
     t.splits = static_cast<int>(std::min<int64_t>(ceil_div(d->kv_len, share), kMaxSplits));
   } else {
     const int64_t documents = m == nullptr ? 0 : m->documents;

@@ -558,7 +558,9 @@ typedef struct ie_attention_desc {
 } ie_attention_desc;
 
 /* Scores, softmax and sums are fp32; the weights are rounded to the type of q, k and
- * v, half a step of each, before they are multiplied with v. */
+ * v, half a step of each, before they are multiplied with v.  Where the slower kernel
+ * takes documents or more than 16 rows (below), sums over more than 2^22 keys of equal
+ * weight lose about 2^-11. */
 
 /* Which keys a query sees; all pointers are device memory and may be NULL.
  *   kv_lens      [batch] keys of each sequence (0 .. kv_len), kv_len without it

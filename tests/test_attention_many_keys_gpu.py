@@ -129,3 +129,36 @@ def test_long_keys_under_masks(batch, sq, hq, hk, keys, dtype, options):
         both = joined(two, hq * d, hq * d).reshape(o.shape)
         # one rounding to bf16 apart, and the lo plane's own
         assert ((both - o.double()).abs() <= (2.0 ** -8 + 2.0 ** -16) * both.abs() + 2.0 ** -126).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("weight", [0.3, 0.7071])
+@pytest.mark.parametrize("sq, batch, document, keys", [
+    (20, 1, True, 1 << 26), (300, 1, True, 1 << 24), (1, 1, False, 1 << 26),
+    (1, 300, False, 1 << 20), (40, 80, False, 1 << 19)])
+def test_equal_weights_that_round(sq, batch, document, keys, weight, dtype):
+    """The first key's weight is 1 and its value 0, all others weigh the same and hold 1:
+    each addition to a long sum rounds the same way.  The scores' spread is exact to
+    2^-22, the weights' sum to 2^-12 (lse) and o to a few 2^-12 besides its rounding."""
+    import math
+    import torch
+    from computeengine_b200 import _lib as L
+    dt = getattr(torch, dtype)
+    scale = -math.log(weight)
+    v = torch.ones(batch, keys, 1, 8, dtype=dt, device="cuda")
+    k = torch.zeros_like(v)
+    k[:, 0, :, 0], v[:, 0] = 1, 0
+    q = torch.zeros(batch, sq, 1, 8, dtype=dt, device="cuda")
+    q[..., 0] = 1
+    o = torch.zeros_like(q)
+    lse = torch.zeros(batch, 1, sq, device="cuda")
+    m = attention_mask(L)
+    if document:
+        at = [torch.tensor([0, n], dtype=torch.int32, device="cuda") for n in (sq, keys)]
+        m = attention_mask(L, documents=1, q_offsets=at[0], kv_offsets=at[1])
+    run_attention(L, attention_desc(L, q, k, v, o, scale), m, q, k, v, o, lse)
+    assert L.take_device_error() == 0
+    total = 1 + (keys - 1) * math.exp(-scale)
+    assert (lse.double() - (math.log(total) + scale)).abs().max() <= 2.0 ** -12
+    want = (total - 1) / total
+    assert (o.double() - want).abs().max() <= HALF_STEP[dt] + 2.0 ** -11
