@@ -80,8 +80,8 @@ bool range_fits(const ie_group_norm_desc* d, int64_t g, int v) {
 // where that saves a larger cluster; narrower pieces waste part of each DRAM
 // access), cut into blocks of pixels of at most 32768 elements and half an SM's
 // shared memory, so that one block's loads cover another's arithmetic: 32
-// images of 56 x 56 x 256 fp32 take 59 us in clusters of 2, 70 us in clusters
-// of 8 and a quarter of the size.  Up to 8 blocks are a cluster; ranges too
+// images of 56 x 56 x 256 fp32 take 56 us in clusters of 2 (59 when clusters of
+// 8 and a quarter of the size, not timed since, took 70).  Up to 8 blocks are a cluster; ranges too
 // large for that take two kernels, 256 blocks an image at most.
 Plan plan_for(const ie_group_norm_desc* d, int v) {
   Plan p;
